@@ -42,7 +42,8 @@ from .verify import check_output
 
 WORKLOADS = {n: getattr(W, n) for n in (
     "qconv_stack_int8", "llama_mlp_int4", "mlp_fp32", "lstm_fp32", "attention_fp16", "matmul_nbits_f16",
-    "swish_mul_f16", "qlinear_matmul_u8", "matmul_integer_u8", "conv_f32", "softmax_f32", "quant_dequant")}
+    "swish_mul_f16", "qlinear_matmul_u8", "matmul_integer_u8", "conv_f32", "softmax_f32", "quant_dequant",
+    "norm_rope", "decoder_attention", "decoder_layer")}
 
 
 class CliError(Exception):
@@ -201,9 +202,10 @@ def _common(p):
     p.add_argument("--nbits-rounded-dequant", action="store_true",
                    help="MatMulNBits: one fp16 MMA per K slice on rounded dequantised weights (faster, "
                         "not bit-compatible with the reference's fp32 dequantisation)")
-    p.add_argument("--attention-mode", choices=["exact", "tensor"], default="exact",
-                   help="Attention: the reference's fp16 rounding bit for bit (exact), or tensor cores with "
-                        "fp32 accumulation for 128-wide heads (tensor)")
+    p.add_argument("--attention-mode", choices=["exact", "tensor", "flash"], default="exact",
+                   help="Attention: the reference's fp16 rounding bit for bit (exact), tensor cores with "
+                        "fp32 accumulation for 128-wide heads (tensor), or that for every head size up to 128 "
+                        "with masks, key counts and past keys (flash)")
 
 
 def build_parser() -> argparse.ArgumentParser:

@@ -1,0 +1,806 @@
+// ONNX Attention (opsets 23/24), fp16 in and out, for the forms a decoder
+// layer uses beside plain self-attention: queries and keys of different
+// lengths (cross attention), boolean and additive masks, valid key counts,
+// grouped key/value heads, head sizes up to 128, and a past that is one prefix
+// shared by the whole batch.  (attention.cu repeats the reference's fp16
+// rounding, attention_tc.cu is the unmasked 128-wide fast mode.)
+//
+// Mathematics: per query row, over its visible keys,
+//   o = sum_k 2^(x_k - m) v_k / sum_k 2^(x_k - m),   x_k = (scale q.k + mask_k) log2 e
+// evaluated online tile by tile: running reference m, sum l and output
+// accumulator are fp32 (TMEM for the latter); the weights are rounded to fp16
+// for the second matrix product (half an fp16 step each, 2^-11 relative: the
+// output type's own step) and the sum adds those same rounded weights.  A row
+// that sees no key gives 0.  An additive mask enters the exponent as
+// (mask log2 e - m) before the score is added, so scores keep their digits
+// beside masks as large as the type's lowest value.
+//
+// Rows: the query rows that read the same keys are packed into tiles of 128
+// whatever (token, head, sequence) they come from -- the group of query heads
+// of one key/value head, all tokens, and, against a shared prefix, all
+// sequences of the batch.  Against a shared prefix the prefix's K and V are so
+// read once for the batch instead of once per sequence.
+//
+// Key ranges: the past ("segment 1") and the current keys ("segment 0") are
+// separate work items, and each may be split further along the keys when there
+// are too few row tiles for the SMs.  With more than one item per row every
+// item writes its (m, l, o) in fp32 and attention_combine_kernel merges them:
+//   M = max m_s,  o = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s
+// in a fixed order, so results do not depend on timing.
+//
+// One CTA per work item, two per SM.  Warp 0: TMA producer of K and V tiles of
+// 64 keys.  Warp 1: S_j = Q K_j^T (tcgen05 kind::f16) into one of two TMEM
+// score buffers.  Warp 2: O += P_j V_j.  Warps 4-7: one thread per query row,
+// softmax and epilogue; a warp without rows leaves at once.  Every wait is
+// bounded (tc100.cuh).  Operand layouts in shared memory are the 128-byte
+// swizzle the TMA writes: Q and K as 64-wide slabs (K-major), P one such slab,
+// V as 64-wide slabs read MN-major.
+//
+// Boolean masks are first packed by mask_pack_kernel to one 64-bit word per
+// (mask row, 64 keys) plus each row's first and last visible key, so a row's
+// thread reads 8 aligned bytes per tile whatever the mask's alignment, and
+// tiles outside the rows' span (padding) are not read at all.  Keys past a
+// work item's last visible key inside its last tile have their V rows zeroed
+// in shared memory: what padding holds, NaN included, reaches no result.
+#include <cuda_fp16.h>
+
+#include "host_util.h"
+#include "kernels.h"
+#include "tc100.cuh"
+#include "tmem32.cuh"
+
+namespace emx {
+
+constexpr int AFK_M = 128;  // packed query rows per work item
+constexpr int AFK_N = 64;   // keys per tile
+constexpr int AFK_THREADS = 256;
+constexpr uint32_t AFK_QSLAB = AFK_M * 128u;  // 64 fp16 columns of the Q tile (and the P tile): 16 KB
+constexpr uint32_t AFK_KSLAB = AFK_N * 128u;  // 64 fp16 columns of a K or V tile: 8 KB
+constexpr uint32_t AFK_TMEM_COLS = 256;       // scores at columns 0 and 64, output at 128
+constexpr uint32_t AFK_O_COL = 128;
+constexpr float AFK_RESCALE = 8.0f;  // the output is rescaled when a row's maximum grows by more (log2 units)
+constexpr float AFK_LOG2E = 1.4426950408889634f;
+
+enum { MASK_NONE = 0, MASK_BITS = 1, MASK_ADD = 2 };  // kernel variants
+
+struct FlashSegment {
+  CUtensorMap map_k, map_v;  // 4-D (d, key, head, batch), box (64, 64, 1, 1), 128-byte swizzle
+  int keys;                  // keys of the segment
+  int mask_off;              // first key's position in a mask row (elements)
+  int word_off;              // first word of the segment in a packed mask row
+  int shared;                // one copy for every sequence
+  int splits;                // work items along the keys
+  int tiles;                 // row tiles per (batch or all, key/value head)
+  int part0;                 // first partial slot
+  int limited;               // causal and valid-count limits apply (the current keys)
+};
+
+struct FlashParams {
+  FlashSegment seg[2];
+  int first1;  // CTAs below run segment 1 (the longer, shared one first), from here on segment 0
+  const uint16_t* q;
+  uint16_t* o;
+  float* part_o;   // [slot][row][DV], null: one item per row, written to o
+  float2* part_ml; // [slot][row] (m, l)
+  int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
+  int B, HQ, HKV, group, TQ, D, DV, causal;
+  const long long* counts;  // valid keys of each sequence, or null
+  // mask rows: (b * mask_sb + h * mask_sh + t * mask_st)
+  int64_t mask_sb, mask_sh, mask_st;
+  const unsigned long long* bits;  // packed boolean mask [row][words]
+  const int4* spans;               // per mask row: first and end visible key of segments 0 and 1
+  const void* add;                 // additive mask [row][mask_len]
+  int words, mask_len, add_f32, add_vec;
+  float scale_log2;
+  int* err;
+};
+
+struct RowId {
+  int b, h, t;
+};
+
+__device__ __forceinline__ RowId row_of(const FlashParams& p, int r, int kvh, int b, bool shared) {
+  const int g = r % p.group, bt = r / p.group;
+  RowId id;
+  id.h = kvh * p.group + g;
+  id.b = shared ? bt / p.TQ : b;
+  id.t = shared ? bt - id.b * p.TQ : bt;
+  return id;
+}
+
+__device__ __forceinline__ float mask_value(const FlashParams& p, int64_t at) {
+  if (p.add_f32) {
+    // Finite entries beyond 2^24 count as 2^24: no score reaches across that, and the differences formed
+    // below stay finite.  -inf (and NaN) stay.
+    const float v = __ldg(static_cast<const float*>(p.add) + at);
+    return v > 0x1p24f ? 0x1p24f : (v < -0x1p24f && v > -INFINITY ? -0x1p24f : v);
+  }
+  return __half2float(__ldg(static_cast<const __half*>(p.add) + at));
+}
+
+template <int NS, int MASK>
+__global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const __grid_constant__ FlashParams p) {
+  constexpr uint32_t QTILE = NS * AFK_QSLAB, KTILE = NS * AFK_KSLAB;
+  constexpr int ST = NS == 1 ? 4 : 2;  // K and V stages: 64 KB of loads in flight per CTA at either head size
+  extern __shared__ __align__(1024) uint8_t afk_raw[];
+  if (smem_u32(afk_raw) & 1023u) {  // the swizzled operands need a 1 KB aligned window
+    if (threadIdx.x == 0) record_error(p.err, DEV_BAD_CONFIG);
+    return;
+  }
+  uint8_t* s_q = afk_raw;
+  uint8_t* s_k = s_q + QTILE;
+  uint8_t* s_v = s_k + ST * KTILE;
+  uint8_t* s_p = s_v + ST * KTILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_p + AFK_QSLAB);
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = bars + ST;
+  uint64_t* v_full = bars + 2 * ST;
+  uint64_t* v_empty = bars + 3 * ST;
+  uint64_t* s_full = bars + 4 * ST;
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* p_full = s_full + 4;
+  uint64_t* o_done = s_full + 5;
+  uint64_t* drain = s_full + 6;  // [2]
+  uint32_t* holder = reinterpret_cast<uint32_t*>(s_full + 8);
+  int* span = reinterpret_cast<int*>(holder + 1);  // [2] first and end key of the work item's rows
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* const err = p.err;
+
+  // ---------------- work item
+  const int si = (int)blockIdx.x < p.first1 ? 1 : 0;
+  const FlashSegment& sg = p.seg[si];
+  int id = (int)blockIdx.x - (si ? 0 : p.first1);
+  const int split = id % sg.splits;
+  id /= sg.splits;
+  const int tile = sg.tiles - 1 - id % sg.tiles;  // later tokens, which see more keys, first
+  id /= sg.tiles;
+  const int kvh = id % p.HKV;
+  const int b = id / p.HKV;  // 0 for a shared segment
+  const bool shared = sg.shared != 0;
+  const int rows_all = p.TQ * p.group * (shared ? p.B : 1);
+  const int row0 = tile * AFK_M;
+  const int rows = min(AFK_M, rows_all - row0);
+  const int nact = (rows + 31) >> 5;  // softmax warps with rows
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_empty[s], (uint32_t)nact);
+      mbar_init(&drain[s], 1);
+    }
+    mbar_init(p_full, (uint32_t)nact);
+    mbar_init(o_done, 1);
+    fence_barrier_init();
+    span[0] = 0x7fffffff;
+    span[1] = 0;
+  }
+  if (warp == 1) {
+    tmem_alloc(holder, AFK_TMEM_COLS);
+    tmem_relinquish();
+  }
+  pdl_wait();  // Q, K, V, masks and counts may come from the preceding kernel
+  pdl_launch_dependents();
+
+  // ---------------- Q tile, zero past the head size and the rows
+  for (int i = threadIdx.x; i < AFK_M * NS * 8; i += AFK_THREADS) {
+    const int c = i % (NS * 8), r = i / (NS * 8);
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (r < rows && c * 8 < p.D) {
+      const RowId w = row_of(p, row0 + r, kvh, b, shared);
+      v = *reinterpret_cast<const uint4*>(p.q + (int64_t)w.b * p.q_sb + (int64_t)w.h * p.q_sh + (int64_t)w.t * p.q_st +
+                                          c * 8);
+    }
+    *reinterpret_cast<uint4*>(s_q + (c >> 3) * AFK_QSLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+  }
+  fence_async_shared();
+
+  // ---------------- keys that some row of the work item sees
+  int kbeg = 0, kend = sg.keys;
+  if (sg.limited) {
+    if (p.causal) kend = min(kend, (row0 + rows - 1) / p.group + 1);  // segment 0 is never shared
+    if (p.counts) {
+      const long long n = p.counts[b];
+      if (n < 0 || n > sg.keys) record_error(err, DEV_BAD_INDEX);
+      kend = min(kend, (int)max(0ll, min(n, (long long)sg.keys)));
+    }
+  }
+  const int row_keys = kend;  // before the mask's span: the count limit of every row
+  __syncthreads();            // span initialised
+  if (MASK == MASK_BITS) {
+    if (threadIdx.x < rows) {
+      const RowId w = row_of(p, row0 + threadIdx.x, kvh, b, shared);
+      const int4 v = p.spans[w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st];
+      const int lo = si ? v.z : v.x, hi = si ? v.w : v.y;
+      if (lo < hi) {
+        atomicMin(&span[0], lo);
+        atomicMax(&span[1], hi);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *holder;
+  if (MASK == MASK_BITS) {
+    kbeg = span[0];
+    kend = min(kend, span[1]);
+  }
+  // this split's share of the 64-key tiles
+  const int j_lo = kbeg < kend ? kbeg / AFK_N : 0, j_hi = kbeg < kend ? (kend + AFK_N - 1) / AFK_N : 0;
+  const int per = j_hi - j_lo;
+  const int j0 = j_lo + (int)((long long)per * split / sg.splits);
+  const int J = j_lo + (int)((long long)per * (split + 1) / sg.splits) - j0;
+
+  if (warp == 0) {
+    if (lane == 0 && J > 0) {
+      // ---------------- producer
+      const int kb = shared ? 0 : b;
+      bool ok = true;
+      int issued = 0;
+      for (int j = 0; j < J && ok; ++j) {
+        const int s = j % ST, key0 = (j0 + j) * AFK_N;
+        const uint32_t ph = (uint32_t)(j / ST - 1) & 1u;
+        if (j >= ST && !mbar_wait(&k_empty[s], ph, err, DEV_TIMEOUT_PRODUCER)) ok = false;
+        if (!ok) break;
+        mbar_arrive_expect_tx(&k_full[s], KTILE);
+#pragma unroll
+        for (int c = 0; c < NS; ++c)
+          tma_load_4d(s_k + s * KTILE + c * AFK_KSLAB, &sg.map_k, &k_full[s], 64 * c, key0, kvh, kb);
+        issued = 2 * j + 1;
+        if (j >= ST && !mbar_wait(&v_empty[s], ph, err, DEV_TIMEOUT_PRODUCER)) ok = false;
+        if (!ok) break;
+        mbar_arrive_expect_tx(&v_full[s], KTILE);
+#pragma unroll
+        for (int c = 0; c < NS; ++c)
+          tma_load_4d(s_v + s * KTILE + c * AFK_KSLAB, &sg.map_v, &v_full[s], 64 * c, key0, kvh, kb);
+        issued = 2 * j + 2;
+      }
+      if (!ok) {  // error path: let the copies in flight land before the CTA exits
+        for (int i = max(0, issued - 2 * ST); i < issued; ++i) {
+          const int j = i >> 1;
+          (void)mbar_wait((i & 1) ? &v_full[j % ST] : &k_full[j % ST], (uint32_t)(j / ST) & 1u, nullptr, 0);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && J > 0) {
+      // ---------------- S issuer
+      const uint32_t idesc = make_idesc(1u, 0u, 0u, AFK_M, AFK_N);
+      const int nks = (p.D + 15) / 16;
+      for (int j = 0; j < J; ++j) {
+        const int s = j % ST, sb = j & 1;
+        if (!mbar_wait(&k_full[s], (uint32_t)(j / ST) & 1u, err, DEV_TIMEOUT_MMA)) break;
+        if (j >= 2 && !mbar_wait(&s_empty[sb], (uint32_t)((j >> 1) - 1) & 1u, err, DEV_TIMEOUT_MMA)) break;
+        tc_fence_after();
+        const uint32_t qa = smem_u32(s_q), kb = smem_u32(s_k + s * KTILE);
+        for (int ks = 0; ks < nks; ++ks) {
+          const uint32_t qoff = (uint32_t)(ks >> 2) * AFK_QSLAB + (uint32_t)(ks & 3) * 32u;
+          const uint32_t koff = (uint32_t)(ks >> 2) * AFK_KSLAB + (uint32_t)(ks & 3) * 32u;
+          mma_f16(tmem + (uint32_t)(sb * AFK_N), smem_desc_k_sw128(qa + qoff, 1024), smem_desc_k_sw128(kb + koff, 1024),
+                  idesc, ks > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[sb]);
+        tc_commit(&k_empty[s]);
+      }
+      // every MMA this thread issued completes before TMEM is released
+      tc_commit(&drain[0]);
+      (void)mbar_wait(&drain[0], 0, nullptr, 0);
+    }
+  } else if (warp == 2) {
+    if (J > 0) {
+      // ---------------- P.V issuer (all lanes wait; lane 0 issues)
+      const uint32_t idesc = make_idesc(1u, 0u, 0u, AFK_M, (uint32_t)((p.DV + 15) & ~15)) | (1u << 16);
+      for (int j = 0; j < J; ++j) {
+        const int s = j % ST;
+        bool ok = mbar_wait(&v_full[s], (uint32_t)(j / ST) & 1u, err, DEV_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const int nv = kend - (j0 + j) * AFK_N;
+        if (nv < AFK_N) {  // keys past the last visible one: their values take no part
+          for (int i = lane; i < (AFK_N - nv) * 8 * NS; i += 32) {
+            const int c = i % (8 * NS), r = nv + i / (8 * NS);
+            *reinterpret_cast<uint4*>(s_v + s * KTILE + (c >> 3) * AFK_KSLAB + r * 128 + (c & 7) * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_shared();
+          __syncwarp();
+        }
+        ok = mbar_wait(p_full, (uint32_t)j & 1u, err, DEV_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint32_t pa = smem_u32(s_p), vb = smem_u32(s_v + s * KTILE);
+#pragma unroll
+          for (int kk = 0; kk < AFK_N / 16; ++kk)
+            mma_f16(tmem + AFK_O_COL, smem_desc_k_sw128(pa + (uint32_t)kk * 32u, 1024),
+                    smem_desc_mn_sw128(vb + (uint32_t)kk * 16u * 128u, AFK_KSLAB, 1024u), idesc,
+                    (j > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(o_done);
+          tc_commit(&v_empty[s]);
+        }
+        __syncwarp();
+      }
+      if (lane == 0) {
+        tc_commit(&drain[1]);
+        (void)mbar_wait(&drain[1], 0, nullptr, 0);
+      }
+    }
+  } else if (warp >= 4 && warp - 4 < nact) {
+    // ---------------- softmax and epilogue: thread = query row (warp % 4 = TMEM lane quarter)
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const bool live = r < rows;
+    const RowId w = row_of(p, row0 + (live ? r : 0), kvh, b, shared);
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    int row_end = row_keys;  // end of the keys this row may see
+    if (sg.limited && p.causal) row_end = min(row_end, w.t + 1);
+    const int64_t mrow = MASK == MASK_NONE ? 0 : w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st;
+    float m_used = -INFINITY;  // reference of the exponentials, log2 units
+    float l = 0.0f;            // sum of the fp16-rounded weights
+    const float sc = p.scale_log2;
+    const bool pos = sc > 0.0f;
+    bool ok = true;
+    for (int j = 0; j < J && ok; ++j) {
+      const int sb = j & 1, key0 = (j0 + j) * AFK_N;
+      // visible keys of the tile, one bit each
+      unsigned long long vis = ~0ull;
+      if (row_end - key0 < AFK_N) vis = row_end > key0 ? (1ull << (row_end - key0)) - 1 : 0ull;
+      if (MASK == MASK_BITS) vis &= p.bits[mrow * p.words + sg.word_off + (j0 + j)];
+      if (MASK == MASK_ADD) {  // keys past a short mask are not seen
+        const int left = p.mask_len - sg.mask_off - key0;
+        if (left < AFK_N) vis &= left > 0 ? (1ull << left) - 1 : 0ull;
+      }
+      ok = mbar_wait(&s_full[sb], (uint32_t)(j >> 1) & 1u, err, DEV_TIMEOUT_EPILOGUE);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t sv[2][32];
+      tmem_ld32(tmem + lane_base + (uint32_t)(sb * AFK_N), sv[0]);
+      tmem_ld32(tmem + lane_base + (uint32_t)(sb * AFK_N + 32), sv[1]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[sb]);
+      if (!pos) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sv[c][i] = __float_as_uint(__uint_as_float(sv[c][i]) * sc);
+      }
+      const float mul = pos ? sc : 1.0f;
+      // keys the row does not see become -inf; tiles every row of the warp sees whole skip the test
+      if (!__all_sync(0xffffffffu, vis == ~0ull)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(half & (1u << i))) sv[c][i] = 0xff800000u;
+        }
+      }
+      float mx;
+      if (MASK == MASK_ADD) {
+        // pass 1: -inf mask entries hide their key; the maximum of the masked scores (any value near it will do)
+        const int64_t at = mrow * p.mask_len + sg.mask_off + key0;
+        mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float mk[8];
+            if (p.add_vec && half == ~0u) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.add) + at + 32 * c + i));
+              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vw[e]));
+                mk[2 * e] = f.x;
+                mk[2 * e + 1] = f.y;
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) mk[e] = (half & (1u << (i + e))) ? mask_value(p, at + 32 * c + i + e) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (mk[e] == -INFINITY) sv[c][i + e] = 0xff800000u;
+              else mx = fmaxf(mx, fmaf(__uint_as_float(sv[c][i + e]), mul, mk[e] * AFK_LOG2E));
+            }
+          }
+        }
+      } else {
+        float mxp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mxp[i & 3] = fmaxf(mxp[i & 3], __uint_as_float(sv[c][i]));
+        mx = fmaxf(fmaxf(mxp[0], mxp[1]), fmaxf(mxp[2], mxp[3])) * mul;
+      }
+      float m_new = m_used;
+      bool rescale = false;
+      if (mx > m_used + AFK_RESCALE || m_used == -INFINITY) {
+        m_new = mx;
+        rescale = j > 0 && m_used != -INFINITY;
+      }
+      const float alpha = rescale ? ex2_approx(m_used - m_new) : 1.0f;
+      const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
+      uint32_t pw[2][16];
+      float lp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (MASK == MASK_ADD) {
+        const int64_t at = mrow * p.mask_len + sg.mask_off + key0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float mk[8];
+            if (p.add_vec && half == ~0u) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.add) + at + 32 * c + i));
+              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vw[e]));
+                mk[2 * e] = f.x;
+                mk[2 * e + 1] = f.y;
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) mk[e] = (half & (1u << (i + e))) ? mask_value(p, at + 32 * c + i + e) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              // a hidden key's score is -inf; its mask entry must not turn that into NaN
+              const float mm = mk[e] == -INFINITY ? neg_m : fmaf(mk[e], AFK_LOG2E, neg_m);
+              sv[c][i + e] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(sv[c][i + e]), mul, mm)));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+              pw[c][(i + e) >> 1] = pack_f16x2(__uint_as_float(sv[c][i + e]), __uint_as_float(sv[c][i + e + 1]));
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            lp[i & 3] = add_f16((uint16_t)(pw[c][i] >> 16), add_f16((uint16_t)pw[c][i], lp[i & 3]));
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e0 = ex2_approx(fmaf(__uint_as_float(sv[c][2 * i]), mul, neg_m));
+            const float e1 = ex2_approx(fmaf(__uint_as_float(sv[c][2 * i + 1]), mul, neg_m));
+            pw[c][i] = pack_f16x2(e0, e1);
+            lp[i & 3] = add_f16((uint16_t)(pw[c][i] >> 16), add_f16((uint16_t)pw[c][i], lp[i & 3]));
+          }
+      }
+      l = l * alpha + ((lp[0] + lp[1]) + (lp[2] + lp[3]));
+      m_used = m_new;
+      // P_{j-1} V_{j-1} must be done before P is overwritten and O rescaled
+      if (j > 0) {
+        ok = mbar_wait(o_done, (uint32_t)(j - 1) & 1u, err, DEV_TIMEOUT_EPILOGUE);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+          for (int c = 0; c < 2 * NS; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tmem + lane_base + AFK_O_COL + 32u * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(tmem + lane_base + AFK_O_COL + 32u * c, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      // P row r: keys 8g .. 8g+7 are 16-byte chunk g of the row, swizzled by the row
+#pragma unroll
+      for (int g = 0; g < AFK_N / 8; ++g) {
+        const int c = g >> 2, i = (g & 3) * 4;
+        *reinterpret_cast<uint4*>(s_p + r * 128 + ((g ^ (r & 7)) << 4)) =
+            make_uint4(pw[c][i], pw[c][i + 1], pw[c][i + 2], pw[c][i + 3]);
+      }
+      fence_async_shared();  // the generic writes of P become visible to the tensor cores
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+    }
+    // ---------------- epilogue
+    if (ok && J > 0) {
+      ok = mbar_wait(o_done, (uint32_t)(J - 1) & 1u, err, DEV_TIMEOUT_EPILOGUE);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (ok) {
+      tc_fence_after();
+      const bool part = p.part_o != nullptr;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int64_t row = ((int64_t)w.b * p.TQ + w.t) * p.HQ + w.h;
+      const int64_t slot_row = (int64_t)(sg.part0 + split) * ((int64_t)p.B * p.TQ * p.HQ) + row;
+      uint16_t* orow = p.o + (int64_t)w.b * p.o_sb + (int64_t)w.h * p.o_sh + (int64_t)w.t * p.o_st;
+      float* prow = part ? p.part_o + slot_row * p.DV : nullptr;
+      if (part && live) p.part_ml[slot_row] = make_float2(m_used, l);
+      if (!(part && J == 0)) {  // the merge does not read the output of an item with l = 0
+#pragma unroll
+        for (int c = 0; c < 2 * NS; ++c) {
+          uint32_t o[32];
+          if (J > 0) {
+            tmem_ld32(tmem + lane_base + AFK_O_COL + 32u * c, o);
+            tmem_wait_ld();
+          }
+          if (l == 0.0f) {  // a row that sees no key gives 0 whatever the values hold
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              if (32 * c + i >= p.DV) continue;
+              if (part) {
+                *reinterpret_cast<uint4*>(prow + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                *reinterpret_cast<uint4*>(prow + 32 * c + i + 4) = make_uint4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
+              } else {
+                uint4 v;
+                v.x = pack_f16x2(__uint_as_float(o[i + 0]) * inv, __uint_as_float(o[i + 1]) * inv);
+                v.y = pack_f16x2(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                v.z = pack_f16x2(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                v.w = pack_f16x2(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                *reinterpret_cast<uint4*>(orow + 32 * c + i) = v;
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, AFK_TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ merging split key ranges
+// One warp per query row, DV / 4 lanes with four columns each; slots in order.
+__global__ void __launch_bounds__(256) attention_combine_kernel(const float* __restrict__ part_o,
+                                                                const float2* __restrict__ part_ml, int slots,
+                                                                int64_t rows, int TQ, int HQ, int DV,
+                                                                uint16_t* __restrict__ o, int64_t o_sb, int64_t o_sh,
+                                                                int64_t o_st) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  float m = -INFINITY;
+  for (int s = lane; s < slots; s += 32) {
+    const float2 ml = part_ml[(int64_t)s * rows + row];
+    if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float l = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < slots; ++s) {
+    const float2 ml = part_ml[(int64_t)s * rows + row];
+    if (ml.y == 0.0f) continue;  // this item saw no key of the row (its output is not written)
+    const float wgt = ex2_approx(ml.x - m);
+    l += wgt * ml.y;
+    if (lane * 4 < DV) {
+      const float4 v = *reinterpret_cast<const float4*>(part_o + ((int64_t)s * rows + row) * DV + lane * 4);
+      acc.x += wgt * v.x;
+      acc.y += wgt * v.y;
+      acc.z += wgt * v.z;
+      acc.w += wgt * v.w;
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (lane * 4 < DV) {
+    const int h = (int)(row % HQ);
+    const int64_t bt = row / HQ;
+    uint16_t* y = o + (bt / TQ) * o_sb + h * o_sh + (bt % TQ) * o_st + lane * 4;
+    *reinterpret_cast<uint2*>(y) = make_uint2(pack_f16x2(acc.x * inv, acc.y * inv), pack_f16x2(acc.z * inv, acc.w * inv));
+  }
+}
+
+// ------------------------------------------------------------------ packing boolean masks
+// One CTA per mask row of `len` bytes (key k: past keys first); words of segment
+// 1 (the past) come first, then those of segment 0, each segment from a fresh word.
+__global__ void __launch_bounds__(256) mask_pack_kernel(const uint8_t* __restrict__ mask, int len, int past, int keys,
+                                                        int words1, int words,
+                                                        unsigned long long* __restrict__ bits, int4* __restrict__ spans) {
+  __shared__ int s_span[4];  // first and end of segment 0, first and end of segment 1
+  pdl_wait();
+  pdl_launch_dependents();
+  if (threadIdx.x < 4) s_span[threadIdx.x] = threadIdx.x & 1 ? 0 : 0x7fffffff;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x;
+  const uint8_t* src = mask + row * len;
+  int lo[2] = {0x7fffffff, 0x7fffffff}, hi[2] = {0, 0};
+#pragma unroll 4
+  for (int wd = warp; wd < words; wd += 8) {
+    const int seg = wd < words1 ? 1 : 0;
+    const int k0 = (seg ? wd : wd - words1) * 64;         // within the segment
+    const int n = seg ? past : keys, base = seg ? 0 : past;
+    const int ka = k0 + lane, kb = ka + 32;
+    const bool va = ka < n && base + ka < len && src[base + ka] != 0;
+    const bool vb = kb < n && base + kb < len && src[base + kb] != 0;
+    const uint32_t wa = __ballot_sync(0xffffffffu, va), wb = __ballot_sync(0xffffffffu, vb);
+    const unsigned long long w = (unsigned long long)wa | ((unsigned long long)wb << 32);
+    if (lane == 0) bits[row * words + wd] = w;
+    if (w) {
+      lo[seg] = min(lo[seg], k0 + __ffsll((long long)w) - 1);
+      hi[seg] = max(hi[seg], k0 + 64 - __clzll((long long)w));
+    }
+  }
+  if (lane < 2 && hi[lane]) {
+    atomicMin(&s_span[2 * lane], lo[lane]);
+    atomicMax(&s_span[2 * lane + 1], hi[lane]);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) spans[row] = make_int4(s_span[0], s_span[1], s_span[2], s_span[3]);
+}
+
+// ------------------------------------------------------------------ host side
+static size_t flash_smem(int ns) {
+  const int st = ns == 1 ? 4 : 2;
+  return (size_t)ns * AFK_QSLAB + 2 * (size_t)st * ns * AFK_KSLAB + AFK_QSLAB + 256;
+}
+
+typedef void (*FlashKernel)(const FlashParams);
+
+static FlashKernel flash_kernel(int ns, int mask) {
+  static const FlashKernel table[2][3] = {
+      {attention_flash_kernel<1, MASK_NONE>, attention_flash_kernel<1, MASK_BITS>, attention_flash_kernel<1, MASK_ADD>},
+      {attention_flash_kernel<2, MASK_NONE>, attention_flash_kernel<2, MASK_BITS>, attention_flash_kernel<2, MASK_ADD>}};
+  return table[ns - 1][mask];
+}
+
+static int flash_slabs(const PlanOp& op) {
+  return (op.ip[AF_D] > op.ip[AF_DV] ? op.ip[AF_D] : op.ip[AF_DV]) > 64 ? 2 : 1;
+}
+
+int prepare_attention_flash(const PlanOp& op, void* const*, OpState*, int, char* msg, size_t n) {
+  const int64_t d = op.ip[AF_D], dv = op.ip[AF_DV];
+  if (d < 8 || d > 128 || d % 8 || dv < 8 || dv > 128 || dv % 8)
+    return fail(msg, n, 5, "Attention: head sizes %lld/%lld, needs multiples of 8 up to 128", (long long)d, (long long)dv);
+  for (int s = AF_Q_SB; s <= AF_O_ST; ++s)
+    if (op.ip[s] % 8) return fail(msg, n, 5, "Attention: strides must be 16-byte multiples");
+  for (int ns = 1; ns <= 2; ++ns)
+    for (int m = 0; m < 3; ++m) {
+      cudaError_t e =
+          cudaFuncSetAttribute(flash_kernel(ns, m), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)flash_smem(ns));
+      if (e != cudaSuccess) return fail(msg, n, 4, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    }
+  return 0;
+}
+
+// 4-D map (d, t, h, b) over an fp16 tensor with element strides (1, st, sh, sb),
+// boxes of 64 d x 64 tokens.
+static int make_tmap_kv(CUtensorMap* map, const void* base, int64_t d, int64_t t, int64_t heads, int64_t batch,
+                        int64_t st, int64_t sh, int64_t sb) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc || ((uintptr_t)base & 15u)) return 5;
+  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)t, (cuuint64_t)heads, (cuuint64_t)batch};
+  cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)AFK_N, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 4;
+}
+
+int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, const LaunchCtx& ctx, int* launches) {
+  FlashParams p{};
+  const int64_t* s = &op.ip[AF_Q_SB];
+  auto ptr = [&](int i) -> void* { return op.t[i] >= 0 ? ptrs[op.t[i]] : nullptr; };
+  p.B = (int)eff_batch(ctx, op, op.ip[AF_B]);
+  p.HQ = (int)op.ip[AF_HQ];
+  p.HKV = (int)op.ip[AF_HKV];
+  p.group = p.HQ / p.HKV;
+  p.TQ = (int)op.ip[AF_TQ];
+  p.D = (int)op.ip[AF_D];
+  p.DV = (int)op.ip[AF_DV];
+  p.causal = (int)op.ip[AF_CAUSAL];
+  p.scale_log2 = (float)(op.fp[AFF_SCALE] * 1.4426950408889634);
+  p.q = (const uint16_t*)ptr(0);
+  p.o = (uint16_t*)ptr(3);
+  p.q_sb = s[0], p.q_sh = s[1], p.q_st = s[2];
+  p.o_sb = s[9], p.o_sh = s[10], p.o_st = s[11];
+  p.err = ctx.d_error;
+  if (p.B <= 0 || p.TQ <= 0) return 0;
+  if (((uintptr_t)p.q | (uintptr_t)p.o) & 15u) return 5;
+  if ((uintptr_t)ptr(7) & 7u) return 5;
+  const int tk = (int)op.ip[AF_TK], tp = (int)op.ip[AF_TP];
+  const int64_t rows = (int64_t)p.B * p.TQ * p.HQ;
+
+  FlashSegment& cur = p.seg[0];
+  cur.keys = tk;
+  cur.mask_off = tp;
+  cur.shared = 0;
+  cur.limited = 1;
+  cur.splits = (int)op.ip[AF_SPLITS_K];
+  cur.tiles = (p.TQ * p.group + AFK_M - 1) / AFK_M;
+  cur.part0 = 0;
+  int rc = make_tmap_kv(&cur.map_k, ptr(1), p.D, tk, p.HKV, p.B, s[5], s[4], s[3]);
+  if (!rc) rc = make_tmap_kv(&cur.map_v, ptr(2), p.DV, tk, p.HKV, p.B, s[8], s[7], s[6]);
+  int64_t items = (int64_t)p.B * p.HKV * cur.tiles * cur.splits;
+  int slots = cur.splits;
+  FlashSegment& past = p.seg[1];
+  if (tp > 0 && !rc) {
+    past.keys = tp;
+    past.shared = (int)op.ip[AF_PAST_SHARED];
+    past.splits = (int)op.ip[AF_SPLITS_P];
+    const int64_t packed = (int64_t)p.TQ * p.group * (past.shared ? p.B : 1);
+    past.tiles = (int)((packed + AFK_M - 1) / AFK_M);
+    past.part0 = cur.splits;
+    const int copies = past.shared ? 1 : p.B;
+    rc = make_tmap_kv(&past.map_k, ptr(5), p.D, tp, p.HKV, copies, p.D, (int64_t)tp * p.D, (int64_t)p.HKV * tp * p.D);
+    if (!rc)
+      rc = make_tmap_kv(&past.map_v, ptr(6), p.DV, tp, p.HKV, copies, p.DV, (int64_t)tp * p.DV,
+                        (int64_t)p.HKV * tp * p.DV);
+    p.first1 = copies * p.HKV * past.tiles * past.splits;
+    items += p.first1;
+    slots += past.splits;
+  }
+  if (rc) return rc;
+  if (items > 0x7fffffff) return 5;
+  if (slots > 1) {
+    // (m, l) pairs behind the outputs, both sized for the compiled batch
+    p.part_o = (float*)ptr(8);
+    p.part_ml = (float2*)(p.part_o + (int64_t)slots * rows * p.DV);
+  }
+  p.counts = (const long long*)ptr(7);
+  int variant = MASK_NONE;
+  const int kind = (int)op.ip[AF_MASK_KIND];
+  p.mask_sb = op.ip[AF_MASK_SB], p.mask_sh = op.ip[AF_MASK_SH], p.mask_st = op.ip[AF_MASK_ST];
+  p.mask_len = (int)op.ip[AF_MASK_LEN];
+  if (kind == AF_MASK_BOOL) {
+    variant = MASK_BITS;
+    const int words1 = (tp + 63) / 64, words = words1 + (tk + 63) / 64;
+    const int64_t mrows = p.mask_sb ? p.mask_sb * p.B : op.ip[AF_MASK_ROWS];
+    cur.word_off = words1;
+    p.words = words;
+    p.spans = (const int4*)ptr(9);
+    p.bits = (const unsigned long long*)(p.spans + mrows);
+    cudaError_t e = launch_pdl(mask_pack_kernel, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, (const uint8_t*)ptr(4),
+                               p.mask_len, tp, tk, words1, words, (unsigned long long*)p.bits, (int4*)p.spans);
+    ++*launches;
+    if (e != cudaSuccess) return 4;
+  } else if (kind != AF_MASK_NONE) {
+    variant = MASK_ADD;
+    p.add = ptr(4);
+    p.add_f32 = kind == AF_MASK_F32;
+    if ((uintptr_t)p.add & (p.add_f32 ? 3u : 1u)) return 5;
+    // 16-byte reads of 8 fp16 entries: every row and both segments start on 16 bytes
+    p.add_vec = kind == AF_MASK_F16 && p.mask_len % 8 == 0 && tp % 8 == 0 && ((uintptr_t)p.add & 15u) == 0;
+  }
+  const int ns = flash_slabs(op);
+  cudaError_t e = launch_pdl(flash_kernel(ns, variant), dim3((unsigned)items), dim3(AFK_THREADS), flash_smem(ns),
+                             ctx.stream, p);
+  ++*launches;
+  if (e == cudaSuccess && slots > 1) {
+    e = launch_pdl(attention_combine_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx.stream,
+                   (const float*)p.part_o, (const float2*)p.part_ml, slots, rows, p.TQ, p.HQ, p.DV, p.o, p.o_sb, p.o_sh,
+                   p.o_st);
+    ++*launches;
+  }
+  return e == cudaSuccess ? 0 : 4;
+}
+
+}  // namespace emx

@@ -36,6 +36,9 @@ enum KernelId : uint32_t {
   K_QLINEAR_AVGPOOL = 23,  // com.microsoft QLinearAveragePool, 2-D NCHW, 8-bit
   K_QLINEAR_SOFTMAX = 24,  // com.microsoft QLinearSoftmax, 8-bit
   K_NBITS_I8 = 25,         // MatMulNBits accuracy_level 4: int8 activations, exact block sums (nbits_i8.cu)
+  K_ATTENTION_FLASH = 26,  // Attention with masks, counts, a past and grouped heads: tcgen05 kind::f16 (attention_flash.cu)
+  K_RMS_NORM = 27,         // opset-23 RMSNormalization over the trailing axes (norm_rope.cu)
+  K_NORM_ROPE = 28,        // opset-23 RotaryEmbedding of one or two tensors, each optionally RMS-normalised first
 };
 
 // Chunk-planar zero-bordered layout ("planar" below): [C/16][rows][16 bytes],
@@ -96,6 +99,34 @@ enum {
   AT_Q_SB, AT_Q_SH, AT_Q_ST, AT_K_SB, AT_K_SH, AT_K_ST, AT_V_SB, AT_V_SH, AT_V_ST, AT_O_SB, AT_O_SH, AT_O_ST
 };
 enum { ATF_SCALE };
+
+// ---- K_ATTENTION_FLASH: t[0]=Q, t[1]=K, t[2]=V, t[3]=Y (fp16), t[4]=mask|-1, t[5]=past K|-1, t[6]=past V|-1,
+//      t[7]=valid key counts i64 [B]|-1, t[8]=partial results f32|-1 (slots x rows x (DV + 2), slots = AF_SPLITS_K +
+//      AF_SPLITS_P, rows = B*TQ*HQ), t[9]=packed boolean mask|-1 (16 bytes per mask row, then 8 per 64 keys of each
+//      segment).  Element (b, h, t, d) of Q, K, V, Y sits at b*SB + h*SH + t*ST + d; the past is contiguous
+//      [B or 1][HKV][TP][D].  Mask row of query (b, h, t): b*SB + h*SH + t*ST, each of AF_MASK_LEN keys, past first.
+enum {
+  AF_B, AF_HQ, AF_HKV, AF_TQ, AF_TK, AF_TP, AF_D, AF_DV, AF_CAUSAL,
+  AF_Q_SB, AF_Q_SH, AF_Q_ST, AF_K_SB, AF_K_SH, AF_K_ST, AF_V_SB, AF_V_SH, AF_V_ST, AF_O_SB, AF_O_SH, AF_O_ST,
+  AF_PAST_SHARED /*one past for every sequence*/, AF_SPLITS_K, AF_SPLITS_P /*work items along the keys*/,
+  AF_MASK_KIND, AF_MASK_SB, AF_MASK_SH, AF_MASK_ST, AF_MASK_ROWS, AF_MASK_LEN
+};
+enum { AFF_SCALE };
+enum { AF_MASK_NONE = 0, AF_MASK_BOOL = 1, AF_MASK_F16 = 2, AF_MASK_F32 = 3 };
+
+// ---- K_RMS_NORM: t[0]=x, t[1]=scale, t[2]=y; rows of RN_N contiguous elements
+enum { RN_ROWS, RN_N, RN_F32 /*else fp16*/, RN_ROWS_PER_BATCH };
+enum { RNF_EPS };
+
+// ---- K_NORM_ROPE: t[0]=cos, t[1]=sin, t[2]=position ids i64 [B][T]|-1, t[3]=x, t[4]=norm scale [D]|-1, t[5]=y,
+//      then t[6..8] the same of a second tensor (NR_ITEMS 2).  Element (b, t, h, d) of a tensor sits at
+//      b*SB + t*ST + h*SH + d.  Tables: [NR_POSITIONS][ROT/2] indexed by the ids, or [B][T][ROT/2] (NR_POSITIONS 0).
+enum {
+  NR_B, NR_T, NR_D, NR_ROT /*rotated elements*/, NR_INTERLEAVED, NR_F32 /*else fp16*/, NR_POSITIONS, NR_ITEMS,
+  NR_H0, NR_X0_SB, NR_X0_ST, NR_X0_SH, NR_Y0_SB, NR_Y0_ST, NR_Y0_SH,
+  NR_H1, NR_X1_SB, NR_X1_ST, NR_X1_SH, NR_Y1_SB, NR_Y1_ST, NR_Y1_SH
+};
+enum { NRF_EPS0, NRF_EPS1 };
 
 // ---- K_LSTM_F32: t[0]=X [T][B][I], t[1]=W rows interleaved [4Hp][I] (g = i,o,f,c; see below),
 //      t[2]=R interleaved [4Hp][H], t[3]=Wb+Rb interleaved [4Hp], t[4]=scratch [T*B][4Hp],
@@ -192,6 +223,9 @@ inline int64_t eff_batch(const LaunchCtx& c, const PlanOp& op, int64_t compiled)
   return (c.batch > 0 && op.ip[IP_BATCHED]) ? c.batch : compiled;
 }
 
+// tc100.cuh's DEV_BAD_INDEX, for the host: reported as EMX_ERR_INVALID_ARGUMENT.
+constexpr int DEV_BAD_INDEX_CODE = 6;
+
 // Launch with programmatic stream serialisation allowed (see pdl_wait() in
 // tc100.cuh): every kernel of the library goes through this helper and waits
 // on its predecessor inside the kernel.
@@ -254,6 +288,10 @@ int launch_transpose(const PlanOp&, void* const*, const OpState*, const LaunchCt
 int launch_maxpool(const PlanOp&, void* const*, const OpState*, const LaunchCtx&, int*);
 int launch_qlinear_avgpool(const PlanOp&, void* const*, const OpState*, const LaunchCtx&, int*);
 int launch_qlinear_softmax(const PlanOp&, void* const*, const OpState*, const LaunchCtx&, int*);
+int prepare_attention_flash(const PlanOp&, void* const*, OpState*, int, char*, size_t);
+int launch_attention_flash(const PlanOp&, void* const*, const OpState*, const LaunchCtx&, int*);
+int launch_rms_norm(const PlanOp&, void* const*, const OpState*, const LaunchCtx&, int*);
+int launch_norm_rope(const PlanOp&, void* const*, const OpState*, const LaunchCtx&, int*);
 int prepare_attention_tc(const PlanOp&, void* const*, OpState*, int, char*, size_t);
 int launch_attention_tc(const PlanOp&, void* const*, const OpState*, const LaunchCtx&, int*);
 

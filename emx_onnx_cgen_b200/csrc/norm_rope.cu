@@ -1,0 +1,400 @@
+// RMSNormalization and RotaryEmbedding (opset 23), fp16 and fp32.
+//
+// K_NORM_ROPE: per head row x of D elements of token (b, t)
+//   y = x / sqrt(mean(x^2) + eps) * scale          (when a norm feeds the rotation)
+//   (y_a, y_b) -> (y_a c - y_b s, y_a s + y_b c)   over the first ROT elements
+// with pairs (i, i + ROT/2), or (2i, 2i+1) interleaved, and c, s the token's
+// row of the tables.  Everything between the load and the store is fp32 and
+// rounded once at the end (the separate operators would round in between).
+// The element orders of x and y are strides, so the exchange of the token and
+// head axes that stands between the two operators in a graph costs nothing,
+// and Q and K of a layer go in one launch.
+//
+// The bound is memory: every element is read and written once.  A row is
+// spread over LPR lanes, each holding the two 16-byte pieces that pair up, so
+// a rotation needs no exchange and the row sum log2(LPR) shuffles; a lane
+// group takes HPG head rows of its token and loads the token's table entries
+// once for them.
+//
+// K_RMS_NORM: rows of any length, a warp per row up to 1024 elements, else a
+// CTA per row; the second pass over the row hits L1 / L2.
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "host_util.h"
+#include "kernels.h"
+#include "tc100.cuh"
+
+namespace emx {
+
+struct RopeItem {
+  const void* x;
+  const void* scale;  // null: no norm
+  void* y;
+  int64_t x_sb, x_st, x_sh, y_sb, y_st, y_sh;
+  int heads;
+  float eps;
+};
+
+struct RopeParams {
+  RopeItem item[2];
+  const void *cos, *sin;
+  const long long* pos;
+  int64_t tokens;
+  int T, D, rot, interleaved, heads /*of both items*/, groups /*lane groups per token*/;
+  int64_t positions;
+  int* err;
+};
+
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
+
+// 16 bytes as fp32 values
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<__half> {
+  static constexpr int N = 8;
+  __device__ static __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    }
+  }
+  __device__ static __forceinline__ uint4 pack(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <>
+struct Chunk<float> {
+  static constexpr int N = 4;
+  __device__ static __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
+  __device__ static __forceinline__ uint4 pack(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+
+// Row of the tables that token (b, t) = `token` uses, or -1 (error recorded) for an id out of range.
+__device__ __forceinline__ int64_t table_row(const RopeParams& p, int64_t token) {
+  if (!p.positions) return token;
+  const long long at = p.pos[token];
+  if (at >= 0 && at < p.positions) return at;
+  record_error(p.err, DEV_BAD_INDEX);
+  return -1;
+}
+
+// Vector form: D and the rotated halves are whole 16-byte pieces, every row starts on 16 bytes.
+template <typename T, int LPR, int HPG>
+__global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ RopeParams p) {
+  constexpr int V = Chunk<T>::N;
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t gi = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;  // lane group (their count fits 32 bits)
+  const int u = threadIdx.x % LPR;
+  // lanes of one group take the same path throughout and shuffle among themselves only
+  const uint32_t group_mask = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << (threadIdx.x & 31 & ~(LPR - 1));
+  const uint32_t token = gi / (uint32_t)p.groups;
+  if (token >= p.tokens) return;
+  const int j = (int)(gi - token * (uint32_t)p.groups);
+  const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * (uint32_t)p.T);
+  const int nc = p.D / V, rc = p.rot / V;
+  // this lane's two pieces and how they rotate
+  int c0, c1;
+  bool turn;
+  if (p.interleaved) {
+    c0 = 2 * u, c1 = 2 * u + 1;
+    turn = c0 < rc;
+  } else {
+    turn = u < rc / 2;
+    c0 = turn ? u : rc + 2 * (u - rc / 2);
+    c1 = turn ? u + rc / 2 : c0 + 1;
+  }
+  const bool has0 = c0 < nc, has1 = c1 < nc;
+  uint4 xv[HPG][2];
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    int h = j + i * p.groups;
+    xv[i][0] = xv[i][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (h >= p.heads) continue;
+    const bool second = h >= p.item[0].heads;
+    const RopeItem& it = p.item[second ? 1 : 0];
+    if (second) h -= p.item[0].heads;
+    const T* x = static_cast<const T*>(it.x) + b * it.x_sb + t * it.x_st + h * it.x_sh;
+    if (has0) xv[i][0] = __ldcs(reinterpret_cast<const uint4*>(x + c0 * V));
+    if (has1) xv[i][1] = __ldcs(reinterpret_cast<const uint4*>(x + c1 * V));
+  }
+  // cosines and sines of the V pairs of this lane's pieces (interleaved pieces 2u, 2u+1 use entries uV .. uV+V-1)
+  float cs[V], sn[V];
+  if (turn) {
+    const int64_t row = table_row(p, token);
+    if (row >= 0) {
+      const int64_t at = row * (p.rot / 2) + u * V;
+      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.cos) + at), cs);
+      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.sin) + at), sn);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
+    }
+  }
+  float w0[V], w1[V];
+  int loaded = -1;
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    int h = j + i * p.groups;
+    if (h >= p.heads) continue;
+    const int sel = h >= p.item[0].heads ? 1 : 0;
+    const RopeItem& it = p.item[sel];
+    if (sel) h -= p.item[0].heads;
+    float a[V], c[V];
+    Chunk<T>::unpack(xv[i][0], a);
+    Chunk<T>::unpack(xv[i][1], c);
+    if (it.scale) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss = fmaf(a[e], a[e], fmaf(c[e], c[e], ss));
+#pragma unroll
+      for (int d = LPR / 2; d; d >>= 1) ss += __shfl_xor_sync(group_mask, ss, d, LPR);
+      const float inv = 1.0f / sqrtf(ss / (float)p.D + it.eps);
+      if (loaded != sel) {
+        const T* sc = static_cast<const T*>(it.scale);
+        uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        Chunk<T>::unpack(has0 ? *reinterpret_cast<const uint4*>(sc + c0 * V) : z, w0);
+        Chunk<T>::unpack(has1 ? *reinterpret_cast<const uint4*>(sc + c1 * V) : z, w1);
+        loaded = sel;
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) a[e] = a[e] * inv * w0[e], c[e] = c[e] * inv * w1[e];
+    }
+    if (turn && p.interleaved) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float re = a[e] * cs[e / 2] - a[e + 1] * sn[e / 2], im = a[e] * sn[e / 2] + a[e + 1] * cs[e / 2];
+        a[e] = re, a[e + 1] = im;
+        const float re1 = c[e] * cs[V / 2 + e / 2] - c[e + 1] * sn[V / 2 + e / 2];
+        const float im1 = c[e] * sn[V / 2 + e / 2] + c[e + 1] * cs[V / 2 + e / 2];
+        c[e] = re1, c[e + 1] = im1;
+      }
+    } else if (turn) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float re = a[e] * cs[e] - c[e] * sn[e], im = a[e] * sn[e] + c[e] * cs[e];
+        a[e] = re, c[e] = im;
+      }
+    }
+    T* y = static_cast<T*>(it.y) + b * it.y_sb + t * it.y_st + h * it.y_sh;
+    if (has0) *reinterpret_cast<uint4*>(y + c0 * V) = Chunk<T>::pack(a);
+    if (has1) *reinterpret_cast<uint4*>(y + c1 * V) = Chunk<T>::pack(c);
+  }
+}
+
+// Any head size, rotation width and alignment: a warp per head row, a pair of elements per lane and step.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_rope_any_kernel(const __grid_constant__ RopeParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const int64_t token = row / p.heads;
+  if (token >= p.tokens) return;
+  int h = (int)(row - token * p.heads);
+  const bool second = h >= p.item[0].heads;
+  const RopeItem& it = p.item[second ? 1 : 0];
+  if (second) h -= p.item[0].heads;
+  const int b = (int)(token / p.T), t = (int)(token - (int64_t)b * p.T);
+  const T* x = static_cast<const T*>(it.x) + b * it.x_sb + t * it.x_st + h * it.x_sh;
+  T* y = static_cast<T*>(it.y) + b * it.y_sb + t * it.y_st + h * it.y_sh;
+  const T* sc = static_cast<const T*>(it.scale);
+  float inv = 1.0f;
+  if (sc) {
+    float ss = 0.0f;
+    for (int e = lane; e < p.D; e += 32) {
+      const float v = to_f32(x[e]);
+      ss = fmaf(v, v, ss);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    inv = 1.0f / sqrtf(ss / (float)p.D + it.eps);
+  }
+  const int64_t at = table_row(p, token);
+  const int half = p.rot / 2;
+  const T* ct = static_cast<const T*>(p.cos) + at * half;
+  const T* st = static_cast<const T*>(p.sin) + at * half;
+  for (int i = lane; i < half; i += 32) {
+    const int ea = p.interleaved ? 2 * i : i, eb = p.interleaved ? 2 * i + 1 : i + half;
+    const float c = at >= 0 ? to_f32(ct[i]) : __int_as_float(0x7fc00000);
+    const float s = at >= 0 ? to_f32(st[i]) : __int_as_float(0x7fc00000);
+    const float va = to_f32(x[ea]) * inv * (sc ? to_f32(sc[ea]) : 1.0f);
+    const float vb = to_f32(x[eb]) * inv * (sc ? to_f32(sc[eb]) : 1.0f);
+    from_f32(va * c - vb * s, y[ea]);
+    from_f32(va * s + vb * c, y[eb]);
+  }
+  for (int e = p.rot + lane; e < p.D; e += 32) from_f32(to_f32(x[e]) * inv * (sc ? to_f32(sc[e]) : 1.0f), y[e]);
+}
+
+template <typename T, int LPR>
+static void launch_vec(const RopeParams& p0, const LaunchCtx& ctx, cudaError_t* e) {
+  RopeParams p = p0;
+  // Four rows per lane group once that still fills every SM's threads: fewer table loads and more bytes in flight
+  const bool four = p.tokens * p.heads * LPR >= (int64_t)ctx.num_sms * 2048 * 4;
+  p.groups = four ? (p.heads + 3) / 4 : p.heads;
+  const int64_t blocks = (p.tokens * p.groups * LPR + 255) / 256;
+  if (p.tokens * p.groups > 0xffff0000ll || blocks > 0x7fffffff) {
+    *e = cudaErrorInvalidConfiguration;
+    return;
+  }
+  if (four)
+    *e = launch_pdl(norm_rope_kernel<T, LPR, 4>, dim3((unsigned)blocks), dim3(256), 0, ctx.stream, p);
+  else
+    *e = launch_pdl(norm_rope_kernel<T, LPR, 1>, dim3((unsigned)blocks), dim3(256), 0, ctx.stream, p);
+}
+
+template <typename T>
+static int launch_rope_t(const RopeParams& p, int items, const LaunchCtx& ctx, int* launches) {
+  constexpr int V = Chunk<T>::N;
+  const int nc = p.D / V;
+  // whole pieces of every row, of its rotated halves and of the tables' rows
+  bool vec = p.D % V == 0 && (p.rot / 2) % V == 0 && nc <= 64;
+  uintptr_t bases = (uintptr_t)p.cos | (uintptr_t)p.sin;
+  for (int i = 0; i < items; ++i) {
+    const RopeItem& it = p.item[i];
+    bases |= (uintptr_t)it.x | (uintptr_t)it.y | (uintptr_t)it.scale;
+    vec = vec && (it.x_sb % V | it.x_st % V | it.x_sh % V | it.y_sb % V | it.y_st % V | it.y_sh % V) == 0;
+  }
+  if ((bases & (sizeof(T) - 1)) != 0 || ((uintptr_t)p.pos & 7u) != 0) return 5;
+  vec = vec && (bases & 15u) == 0;
+  cudaError_t e;
+  if (vec) {
+    const int pairs = (nc + 1) / 2;
+    if (pairs <= 4) launch_vec<T, 4>(p, ctx, &e);
+    else if (pairs <= 8) launch_vec<T, 8>(p, ctx, &e);
+    else if (pairs <= 16) launch_vec<T, 16>(p, ctx, &e);
+    else launch_vec<T, 32>(p, ctx, &e);
+  } else {
+    const int64_t blocks = (p.tokens * p.heads + 7) / 8;
+    if (blocks > 0x7fffffff) return 5;
+    e = launch_pdl(norm_rope_any_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, ctx.stream, p);
+  }
+  ++*launches;
+  return e == cudaSuccess ? 0 : 4;
+}
+
+int launch_norm_rope(const PlanOp& op, void* const* ptrs, const OpState*, const LaunchCtx& ctx, int* launches) {
+  RopeParams p{};
+  auto ptr = [&](int i) -> void* { return op.t[i] >= 0 ? ptrs[op.t[i]] : nullptr; };
+  p.cos = ptr(0);
+  p.sin = ptr(1);
+  p.pos = (const long long*)ptr(2);
+  p.T = (int)op.ip[NR_T];
+  p.tokens = eff_batch(ctx, op, op.ip[NR_B]) * p.T;
+  p.D = (int)op.ip[NR_D];
+  p.rot = (int)op.ip[NR_ROT];
+  p.interleaved = (int)op.ip[NR_INTERLEAVED];
+  p.positions = op.ip[NR_POSITIONS];
+  p.err = ctx.d_error;
+  const int items = (int)op.ip[NR_ITEMS];
+  for (int i = 0; i < items; ++i) {
+    RopeItem& it = p.item[i];
+    const int64_t* s = &op.ip[i ? NR_H1 : NR_H0];
+    it.x = ptr(3 + 3 * i);
+    it.scale = ptr(4 + 3 * i);
+    it.y = ptr(5 + 3 * i);
+    it.heads = (int)s[0];
+    it.x_sb = s[1], it.x_st = s[2], it.x_sh = s[3], it.y_sb = s[4], it.y_st = s[5], it.y_sh = s[6];
+    it.eps = (float)op.fp[NRF_EPS0 + i];
+    p.heads += it.heads;
+  }
+  if (p.tokens <= 0 || p.heads <= 0) return 0;
+  return op.ip[NR_F32] ? launch_rope_t<float>(p, items, ctx, launches)
+                       : launch_rope_t<__half>(p, items, ctx, launches);
+}
+
+// ------------------------------------------------------------------ RMSNormalization
+// WARPS warps per row; VEC: 16-byte accesses (N a multiple of the piece, 16-byte bases).
+template <typename T, int WARPS, bool VEC>
+__global__ void __launch_bounds__(256) rms_norm_kernel(const T* __restrict__ x, const T* __restrict__ scale,
+                                                       T* __restrict__ y, int64_t rows, int64_t n, float eps) {
+  constexpr int V = VEC ? Chunk<T>::N : 1;
+  __shared__ float s_sum[8];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x * (int64_t)(8 / WARPS) + (threadIdx.x >> 5) / WARPS;
+  const int tid = threadIdx.x % (32 * WARPS);
+  if (WARPS == 1 && row >= rows) return;  // a CTA per row has no rows past the end
+  const T* xr = x + row * n;
+  T* yr = y + row * n;
+  float ss = 0.0f;
+  for (int64_t e = (int64_t)tid * V; e < n; e += 32 * WARPS * V) {
+    if (VEC) {
+      float f[Chunk<T>::N];
+      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(xr + e), f);
+#pragma unroll
+      for (int i = 0; i < Chunk<T>::N; ++i) ss = fmaf(f[i], f[i], ss);
+    } else {
+      const float f = to_f32(xr[e]);
+      ss = fmaf(f, f, ss);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+  if (WARPS > 1) {
+    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = ss;
+    __syncthreads();
+    ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) ss += s_sum[i];
+  }
+  const float inv = 1.0f / sqrtf(ss / (float)n + eps);
+  for (int64_t e = (int64_t)tid * V; e < n; e += 32 * WARPS * V) {
+    if (VEC) {
+      float f[Chunk<T>::N], w[Chunk<T>::N];
+      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(xr + e), f);
+      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(scale + e), w);
+#pragma unroll
+      for (int i = 0; i < Chunk<T>::N; ++i) f[i] = f[i] * inv * w[i];
+      *reinterpret_cast<uint4*>(yr + e) = Chunk<T>::pack(f);
+    } else {
+      from_f32(to_f32(xr[e]) * inv * to_f32(scale[e]), yr[e]);
+    }
+  }
+}
+
+template <typename T>
+static int launch_rms_t(const void* x, const void* scale, void* y, int64_t rows, int64_t n, float eps,
+                        const LaunchCtx& ctx, int* launches) {
+  if (((uintptr_t)x | (uintptr_t)scale | (uintptr_t)y) & (sizeof(T) - 1)) return 5;
+  const bool vec = n % Chunk<T>::N == 0 && (((uintptr_t)x | (uintptr_t)scale | (uintptr_t)y) & 15u) == 0;
+  const bool wide = n > 1024;
+  const int64_t blocks = wide ? rows : (rows + 7) / 8;
+  if (blocks > 0x7fffffff) return 5;
+  auto kernel = wide ? (vec ? rms_norm_kernel<T, 8, true> : rms_norm_kernel<T, 8, false>)
+                     : (vec ? rms_norm_kernel<T, 1, true> : rms_norm_kernel<T, 1, false>);
+  cudaError_t e = launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), 0, ctx.stream, (const T*)x, (const T*)scale,
+                             (T*)y, rows, n, eps);
+  ++*launches;
+  return e == cudaSuccess ? 0 : 4;
+}
+
+int launch_rms_norm(const PlanOp& op, void* const* ptrs, const OpState*, const LaunchCtx& ctx, int* launches) {
+  const int64_t rpb = op.ip[RN_ROWS_PER_BATCH];
+  const int64_t rows = op.ip[IP_BATCHED] && ctx.batch > 0 ? ctx.batch * rpb : op.ip[RN_ROWS];
+  if (rows <= 0) return 0;
+  const void *x = ptrs[op.t[0]], *scale = ptrs[op.t[1]];
+  void* y = ptrs[op.t[2]];
+  return op.ip[RN_F32] ? launch_rms_t<float>(x, scale, y, rows, op.ip[RN_N], (float)op.fp[RNF_EPS], ctx, launches)
+                       : launch_rms_t<__half>(x, scale, y, rows, op.ip[RN_N], (float)op.fp[RNF_EPS], ctx, launches);
+}
+
+}  // namespace emx

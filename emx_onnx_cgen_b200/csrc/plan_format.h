@@ -30,7 +30,7 @@ enum EmxTensorKind : uint32_t {
 };
 
 enum EmxDtype : uint32_t {
-  EMX_F32 = 1, EMX_U8 = 2, EMX_I8 = 3, EMX_I32 = 6, EMX_I64 = 7, EMX_F16 = 10, EMX_F64 = 11,
+  EMX_F32 = 1, EMX_U8 = 2, EMX_I8 = 3, EMX_I32 = 6, EMX_I64 = 7, EMX_BOOL = 9, EMX_F16 = 10, EMX_F64 = 11,
 };
 
 enum EmxPlanFlags : uint32_t {

@@ -54,6 +54,9 @@ const KernelEntry kKernels[] = {
     {emx::K_LSTM_F32, emx::prepare_lstm_f32, emx::launch_lstm_f32, "lstm_f32"},
     {emx::K_ATTENTION_F16, emx::prepare_attention, emx::launch_attention, "attention_f16"},
     {emx::K_ATTENTION_TC, emx::prepare_attention_tc, emx::launch_attention_tc, "attention_tc"},
+    {emx::K_ATTENTION_FLASH, emx::prepare_attention_flash, emx::launch_attention_flash, "attention_flash"},
+    {emx::K_RMS_NORM, nullptr, emx::launch_rms_norm, "rms_norm"},
+    {emx::K_NORM_ROPE, nullptr, emx::launch_norm_rope, "norm_rope"},
     {emx::K_COPY, nullptr, emx::launch_copy, "copy"},
     {emx::K_TRANSPOSE, nullptr, emx::launch_transpose, "transpose"},
     {emx::K_MAXPOOL, nullptr, emx::launch_maxpool, "maxpool"},
@@ -144,7 +147,7 @@ namespace {
 
 size_t dtype_size(uint32_t dt) {
   switch (dt) {
-    case EMX_U8: case EMX_I8: return 1;
+    case EMX_U8: case EMX_I8: case EMX_BOOL: return 1;
     case EMX_F16: return 2;
     case EMX_F32: case EMX_I32: return 4;
     case EMX_I64: case EMX_F64: return 8;
@@ -296,6 +299,9 @@ int launch_ops(emx_plan* p, int64_t run_batch, cudaStream_t stream, int* launche
     if (rc) {
       if (p->profiling) *(volatile int*)p->h_hold = seq;
       cudaError_t e = cudaGetLastError();
+      if (rc == EMX_ERR_UNSUPPORTED)
+        return set_error(rc, "op %zu (%s): a buffer of this run does not start on the boundary the kernel needs (16 bytes), "
+                         "or the run is too large for one launch", i, p->entries[i]->name);
       return set_error(rc == EMX_ERR_CUDA ? EMX_ERR_CUDA : rc, "op %zu (%s) launch failed: %s", i,
                        p->entries[i]->name, cudaGetErrorString(e));
     }
@@ -766,6 +772,8 @@ int emx_b200_sync(emx_plan_t* p) {
   CUDA_TRY(cudaMemcpy(&err, p->d_error, sizeof(int), cudaMemcpyDeviceToHost), "error word read");
   if (err) {
     cudaMemset(p->d_error, 0, sizeof(int));
+    if (err == emx::DEV_BAD_INDEX_CODE)
+      return set_error(EMX_ERR_INVALID_ARGUMENT, "an input of position ids or valid key counts holds a value out of range");
     return set_error(EMX_ERR_DEVICE_TIMEOUT, "device-side wait gave up (code %d)", err);
   }
   return EMX_OK;

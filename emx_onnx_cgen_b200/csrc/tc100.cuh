@@ -18,6 +18,7 @@ enum DeviceError : int {
   DEV_TIMEOUT_EPILOGUE = 3,
   DEV_TIMEOUT_GRID = 4,
   DEV_BAD_CONFIG = 5,
+  DEV_BAD_INDEX = 6,  // an input tensor of positions or counts holds a value out of range
 };
 
 // Bounded waits: give up after this many nanoseconds of %globaltimer.  The

@@ -16,6 +16,9 @@ the same class names and the same fields for the ops this backend runs:
   TransposeOp     ir/ops/misc.py:1927   MaxPoolOp     ir/ops/nn.py:9614
   QLinearAveragePoolOp ir/ops/nn.py:5454 QLinearSoftmaxOp ir/ops/nn.py:5997
 
+and, named the same way, RMSNormalizationOp, RotaryEmbeddingOp and ExpandOp for
+the decoder operators of opsets 23 and 24.
+
 Attribute defaults follow the reference's lowerings (lowering/qlinear_conv.py:40,
 qlinear_add.py:31, gemm.py:9, matmul_nbits.py:120, attention.py:363 (scale
 default 1/sqrt(head_size), attention.py:313), lstm.py:335).  The test suite
@@ -220,6 +223,38 @@ class AttentionOp:
     q_rank: int
     head_group_size: int
     dtype: ScalarType
+    input_nonpad_kv_seqlen: str | None = None
+    k_rank: int = 4
+    v_rank: int = 4
+    output_rank: int = 4
+
+
+@dataclass(frozen=True)
+class RMSNormalizationOp:
+    input0: str
+    scale: str
+    output: str
+    axis: int
+    epsilon: float
+
+
+@dataclass(frozen=True)
+class RotaryEmbeddingOp:
+    input0: str
+    cos_cache: str
+    sin_cache: str
+    position_ids: str | None
+    output: str
+    num_heads: int
+    head_size: int
+    rotary_dim: int
+    interleaved: bool
+
+
+@dataclass(frozen=True)
+class ExpandOp:
+    input0: str
+    output: str
 
 
 @dataclass(frozen=True)
@@ -510,6 +545,64 @@ def _initializer(name: str) -> np.ndarray:
     return _INITS[name]
 
 
+def _lower_attention(node, a, ins, shapes, dtypes) -> AttentionOp:
+    """Attention (opsets 23 and 24).  Q, K, V are [batch, heads, tokens, size],
+    or [batch, tokens, heads * size] with q_num_heads / kv_num_heads; the
+    optional inputs are attn_mask, past_key, past_value, nonpad_kv_seqlen."""
+    ins = list(ins) + [""] * (7 - len(ins))
+
+    def bad(why):
+        return UnsupportedOpError(f"Attention: {why}")
+
+    def layout(name, what, heads_attr):
+        shp = tuple(int(v) for v in shapes[name])
+        if len(shp) == 4:
+            return shp
+        heads = int(a.get(heads_attr, 0))
+        if len(shp) != 3 or heads < 1 or shp[2] % heads:
+            raise bad(f"{what} {shp}: rank 4, or rank 3 with {heads_attr} dividing the last axis")
+        return shp[0], heads, shp[1], shp[2] // heads
+
+    b, hq, tq, d = layout(ins[0], "Q", "q_num_heads")
+    kb, hkv, tkv, kd = layout(ins[1], "K", "kv_num_heads")
+    vb, vh, vt, dv = layout(ins[2], "V", "kv_num_heads")
+    if (kb, kd) != (b, d) or (vb, vh, vt) != (b, hkv, tkv):
+        raise bad(f"Q {shapes[ins[0]]}, K {shapes[ins[1]]} and V {shapes[ins[2]]} do not fit together")
+    if hkv < 1 or hq % hkv:
+        raise bad(f"{hq} query heads over {hkv} key/value heads")
+    mask, past_k, past_v, nonpad = (n or None for n in ins[3:7])
+    past = 0
+    if (past_k is None) != (past_v is None):
+        raise bad("past_key and past_value come together")
+    if past_k is not None:
+        past = int(shapes[past_k][2]) if len(shapes[past_k]) == 4 else -1
+        if tuple(shapes[past_k]) != (b, hkv, past, d) or tuple(shapes[past_v]) != (b, hkv, past, dv):
+            raise bad(f"past_key {shapes[past_k]} and past_value {shapes[past_v]} do not fit K and V")
+    total = past + tkv
+    if mask is not None:
+        ms = tuple(int(v) for v in shapes[mask])
+        lead = (1,) * (4 - len(ms)) + ms[:-1]
+        if not 2 <= len(ms) <= 4 or any(m not in (1, n) for m, n in zip(lead, (b, hq, tq))) or ms[-1] > total:
+            raise bad(f"attn_mask {ms} does not broadcast to {(b, hq, tq, total)}")
+        if ms[-1] == 1 < total:  # broadcast, or a mask of one key padded with -inf: definitions differ
+            raise bad(f"attn_mask {ms}: one entry for {total} keys")
+    if nonpad is not None and tuple(shapes[nonpad]) != (b,):
+        raise bad(f"nonpad_kv_seqlen {tuple(shapes[nonpad])} for a batch of {b}")
+    outs = list(node.outputs) + [""] * (4 - len(node.outputs))
+    rank = len(shapes[ins[0]])
+    y = outs[0]
+    shapes[y] = (b, hq, tq, dv) if rank == 4 else (b, tq, hq * dv)
+    dtypes[y] = dtypes[ins[0]]
+    return AttentionOp(
+        input_q=ins[0], input_k=ins[1], input_v=ins[2], input_attn_mask=mask, input_past_key=past_k,
+        input_past_value=past_v, output=y, output_present_key=outs[1] or None, output_present_value=outs[2] or None,
+        output_qk_matmul=outs[3] or None, batch=b, q_heads=hq, kv_heads=hkv, q_seq=tq, kv_seq=tkv, total_seq=total,
+        past_seq=past, qk_head_size=d, v_head_size=dv, scale=float(a["scale"]) if "scale" in a else 1.0 / math.sqrt(d),
+        is_causal=bool(a.get("is_causal", 0)), softcap=float(a.get("softcap", 0.0)), q_rank=rank,
+        head_group_size=hq // hkv, dtype=dtypes[ins[0]], input_nonpad_kv_seqlen=nonpad, k_rank=len(shapes[ins[1]]),
+        v_rank=len(shapes[ins[2]]), output_rank=rank)
+
+
 def _lower_node(node, shapes, dtypes):
     a = dict(node.attrs)
     ins = list(node.inputs)
@@ -646,19 +739,48 @@ def _lower_node(node, shapes, dtypes):
                    axis=int(a["axis"]) if "axis" in a else None,
                    block_size=int(a["block_size"]) if "block_size" in a else None)
     if op == "Attention":
-        b, hq, tq, d = shapes[ins[0]]
-        _, hkv, tkv, _ = shapes[ins[1]]
-        dv = shapes[ins[2]][3]
+        return _lower_attention(node, a, ins, shapes, dtypes)
+    if op == "RMSNormalization":
+        axis = int(a.get("axis", -1))
+        rank = len(shapes[ins[0]])
+        if not -rank <= axis < rank:
+            raise UnsupportedOpError(f"RMSNormalization: axis {axis} of a rank-{rank} input")
+        if int(a.get("stash_type", 1)) != 1:
+            raise UnsupportedOpError(f"RMSNormalization: stash_type {a['stash_type']} has no B200 kernel (1: fp32)")
         y = node.outputs[0]
-        shapes[y] = (b, hq, tq, dv)
+        shapes[y] = shapes[ins[0]]
         dtypes[y] = dtypes[ins[0]]
-        scale = float(a["scale"]) if "scale" in a else 1.0 / math.sqrt(d)
-        return AttentionOp(
-            input_q=ins[0], input_k=ins[1], input_v=ins[2], input_attn_mask=None, input_past_key=None,
-            input_past_value=None, output=y, output_present_key=None, output_present_value=None,
-            output_qk_matmul=None, batch=b, q_heads=hq, kv_heads=hkv, q_seq=tq, kv_seq=tkv, total_seq=tkv,
-            past_seq=0, qk_head_size=d, v_head_size=dv, scale=scale, is_causal=bool(a.get("is_causal", 0)),
-            softcap=float(a.get("softcap", 0.0)), q_rank=4, head_group_size=hq // hkv, dtype=dtypes[ins[0]])
+        return RMSNormalizationOp(input0=ins[0], scale=ins[1], output=y, axis=axis % rank,
+                                  epsilon=float(a.get("epsilon", 1e-5)))
+    if op == "RotaryEmbedding":
+        xs = shapes[ins[0]]
+        if len(xs) == 4:
+            heads, d = int(xs[1]), int(xs[3])
+            if int(a.get("num_heads", 0)) not in (0, heads):
+                raise UnsupportedOpError(f"RotaryEmbedding: num_heads {a['num_heads']} of an input with {heads} heads")
+        elif len(xs) == 3:
+            heads = int(a.get("num_heads", 0))
+            if heads < 1 or xs[2] % heads:
+                raise UnsupportedOpError(f"RotaryEmbedding: a rank-3 input {tuple(xs)} needs num_heads dividing its last axis")
+            d = int(xs[2]) // heads
+        else:
+            raise UnsupportedOpError(f"RotaryEmbedding: rank-{len(xs)} input")
+        y = node.outputs[0]
+        shapes[y] = xs
+        dtypes[y] = dtypes[ins[0]]
+        return RotaryEmbeddingOp(input0=ins[0], cos_cache=ins[1], sin_cache=ins[2],
+                                 position_ids=ins[3] if len(ins) > 3 and ins[3] else None, output=y, num_heads=heads,
+                                 head_size=d, rotary_dim=int(a.get("rotary_embedding_dim", 0)) or d,
+                                 interleaved=bool(a.get("interleaved", 0)))
+    if op == "Expand":
+        target = tuple(int(v) for v in np.asarray(_initializer(ins[1])).reshape(-1))
+        y = node.outputs[0]
+        try:
+            shapes[y] = tuple(np.broadcast_shapes(tuple(shapes[ins[0]]), target))
+        except ValueError:
+            raise UnsupportedOpError(f"Expand: {tuple(shapes[ins[0]])} does not broadcast to {target}") from None
+        dtypes[y] = dtypes[ins[0]]
+        return ExpandOp(input0=ins[0], output=y)
     if op == "LSTM":
         t, b, i = shapes[ins[0]]
         h = int(a["hidden_size"])

@@ -384,6 +384,18 @@ def infer_types(spec: GraphSpec) -> GraphSpec:
             res = [(x.dtype, _broadcast(x.shape, t(ins[1]).shape))]
         elif op in ("Relu", "Sigmoid", "Tanh", "Softmax", "Swish", "Identity"):
             res = [(x.dtype, x.shape)]
+        elif op in ("RMSNormalization", "RotaryEmbedding"):
+            res = [(x.dtype, x.shape)]
+        elif op == "Expand":
+            res = [(x.dtype, _broadcast(x.shape, [int(v) for v in np.asarray(spec.initializers[ins[1]]).reshape(-1)]))]
+        elif op == "Attention":
+            v = t(ins[2])
+            heads = int(a.get("kv_num_heads", 0)) if len(v.shape) == 3 else v.shape[1]
+            dv = v.shape[-1] // max(heads, 1) if len(v.shape) == 3 else v.shape[-1]
+            res = [(x.dtype, (*x.shape[:-1], dv) if len(x.shape) == 4 else
+                    (*x.shape[:-1], int(a.get("q_num_heads", 0)) * dv))]
+        elif op == "MatMulNBits":
+            res = [(x.dtype, (*x.shape[:-1], int(a["N"])))]
         elif op == "QLinearSoftmax":
             res = [(t(ins[4]).dtype, x.shape)]
         elif op == "Gemm":

@@ -37,9 +37,9 @@ PLAN_VERSION = 1
 MAX_RANK = 8
 OP_MAX_T, OP_MAX_I, OP_MAX_F = 12, 40, 8
 T_WEIGHT, T_INPUT, T_OUTPUT, T_TEMP = 0, 1, 2, 3
-DT = {"f32": 1, "u8": 2, "i8": 3, "i32": 6, "i64": 7, "f16": 10, "f64": 11}
+DT = {"f32": 1, "u8": 2, "i8": 3, "i32": 6, "i64": 7, "bool": 9, "f16": 10, "f64": 11}
 NP = {"f32": np.float32, "u8": np.uint8, "i8": np.int8, "i32": np.int32, "i64": np.int64,
-      "f16": np.float16, "f64": np.float64}
+      "bool": np.bool_, "f16": np.float16, "f64": np.float64}
 ALIGN = 256
 
 _HDR = struct.Struct("<IIIIIIqQQII")
@@ -268,6 +268,20 @@ def lstm_persistent_fits(b: int, isz: int, h: int, sms: int) -> bool:
             and smem <= K.LP_SMEM_LIMIT and grid <= sms)
 
 
+FLASH_ROWS, FLASH_KEYS = 128, 64   # packed query rows of a work item, keys of a tile (attention_flash.cu)
+FLASH_CTAS = 2 * K.LP_PLAN_SMS     # two work items run on an SM at a time
+
+
+def flash_splits(items_tiles) -> list[int]:
+    """Work items along the keys for each (items, key tiles of one item) of
+    attention_flash.cu: none while the items fill the device, else as many as
+    keep every item resident at once with about the same number of tiles (at
+    least 4: a shorter item is mostly set-up)."""
+    total = sum(n * t for n, t in items_tiles)
+    target = max(4, -(-total // FLASH_CTAS))
+    return [max(1, t // target) for _, t in items_tiles]
+
+
 def qconv_int_requant_ok(w: np.ndarray, bias: np.ndarray, scale: np.ndarray, a_signed: int) -> int:
     """1 when every accumulator the weights allow keeps |(float)acc * scale| < 2^21.
 
@@ -398,9 +412,13 @@ class B200PlanEmitter:
         "tensor" runs fp16 Attention with 128-wide heads on the tensor cores
         (fp32 accumulation and online softmax: closer to the exact value than
         the reference, not bit-identical to it); other head sizes keep the
-        exact kernel."""
-        if attention_mode not in ("exact", "tensor"):
-            raise ValueError(f"attention_mode {attention_mode!r}: 'exact' or 'tensor'")
+        exact kernel.  "flash" runs every fp16 Attention with head sizes that
+        are multiples of 8 up to 128 on the tensor cores in the same
+        arithmetic, and adds what the other modes reject: boolean and additive
+        masks, valid key counts, past keys, and a past shared by the batch
+        (an Expand of one copy, read once for all sequences)."""
+        if attention_mode not in ("exact", "tensor", "flash"):
+            raise ValueError(f"attention_mode {attention_mode!r}: 'exact', 'tensor' or 'flash'")
         self.attention_mode = attention_mode
         self.use_tensor_cores = use_tensor_cores
         self.nbits_rounded_dequant = nbits_rounded_dequant
@@ -448,7 +466,8 @@ class B200PlanEmitter:
                     if o not in self._nchw:
                         self._dest(o, self._dtype(o), tuple(self._shape(o)))
                 continue
-            empty_in = [n for n in self._op_inputs(op) if int(np.prod(self._shape(n), dtype=np.int64)) == 0]
+            empty_in = [n for n in self._op_inputs(op) if int(np.prod(self._shape(n), dtype=np.int64)) == 0
+                        and not (_name(op) == "AttentionOp" and n in (op.input_past_key, op.input_past_value))]
             if empty_in:
                 # e.g. an LSTM over zero steps or a Gemm with K = 0: outputs that are not
                 # sums over the empty extent have no kernel path here
@@ -604,6 +623,8 @@ class B200PlanEmitter:
                 self._nbits_fused[first] = {"gate": g, "up": u, "mul": op, "alpha": alpha}
                 self._absorbed.update({max(i_g, i_u), i_s, mi})
                 break
+        self._analyse_rotary(ops)
+        self._analyse_shared_past(ops)
         for i, j in self._fused_add.items():
             add = ops[j]
             conv_out = ops[i].output
@@ -645,12 +666,120 @@ class B200PlanEmitter:
                         self._batched_names.add(o)
         del tc_inputs, resid_inputs
 
+    def _only_feeds(self, name: str, i: int) -> bool:
+        """Whether op ``i`` is the one reader of intermediate ``name``."""
+        return self._consumers.get(name) == [i] and name not in self._graph_outputs
+
+    def _rotary_item(self, i, op, ops) -> dict | None:
+        """A RotaryEmbedding with the per-head RMSNormalization that feeds it, if
+        one does (directly, through the exchange of the token and head axes, or
+        through the reshape that joins heads): source tensor and how (batch,
+        token, head) index it.  None: the rotation is rejected when emitted."""
+        if self._dtype(op.input0) not in ("f16", "f32"):
+            return None
+        shape = tuple(int(v) for v in self._shape(op.input0))
+        h, d = int(op.num_heads), int(op.head_size)
+        # (batch, token, head) strides of the rotated tensor
+        if len(shape) == 4:
+            b, t = shape[0], shape[2]
+            strides = (h * t * d, d, t * d)
+        else:
+            b, t = shape[0], shape[1]
+            strides = (t * h * d, h * d, d)
+        item = {"op": op, "index": i, "b": b, "t": t, "h": h, "d": d, "x": op.input0, "xs": strides, "ys": strides,
+                "norm": None, "absorbed": []}
+        j, x = self._producers.get(op.input0), op.input0
+        absorbed, xs = [], strides
+        if j is not None and self._only_feeds(x, i):
+            mid = ops[j]
+            if _name(mid) == "TransposeOp" and len(shape) == 4 and tuple(mid.perm) == (0, 2, 1, 3):
+                absorbed, xs = [j], (t * h * d, h * d, d)
+            elif _name(mid) == "ReshapeOp" and len(shape) == 3 and tuple(self._shape(mid.input0)) == (b, t, h, d):
+                absorbed = [j]
+            if absorbed:
+                x = mid.input0
+                if _name(mid) == "TransposeOp":  # strides take it in with or without a norm
+                    item.update(x=x, xs=xs, absorbed=absorbed)
+                j = self._producers.get(x) if self._only_feeds(x, absorbed[0]) else None
+        else:
+            j = None
+        if j is not None and _name(ops[j]) == "RMSNormalizationOp":
+            norm = ops[j]
+            ns = tuple(int(v) for v in self._shape(norm.input0))
+            if (len(ns) == 4 and ns[3] == d and int(norm.axis) == 3 and tuple(self._shape(norm.scale)) == (d,)
+                    and self._dtype(norm.scale) == self._dtype(norm.input0)):
+                item.update(x=norm.input0, xs=xs, norm=norm, absorbed=absorbed + [j])
+        return item
+
+    def _analyse_rotary(self, ops) -> None:
+        """Per-head norms into the rotations they feed, and two rotations of one
+        position (Q and K of a layer) into one launch, issued at the later of
+        the two where nothing reads the first one's output before."""
+        self._rotary: dict[int, list[dict]] = {}
+        items = {}
+        for i, op in enumerate(ops):
+            if _name(op) == "RotaryEmbeddingOp":
+                item = self._rotary_item(i, op, ops)
+                if item is not None:
+                    items[i] = item
+
+        def key(it):
+            o = it["op"]
+            return (it["b"], it["t"], it["d"], int(o.rotary_dim), bool(o.interleaved), o.cos_cache, o.sin_cache,
+                    o.position_ids, self._dtype(o.input0))
+
+        order = sorted(items)
+        done: set[int] = set()
+        for n, i in enumerate(order):
+            if i in done:
+                continue
+            group = [items[i]]
+            for j in order[n + 1:]:
+                if j not in done and key(items[j]) == key(items[i]):
+                    if all(c > j for c in self._consumers.get(items[i]["op"].output, [])):
+                        group.append(items[j])
+                        done.add(j)
+                    break
+            last = group[-1]["index"]
+            self._rotary[last] = group
+            for it in group:
+                self._absorbed.update(it["absorbed"])
+                if it["index"] != last:
+                    self._absorbed.add(it["index"])
+
+    def _analyse_shared_past(self, ops) -> None:
+        """Attention whose past is an Expand of one copy along the batch reads the
+        one copy; the Expand then needs no kernel."""
+        self._shared_past: dict[int, tuple[str, str]] = {}
+        if self.attention_mode != "flash" or not self.use_tensor_cores:
+            return
+        expands = {}
+        for i, op in enumerate(ops):
+            if _name(op) != "ExpandOp":
+                continue
+            src, dst = tuple(self._shape(op.input0)), tuple(self._shape(op.output))
+            if len(src) == 4 and len(dst) == 4 and src[0] == 1 and src[1:] == dst[1:]:
+                expands[op.output] = i
+        for i, op in enumerate(ops):
+            if (_name(op) == "AttentionOp" and self._flash_reject(op) is None and op.input_past_key in expands
+                    and op.input_past_value in expands):
+                self._shared_past[i] = tuple(ops[expands[n]].input0 for n in (op.input_past_key, op.input_past_value))
+        for name, i in expands.items():
+            users = self._consumers.get(name, [])
+            if users and name not in self._graph_outputs and all(
+                    u in self._shared_past and name not in (ops[u].input_q, ops[u].input_k, ops[u].input_v,
+                                                            ops[u].input_attn_mask) for u in users):
+                self._absorbed.add(i)
+
     @staticmethod
     def _op_inputs(op):
         fields = {
             "QLinearConvOp": ("input0",), "QLinearAddOp": ("input0", "input1"),
             "GemmOp": ("input_a", "input_b", "input_c"), "UnaryOp": ("input0",), "BinaryOp": ("input0", "input1"),
-            "MatMulNBitsOp": ("input0",), "AttentionOp": ("input_q", "input_k", "input_v"),
+            "MatMulNBitsOp": ("input0",), "AttentionOp": ("input_q", "input_k", "input_v", "input_attn_mask", "input_past_key", "input_past_value",
+                            "input_nonpad_kv_seqlen"),
+            "RMSNormalizationOp": ("input0", "scale"),
+            "RotaryEmbeddingOp": ("input0", "cos_cache", "sin_cache", "position_ids"), "ExpandOp": ("input0",),
             "LstmOp": ("input_x",), "QLinearMatMulOp": ("input0", "input1"), "MatMulIntegerOp": ("input0", "input1"),
             "ConvOp": ("input0", "weights", "bias"), "SoftmaxOp": ("input0",), "QuantizeLinearOp": ("input0",),
             "DequantizeLinearOp": ("input0",), "ReshapeOp": ("input0",), "TransposeOp": ("input0",),
@@ -1261,8 +1390,182 @@ class B200PlanEmitter:
     def _emit_DequantizeLinearOp(self, i, op):
         self._emit_quant(op, False)
 
+    # ------------------------------------------------------------------ RMSNormalization / RotaryEmbedding / Expand
+    def _fixed_or_batched(self, name: str, led_by_batch: bool) -> bool:
+        """Whether operand ``name`` follows a batch slice: an initializer not led
+        by the batch, or a batched tensor led by it."""
+        return self._is_batched(name) if led_by_batch else name in self._consts
+
+    def _emit_RMSNormalizationOp(self, i, op):
+        dt = self._dtype(op.input0)
+        if dt not in ("f16", "f32") or self._dtype(op.scale) != dt:
+            raise UnsupportedOpError(f"RMSNormalization of {dt} with {self._dtype(op.scale)} scale has no B200 kernel")
+        shape = tuple(int(v) for v in self._shape(op.input0))
+        axis = int(op.axis) % len(shape)
+        n = int(np.prod(shape[axis:]))
+        if tuple(self._shape(op.scale)) != shape[axis:]:
+            raise UnsupportedOpError(f"RMSNormalization: scale {tuple(self._shape(op.scale))} for normalised axes "
+                                     f"{shape[axis:]} has no B200 kernel")
+        rows = int(np.prod(shape[:axis]))
+        x, scale = self._src(op.input0), self._src(op.scale)
+        y = self._dest(op.output, dt, shape)
+        batched = (self._batch > 0 and axis > 0 and shape[0] == self._batch and self._is_batched(op.input0)
+                   and self._fixed_or_batched(op.scale, False))
+        self._b.op(K.K_RMS_NORM, [x, scale, y], {K.RN_ROWS: rows, K.RN_N: n, K.RN_F32: int(dt == "f32"),
+                                                 K.RN_ROWS_PER_BATCH: rows // self._batch if batched else 0},
+                   {K.RNF_EPS: float(np.float32(op.epsilon))}, label=f"{op.output} (RMSNormalization {dt})", batched=batched)
+
+    def _emit_RotaryEmbeddingOp(self, i, op):
+        dt = self._dtype(op.input0)
+        if i not in self._rotary:
+            raise UnsupportedOpError(f"RotaryEmbedding of {dt} has no B200 kernel")
+        group = self._rotary[i]
+        op = group[0]["op"]
+        b, t, d, rot = group[0]["b"], group[0]["t"], group[0]["d"], int(op.rotary_dim)
+        if rot < 2 or rot % 2 or rot > d:
+            raise UnsupportedOpError(f"RotaryEmbedding: {rot} rotated elements of a head size of {d}")
+        tables = tuple(int(v) for v in self._shape(op.cos_cache))
+        want = 2 if op.position_ids is not None else 3
+        if (tables != tuple(self._shape(op.sin_cache)) or len(tables) != want or tables[-1] != rot // 2
+                or (want == 3 and tables[:2] != (b, t))
+                or {self._dtype(op.cos_cache), self._dtype(op.sin_cache)} != {dt}):
+            raise UnsupportedOpError(
+                f"RotaryEmbedding: cos/sin caches {tables} / {tuple(self._shape(op.sin_cache))} "
+                f"{'with' if want == 2 else 'without'} position_ids, for {rot // 2} pairs of {dt}")
+        if op.position_ids is not None and (self._dtype(op.position_ids) != "i64"
+                                            or tuple(self._shape(op.position_ids)) != (b, t)):
+            raise UnsupportedOpError(f"RotaryEmbedding: position_ids {tuple(self._shape(op.position_ids))} "
+                                     f"{self._dtype(op.position_ids)}, needs i64 {(b, t)}")
+        batched = self._batch > 0 and b == self._batch
+        for name, led in ((op.cos_cache, want == 3), (op.sin_cache, want == 3),
+                          *(((op.position_ids, True),) if op.position_ids is not None else ())):
+            batched = batched and self._fixed_or_batched(name, led)
+        ip = {K.NR_B: b, K.NR_T: t, K.NR_D: d, K.NR_ROT: rot, K.NR_INTERLEAVED: int(bool(op.interleaved)),
+              K.NR_F32: int(dt == "f32"), K.NR_POSITIONS: tables[0] if want == 2 else 0, K.NR_ITEMS: len(group)}
+        tensors = [self._src(op.cos_cache), self._src(op.sin_cache),
+                   self._src(op.position_ids) if op.position_ids is not None else -1]
+        fp, labels = {}, []
+        for n, it in enumerate(group):
+            o, norm = it["op"], it["norm"]
+            batched = batched and self._is_batched(it["x"]) and (norm is None or self._fixed_or_batched(norm.scale, False))
+            tensors += [self._src(it["x"]), self._src(norm.scale) if norm is not None else -1,
+                        self._dest(o.output, dt, tuple(self._shape(o.output)))]
+            base = K.NR_H1 if n else K.NR_H0
+            for slot, val in enumerate((it["h"], *it["xs"], *it["ys"])):
+                ip[base + slot] = val
+            fp[K.NRF_EPS0 + n] = float(np.float32(norm.epsilon)) if norm is not None else 0.0
+            labels.append(("RMSNormalization + " if norm is not None else "") + f"RotaryEmbedding -> {o.output}")
+        self._b.op(K.K_NORM_ROPE, tensors, ip, fp, label=", ".join(labels) + f" ({dt})", batched=batched)
+
+    def _emit_ExpandOp(self, i, op):
+        """A strided copy whose repeated axes have stride 0."""
+        dt = self._dtype(op.input0)
+        elem = np.dtype(NP[dt]).itemsize
+        src, out = tuple(self._shape(op.input0)), tuple(self._shape(op.output))
+        if elem not in (1, 2, 4) or len(out) > 6:
+            raise UnsupportedOpError(f"Expand of {dt} to rank {len(out)} has no B200 kernel")
+        ip = {K.TR_ELEM: elem, K.TR_BATCH_AXIS: -1}
+        full = (1,) * (6 - len(src)) + src
+        shape = (1,) * (6 - len(out)) + out
+        for j in range(6):
+            ip[K.TR_D0 + j] = shape[j]
+            ip[K.TR_S0 + j] = 0 if full[j] == 1 else int(np.prod(full[j + 1:]))
+        x = self._src(op.input0)
+        y = self._dest(op.output, dt, out)
+        self._b.op(K.K_TRANSPOSE, [x, y], ip, label=f"{op.output} (Expand)", batched=False)
+
     # ------------------------------------------------------------------ Attention
+    def _flash_reject(self, op) -> str | None:
+        """Why this Attention has no flash-mode kernel (None: it has one)."""
+        d, dv = int(op.qk_head_size), int(op.v_head_size)
+        past = int(op.past_seq)
+        if any(self._dtype(n) != "f16" for n in (op.input_q, op.input_k, op.input_v)) or _suffix(op.dtype) != "f16":
+            return "only fp16"
+        if past and any(self._dtype(n) != "f16" for n in (op.input_past_key, op.input_past_value)):
+            return "only an fp16 past"
+        if op.output_present_key or op.output_present_value or op.output_qk_matmul:
+            return "present key/value and score outputs"
+        if float(op.softcap) != 0.0:
+            return "softcap"
+        if any(v < 8 or v > 128 or v % 8 for v in (d, dv)):
+            return f"head sizes {d} / {dv} (multiples of 8 up to 128)"
+        nonpad = getattr(op, "input_nonpad_kv_seqlen", None)
+        if nonpad and (op.input_past_key or op.is_causal):
+            return "nonpad_kv_seqlen together with a past or a causal mask"
+        if nonpad and self._dtype(nonpad) != "i64":
+            return "nonpad_kv_seqlen that is not int64"
+        if op.input_attn_mask and self._dtype(op.input_attn_mask) not in ("bool", "f16", "f32"):
+            return f"a {self._dtype(op.input_attn_mask)} mask"
+        return None
+
+    def _emit_attention_flash(self, i, op):
+        why = self._flash_reject(op)
+        if why:
+            raise UnsupportedOpError(f"Attention: {why} has no B200 kernel in flash mode")
+        b, hq, hkv, tq = int(op.batch), int(op.q_heads), int(op.kv_heads), int(op.q_seq)
+        tk, tp, d, dv = int(op.kv_seq), int(op.past_seq), int(op.qk_head_size), int(op.v_head_size)
+        ss = self._attention_strides(op, b, hq, hkv, tq, tk, d, dv)
+        shared = i in self._shared_past
+        batched = self._batch > 0 and b == self._batch and not shared and all(
+            self._is_batched(n) for n in (op.input_q, op.input_k, op.input_v))
+        ip = {K.AF_B: b, K.AF_HQ: hq, K.AF_HKV: hkv, K.AF_TQ: tq, K.AF_TK: tk, K.AF_TP: tp, K.AF_D: d, K.AF_DV: dv,
+              K.AF_CAUSAL: int(bool(op.is_causal)), K.AF_PAST_SHARED: int(shared)}
+        for slot, val in zip(range(K.AF_Q_SB, K.AF_O_ST + 1), ss):
+            ip[slot] = val
+        t_mask = t_bits = t_part = t_count = t_pk = t_pv = -1
+        if op.input_attn_mask:
+            ms = tuple(int(v) for v in self._shape(op.input_attn_mask))
+            mb, mh, mt = (1,) * (4 - len(ms)) + ms[:-1]
+            kind = {"bool": K.AF_MASK_BOOL, "f16": K.AF_MASK_F16, "f32": K.AF_MASK_F32}[self._dtype(op.input_attn_mask)]
+            ip.update({K.AF_MASK_KIND: kind, K.AF_MASK_SB: mh * mt if mb > 1 else 0, K.AF_MASK_SH: mt if mh > 1 else 0,
+                       K.AF_MASK_ST: 1 if mt > 1 else 0, K.AF_MASK_ROWS: mb * mh * mt, K.AF_MASK_LEN: ms[-1]})
+            t_mask = self._src(op.input_attn_mask)
+            batched = batched and self._fixed_or_batched(op.input_attn_mask, len(ms) == 4 and mb == self._batch)
+            if kind == K.AF_MASK_BOOL:
+                words = -(-tp // FLASH_KEYS) + -(-tk // FLASH_KEYS)
+                t_bits = self._b.arena_tensor(T_TEMP, "u8", (mb * mh * mt, 16 + 8 * words), name="attention:mask-bits")
+        nonpad = getattr(op, "input_nonpad_kv_seqlen", None)
+        if nonpad:
+            t_count = self._src(nonpad)
+            batched = batched and self._fixed_or_batched(nonpad, True)
+        row_tiles = lambda rows: -(-rows // FLASH_ROWS)
+        group = hq // hkv
+        work = [(b * hkv * row_tiles(tq * group), -(-tk // FLASH_KEYS))]
+        if tp:
+            names = self._shared_past[i] if shared else (op.input_past_key, op.input_past_value)
+            t_pk, t_pv = (self._src(n) for n in names)
+            if not shared:
+                batched = batched and all(self._fixed_or_batched(n, True) for n in names)
+            work.append(((1 if shared else b) * hkv * row_tiles(tq * group * (b if shared else 1)), -(-tp // FLASH_KEYS)))
+        splits = flash_splits(work)
+        ip.update({K.AF_SPLITS_K: splits[0], K.AF_SPLITS_P: splits[1] if tp else 0})
+        if sum(splits) > 1:
+            t_part = self._b.arena_tensor(T_TEMP, "f32", (sum(splits), b * tq * hq, dv + 2), name="attention:partials")
+        q, k, v = self._src(op.input_q), self._src(op.input_k), self._src(op.input_v)
+        y = self._dest(op.output, "f16", tuple(self._shape(op.output)))
+        what = "shared past, " if shared and tp else ("past, " if tp else "")
+        self._b.op(K.K_ATTENTION_FLASH, [q, k, v, y, t_mask, t_pk, t_pv, t_count, t_part, t_bits], ip,
+                   {K.AFF_SCALE: float(op.scale)},
+                   label=f"{op.output} ({what}tensor cores, fp32 online softmax, key splits {'+'.join(map(str, splits))})",
+                   batched=batched)
+
+    @staticmethod
+    def _attention_strides(op, b, hq, hkv, tq, tk, d, dv):
+        """(batch, head, token) element strides of Q, K, V and the output."""
+        def strides(rank, heads, t, hd):
+            # 4-D [B][H][T][hd] or 3-D [B][T][H*hd]
+            return (heads * t * hd, t * hd, hd) if rank == 4 else (t * heads * hd, hd, heads * hd)
+
+        q_rank = int(op.q_rank)
+        k_rank = int(getattr(op, "k_rank", q_rank))
+        v_rank = int(getattr(op, "v_rank", q_rank))
+        o_rank = int(getattr(op, "output_rank", q_rank))
+        return (*strides(q_rank, hq, tq, d), *strides(k_rank, hkv, tk, d), *strides(v_rank, hkv, tk, dv),
+                *strides(o_rank, hq, tq, dv))
+
     def _emit_AttentionOp(self, i, op):
+        if self.attention_mode == "flash" and self.use_tensor_cores:
+            return self._emit_attention_flash(i, op)
         why = None
         if self._dtype(op.input_q) != "f16" or _suffix(op.dtype) != "f16":
             why = "only fp16"
@@ -1275,20 +1578,10 @@ class B200PlanEmitter:
         elif int(op.v_head_size) > 128 or int(op.v_head_size) % 2:
             why = "v head size above 128 or odd"
         if why:
-            raise UnsupportedOpError(f"Attention: {why} has no B200 kernel")
+            raise UnsupportedOpError(f"Attention: {why} has no B200 kernel in {self.attention_mode} mode")
         b, hq, hkv = int(op.batch), int(op.q_heads), int(op.kv_heads)
         tq, tk, d, dv = int(op.q_seq), int(op.total_seq), int(op.qk_head_size), int(op.v_head_size)
-
-        def strides(rank, heads, t, hd):
-            # 4-D [B][H][T][hd] or 3-D [B][T][H*hd]: (batch, head, token) strides in elements
-            return (heads * t * hd, t * hd, hd) if rank == 4 else (t * heads * hd, hd, heads * hd)
-
-        q_rank = int(op.q_rank)
-        k_rank = int(getattr(op, "k_rank", q_rank))
-        v_rank = int(getattr(op, "v_rank", q_rank))
-        o_rank = int(getattr(op, "output_rank", q_rank))
-        ss = (*strides(q_rank, hq, tq, d), *strides(k_rank, hkv, int(op.kv_seq), d),
-              *strides(v_rank, hkv, int(op.kv_seq), dv), *strides(o_rank, hq, tq, dv))
+        ss = self._attention_strides(op, b, hq, hkv, tq, int(op.kv_seq), d, dv)
         q, k, v = self._src(op.input_q), self._src(op.input_k), self._src(op.input_v)
         out_shape = tuple(self._shape(op.output))
         y = self._dest(op.output, "f16", out_shape)

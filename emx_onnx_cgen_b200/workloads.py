@@ -505,6 +505,183 @@ def transpose(shape: tuple[int, ...] = (2, 3, 4, 5), perm: tuple[int, ...] = (0,
                     dict(shape=tuple(shape), perm=tuple(perm)))
 
 
+def norm_rope(batch: int = 2, seq: int = 16, q_heads: int = 8, kv_heads: int = 2, head_dim: int = 64,
+              rotary_dim: int = 0, interleaved: bool = False, dtype: str = "f16", layout: str = "transpose",
+              norm: bool = True, positions: str = "ids", eps: float = 1e-6, weight_seed: int = 1) -> Workload:
+    """Per-head RMSNormalization and RotaryEmbedding of a layer's queries and
+    keys.  ``layout`` "transpose": [batch, token, head, size] in, heads before
+    tokens out; "heads": [batch, head, token, size] in and out; "flat": the
+    norm on [batch, token, head, size], the rotation on the joined heads.
+    ``positions`` "ids": tables [position, pairs] with position_ids; "rows":
+    tables [batch, token, pairs].  ``norm`` False: the rotation alone."""
+    rng = np.random.default_rng(weight_seed)
+    npt = np.float16 if dtype == "f16" else np.float32
+    rot = rotary_dim or head_dim
+    longest = seq + 9
+    angle = np.arange(longest)[:, None] * 10000.0 ** (-np.arange(rot // 2) / max(rot // 2, 1))[None, :]
+    tables = [f(angle).astype(npt) for f in (np.cos, np.sin)]
+    inits = {"q_scale": rng.uniform(0.5, 1.5, head_dim).astype(npt),
+             "k_scale": rng.uniform(0.5, 1.5, head_dim).astype(npt)} if norm else {}
+    inputs, nodes, outs, values = [], [], [], []
+    if positions == "ids":
+        inits.update(cos=tables[0], sin=tables[1])
+        inputs.append(TensorSpec("pos", "i64", (batch, seq)))
+    else:
+        inputs += [TensorSpec(n, dtype, (batch, seq, rot // 2)) for n in ("cos", "sin")]
+    last = ("pos",) if positions == "ids" else ()
+    attrs = {"interleaved": int(interleaved), "rotary_embedding_dim": rotary_dim}
+    for x, h in (("Q", q_heads), ("K", kv_heads)):
+        token_major, head_major = (batch, seq, h, head_dim), (batch, h, seq, head_dim)
+        shape = head_major if layout == "heads" else token_major
+        inputs.append(TensorSpec(x, dtype, shape))
+        cur = x
+        if norm:
+            nodes.append(NodeSpec("RMSNormalization", f"{x}_norm", (cur, x.lower() + "_scale"), (f"{x}n",),
+                                  {"axis": -1, "epsilon": eps}))
+            values.append(TensorSpec(f"{x}n", dtype, shape))
+            cur = f"{x}n"
+        rope = dict(attrs)
+        if layout == "transpose":
+            nodes.append(NodeSpec("Transpose", f"{x}_heads", (cur,), (f"{x}t",), {"perm": [0, 2, 1, 3]}))
+            values.append(TensorSpec(f"{x}t", dtype, head_major))
+            cur, shape = f"{x}t", head_major
+        elif layout == "flat":
+            shape = (batch, seq, h * head_dim)
+            inits[f"{x}_flat"] = np.array(shape, np.int64)
+            nodes.append(NodeSpec("Reshape", f"{x}_join", (cur, f"{x}_flat"), (f"{x}j",)))
+            values.append(TensorSpec(f"{x}j", dtype, shape))
+            cur, rope["num_heads"] = f"{x}j", h
+        nodes.append(NodeSpec("RotaryEmbedding", f"{x}_rope", (cur, "cos", "sin", *last), (f"Y{x}",), rope))
+        outs.append(TensorSpec(f"Y{x}", dtype, shape))
+    g = GraphSpec("norm_rope", inputs, outs, nodes, inits, values, (("", 23),))
+
+    def make_inputs(seed: int = 0) -> dict[str, np.ndarray]:
+        r = np.random.default_rng(seed)
+        x = {n: (3 * r.standard_normal((batch, seq, h, head_dim))).astype(npt)
+             for n, h in (("Q", q_heads), ("K", kv_heads))}
+        if layout == "heads":
+            x = {n: np.ascontiguousarray(v.transpose(0, 2, 1, 3)) for n, v in x.items()}
+        pos = r.integers(0, 9, (batch, 1)) + np.arange(seq)[None, :]
+        if positions == "ids":
+            return {**x, "pos": pos.astype(np.int64)}
+        return {**x, "cos": tables[0][pos], "sin": tables[1][pos]}
+
+    return Workload("norm_rope", g, make_inputs, {n.name: 0 for n in (*inputs, *outs)},
+                    dict(batch=batch, seq=seq, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, rot=rot,
+                         interleaved=interleaved, layout=layout, norm=norm, positions=positions, eps=eps))
+
+
+def decoder_attention(batch: int = 2, q_heads: int = 4, kv_heads: int = 2, q_seq: int = 5, kv_seq: int = 70,
+                      head_dim: int = 64, v_dim: int = 0, rank: int = 4, mask: str = "none",
+                      mask_shape: tuple[int, ...] | None = None, count: bool = False, past: int = 0,
+                      shared_past: bool = True, causal: bool = False, scale: float | None = None) -> Workload:
+    """One Attention of decoder tokens: over an encoder's states of another
+    length (``count``: nonpad_kv_seqlen; ``mask``: "bool", "f16" or "f32" of
+    ``mask_shape``, by default one row per sequence), or behind a ``past``
+    that is the Expand of one copy (``shared_past``) or one per sequence."""
+    dv = v_dim or head_dim
+    total = past + kv_seq
+    mshape = tuple(mask_shape) if mask_shape else (batch, 1, 1, total)
+
+    def shp(h, t, d):
+        return (batch, h, t, d) if rank == 4 else (batch, t, h * d)
+
+    inputs = [TensorSpec("Q", "f16", shp(q_heads, q_seq, head_dim)), TensorSpec("K", "f16", shp(kv_heads, kv_seq, head_dim)),
+              TensorSpec("V", "f16", shp(kv_heads, kv_seq, dv))]
+    names = ["Q", "K", "V", "", "", "", ""]
+    nodes, inits, values = [], {}, []
+    if mask != "none":
+        inputs.append(TensorSpec("mask", mask, mshape))
+        names[3] = "mask"
+    if past:
+        pb = 1 if shared_past else batch
+        for slot, n, d in ((4, "PK", head_dim), (5, "PV", dv)):
+            inputs.append(TensorSpec(n, "f16", (pb, kv_heads, past, d)))
+            names[slot] = n
+            if shared_past:
+                inits[f"{n}_shape"] = np.array([batch, kv_heads, past, d], np.int64)
+                nodes.append(NodeSpec("Expand", f"{n}_share", (n, f"{n}_shape"), (f"{n}x",)))
+                values.append(TensorSpec(f"{n}x", "f16", (batch, kv_heads, past, d)))
+                names[slot] = f"{n}x"
+    if count:
+        inputs.append(TensorSpec("count", "i64", (batch,)))
+        names[6] = "count"
+    attrs = {"is_causal": int(causal)}
+    if rank == 3:
+        attrs.update(q_num_heads=q_heads, kv_num_heads=kv_heads)
+    if scale is not None:
+        attrs["scale"] = float(scale)
+    while names[-1] == "":
+        names.pop()
+    nodes.append(NodeSpec("Attention", "attn", tuple(names), ("Y",), attrs))
+    outputs = [TensorSpec("Y", "f16", shp(q_heads, q_seq, dv))]
+    g = GraphSpec("decoder_attention", inputs, outputs, nodes, inits, values, (("", 24),))
+
+    def make_inputs(seed: int = 0) -> dict[str, np.ndarray]:
+        r = np.random.default_rng(seed)
+        x = {}
+        for t in inputs:
+            if t.name == "count":
+                x["count"] = r.integers(max(kv_seq // 2, 1), kv_seq + 1, batch).astype(np.int64)
+            elif t.name == "mask" and mask == "bool":
+                x["mask"] = r.random(mshape) < 0.7
+            elif t.name == "mask":
+                x["mask"] = (-np.abs(r.standard_normal(mshape))).astype(np.float16 if mask == "f16" else np.float32)
+            else:
+                x[t.name] = r.standard_normal(t.shape).astype(np.float16)
+        return x
+
+    return Workload("decoder_attention", g, make_inputs, {t.name: 0 for t in (*inputs, *outputs)},
+                    dict(batch=batch, q_heads=q_heads, kv_heads=kv_heads, q_seq=q_seq, kv_seq=kv_seq, head_dim=head_dim,
+                         v_dim=dv, rank=rank, past=past, shared_past=shared_past, causal=causal,
+                         scale=scale if scale is not None else 1.0 / np.sqrt(head_dim)))
+
+
+def decoder_layer(batch: int = 3, tokens: int = 2, q_heads: int = 4, kv_heads: int = 2, head_dim: int = 64,
+                  prefix: int = 100, frames: int = 77, weight_seed: int = 1) -> Workload:
+    """The attention side of a decoder layer: per-head norm and rotation of Q
+    and K, causal self-attention behind a prefix the batch shares, a norm of
+    the joined heads, and cross attention of the result over encoder states
+    with a valid count per sequence."""
+    rng = np.random.default_rng(weight_seed)
+    b, t, hq, hkv, d = batch, tokens, q_heads, kv_heads, head_dim
+    pos = np.arange(prefix + tokens)[:, None] * 10000.0 ** (-np.arange(d // 2) / (d // 2))[None, :]
+    inits = {"q_scale": rng.uniform(0.5, 1.5, d).astype(np.float16), "k_scale": rng.uniform(0.5, 1.5, d).astype(np.float16),
+             "cos": np.cos(pos).astype(np.float16), "sin": np.sin(pos).astype(np.float16),
+             "full": np.array([b, hkv, prefix, d], np.int64), "joined": np.array([b, t, hq * d], np.int64),
+             "x_scale": rng.uniform(0.5, 1.5, hq * d).astype(np.float16)}
+    inputs = [TensorSpec("Q", "f16", (b, t, hq, d)), TensorSpec("K", "f16", (b, t, hkv, d)),
+              TensorSpec("V", "f16", (b, hkv, t, d)), TensorSpec("pos", "i64", (b, t)),
+              TensorSpec("prefix_k", "f16", (1, hkv, prefix, d)), TensorSpec("prefix_v", "f16", (1, hkv, prefix, d)),
+              TensorSpec("enc_k", "f16", (b, frames, hq * d)), TensorSpec("enc_v", "f16", (b, frames, hq * d)),
+              TensorSpec("count", "i64", (b,))]
+    nodes = []
+    for x in ("Q", "K"):
+        nodes += [NodeSpec("RMSNormalization", f"{x}_norm", (x, f"{x.lower()}_scale"), (f"{x}n",), {"epsilon": 1e-6}),
+                  NodeSpec("Transpose", f"{x}_heads", (f"{x}n",), (f"{x}t",), {"perm": [0, 2, 1, 3]}),
+                  NodeSpec("RotaryEmbedding", f"{x}_rope", (f"{x}t", "cos", "sin", "pos"), (f"{x}r",))]
+    nodes += [NodeSpec("Expand", "share_k", ("prefix_k", "full"), ("past_k",)),
+              NodeSpec("Expand", "share_v", ("prefix_v", "full"), ("past_v",)),
+              NodeSpec("Attention", "self", ("Qr", "Kr", "V", "", "past_k", "past_v"), ("S",), {"is_causal": 1}),
+              NodeSpec("Transpose", "tokens", ("S",), ("St",), {"perm": [0, 2, 1, 3]}),
+              NodeSpec("Reshape", "join", ("St", "joined"), ("Sj",)),
+              NodeSpec("RMSNormalization", "x_norm", ("Sj", "x_scale"), ("X",), {"epsilon": 1e-5}),
+              NodeSpec("Attention", "cross", ("X", "enc_k", "enc_v", "", "", "", "count"), ("Y",),
+                       {"q_num_heads": hq, "kv_num_heads": hq})]
+    g = GraphSpec("decoder_layer", inputs, [TensorSpec("Y", "f16", (b, t, hq * d))], nodes, inits,
+                  opset_imports=(("", 24),))
+
+    def make_inputs(seed: int = 0) -> dict[str, np.ndarray]:
+        r = np.random.default_rng(seed)
+        x = {s.name: r.standard_normal(s.shape).astype(np.float16) for s in inputs if s.dtype == "f16"}
+        x["pos"] = np.broadcast_to(prefix + np.arange(t), (b, t)).astype(np.int64).copy()
+        x["count"] = r.integers(frames // 2, frames + 1, b).astype(np.int64)
+        return x
+
+    return Workload("decoder_layer", g, make_inputs, {}, dict(batch=b, tokens=t, q_heads=hq, kv_heads=hkv, head_dim=d,
+                                                             prefix=prefix, frames=frames))
+
+
 BUILDERS = {
     "mlp_fp32": mlp_fp32,
     "qconv_stack_int8": qconv_stack_int8,
@@ -521,4 +698,7 @@ BUILDERS = {
     "pool8": pool8,
     "qlinear_softmax8": qlinear_softmax8,
     "transpose": transpose,
+    "norm_rope": norm_rope,
+    "decoder_attention": decoder_attention,
+    "decoder_layer": decoder_layer,
 }
