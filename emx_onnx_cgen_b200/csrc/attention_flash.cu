@@ -44,6 +44,7 @@
 // in shared memory: what padding holds, NaN included, reaches no result.
 #include <cuda_fp16.h>
 
+#include "attention_flash.cuh"
 #include "host_util.h"
 #include "kernels.h"
 #include "tc100.cuh"
@@ -58,68 +59,9 @@ constexpr uint32_t AFK_QSLAB = AFK_M * 128u;  // 64 fp16 columns of the Q tile (
 constexpr uint32_t AFK_KSLAB = AFK_N * 128u;  // 64 fp16 columns of a K or V tile: 8 KB
 constexpr uint32_t AFK_TMEM_COLS = 256;       // scores at columns 0 and 64, output at 128
 constexpr uint32_t AFK_O_COL = 128;
-constexpr float AFK_RESCALE = 8.0f;  // the output is rescaled when a row's maximum grows by more (log2 units)
-constexpr float AFK_LOG2E = 1.4426950408889634f;
-
-enum { MASK_NONE = 0, MASK_BITS = 1, MASK_ADD = 2 };  // kernel variants
-
-struct FlashSegment {
-  CUtensorMap map_k, map_v;  // 4-D (d, key, head, batch), box (64, 64, 1, 1), 128-byte swizzle
-  int keys;                  // keys of the segment
-  int mask_off;              // first key's position in a mask row (elements)
-  int word_off;              // first word of the segment in a packed mask row
-  int shared;                // one copy for every sequence
-  int splits;                // work items along the keys
-  int tiles;                 // row tiles per (batch or all, key/value head)
-  int part0;                 // first partial slot
-  int limited;               // causal and valid-count limits apply (the current keys)
-};
-
-struct FlashParams {
-  FlashSegment seg[2];
-  int first1;  // CTAs below run segment 1 (the longer, shared one first), from here on segment 0
-  const uint16_t* q;
-  uint16_t* o;
-  float* part_o;   // [slot][row][DV], null: one item per row, written to o
-  float2* part_ml; // [slot][row] (m, l)
-  int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
-  int B, HQ, HKV, group, TQ, D, DV, causal;
-  const long long* counts;  // valid keys of each sequence, or null
-  // mask rows: (b * mask_sb + h * mask_sh + t * mask_st)
-  int64_t mask_sb, mask_sh, mask_st;
-  const unsigned long long* bits;  // packed boolean mask [row][words]
-  const int4* spans;               // per mask row: first and end visible key of segments 0 and 1
-  const void* add;                 // additive mask [row][mask_len]
-  int words, mask_len, add_f32, add_vec;
-  float scale_log2;
-  int* err;
-};
-
-struct RowId {
-  int b, h, t;
-};
-
-__device__ __forceinline__ RowId row_of(const FlashParams& p, int r, int kvh, int b, bool shared) {
-  const int g = r % p.group, bt = r / p.group;
-  RowId id;
-  id.h = kvh * p.group + g;
-  id.b = shared ? bt / p.TQ : b;
-  id.t = shared ? bt - id.b * p.TQ : bt;
-  return id;
-}
-
-__device__ __forceinline__ float mask_value(const FlashParams& p, int64_t at) {
-  if (p.add_f32) {
-    // Finite entries beyond 2^24 count as 2^24: no score reaches across that, and the differences formed
-    // below stay finite.  -inf (and NaN) stay.
-    const float v = __ldg(static_cast<const float*>(p.add) + at);
-    return v > 0x1p24f ? 0x1p24f : (v < -0x1p24f && v > -INFINITY ? -0x1p24f : v);
-  }
-  return __half2float(__ldg(static_cast<const __half*>(p.add) + at));
-}
 
 template <int NS, int MASK>
-__global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const __grid_constant__ FlashParams p) {
+__global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const __grid_constant__ TileParams p) {
   constexpr uint32_t QTILE = NS * AFK_QSLAB, KTILE = NS * AFK_KSLAB;
   constexpr int ST = NS == 1 ? 4 : 2;  // K and V stages: 64 KB of loads in flight per CTA at either head size
   extern __shared__ __align__(1024) uint8_t afk_raw[];
@@ -148,17 +90,16 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
   int* const err = p.err;
 
   // ---------------- work item
-  const int si = (int)blockIdx.x < p.first1 ? 1 : 0;
-  const FlashSegment& sg = p.seg[si];
-  int id = (int)blockIdx.x - (si ? 0 : p.first1);
-  const int split = id % sg.splits;
-  id /= sg.splits;
-  const int tile = sg.tiles - 1 - id % sg.tiles;  // later tokens, which see more keys, first
-  id /= sg.tiles;
+  const bool shared = (int)blockIdx.x < p.first1;  // rows of every sequence
+  const ItemClass& cl = p.cls[shared ? 1 : 0];
+  int id = (int)blockIdx.x - (shared ? 0 : p.first1);
+  const int split = id % cl.splits;
+  id /= cl.splits;
+  const int tile = cl.tiles - 1 - id % cl.tiles;  // later tokens, which see more keys, first
+  id /= cl.tiles;
   const int kvh = id % p.HKV;
-  const int b = id / p.HKV;  // 0 for a shared segment
-  const bool shared = sg.shared != 0;
-  const int rows_all = p.TQ * p.group * (shared ? p.B : 1);
+  const int b = id / p.HKV;  // 0 for rows of every sequence
+  const int rows_all = (int)(p.TQ.d * p.group.d) * (shared ? p.B : 1);
   const int row0 = tile * AFK_M;
   const int rows = min(AFK_M, rows_all - row0);
   const int nact = (rows + 31) >> 5;  // softmax warps with rows
@@ -193,7 +134,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
     const int c = i % (NS * 8), r = i / (NS * 8);
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (r < rows && c * 8 < p.D) {
-      const RowId w = row_of(p, row0 + r, kvh, b, shared);
+      const RowId w = row_of(row0 + r, p.group, p.TQ, kvh, b, shared);
       v = *reinterpret_cast<const uint4*>(p.q + (int64_t)w.b * p.q_sb + (int64_t)w.h * p.q_sh + (int64_t)w.t * p.q_st +
                                           c * 8);
     }
@@ -201,26 +142,31 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
   }
   fence_async_shared();
 
-  // ---------------- keys that some row of the work item sees
-  int kbeg = 0, kend = sg.keys;
-  if (sg.limited) {
-    if (p.causal) kend = min(kend, (row0 + rows - 1) / p.group + 1);  // segment 0 is never shared
+  // ---------------- keys that some row of the work item sees: key tiles, the past's first.  Positions count
+  // through the tiles: past key k is position k, current key k is position np * AFK_N + k.
+  const int np = cl.past ? (p.tp + AFK_N - 1) / AFK_N : 0;
+  int keys = shared ? 0 : p.tk;
+  if (!shared) {
+    if (p.causal) keys = min(keys, p.group.div(row0 + rows - 1) + 1);
     if (p.counts) {
       const long long n = p.counts[b];
-      if (n < 0 || n > sg.keys) record_error(err, DEV_BAD_INDEX);
-      kend = min(kend, (int)max(0ll, min(n, (long long)sg.keys)));
+      if (n < 0 || n > p.tk) record_error(err, DEV_BAD_INDEX);
+      keys = min(keys, (int)max(0ll, min(n, (long long)p.tk)));
     }
   }
-  const int row_keys = kend;  // before the mask's span: the count limit of every row
-  __syncthreads();            // span initialised
+  int pbeg = 0, pend = keys > 0 ? np * AFK_N + keys : (cl.past ? p.tp : 0);
+  __syncthreads();  // span initialised
   if (MASK == MASK_BITS) {
     if (threadIdx.x < rows) {
-      const RowId w = row_of(p, row0 + threadIdx.x, kvh, b, shared);
+      const RowId w = row_of(row0 + threadIdx.x, p.group, p.TQ, kvh, b, shared);
       const int4 v = p.spans[w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st];
-      const int lo = si ? v.z : v.x, hi = si ? v.w : v.y;
-      if (lo < hi) {
-        atomicMin(&span[0], lo);
-        atomicMax(&span[1], hi);
+      if (cl.past && v.z < v.w) {
+        atomicMin(&span[0], v.z);
+        atomicMax(&span[1], v.w);
+      }
+      if (!shared && v.x < v.y) {
+        atomicMin(&span[0], np * AFK_N + v.x);
+        atomicMax(&span[1], np * AFK_N + v.y);
       }
     }
   }
@@ -229,37 +175,38 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
   tc_fence_after();
   const uint32_t tmem = *holder;
   if (MASK == MASK_BITS) {
-    kbeg = span[0];
-    kend = min(kend, span[1]);
+    pbeg = span[0];
+    pend = min(pend, span[1]);
   }
-  // this split's share of the 64-key tiles
-  const int j_lo = kbeg < kend ? kbeg / AFK_N : 0, j_hi = kbeg < kend ? (kend + AFK_N - 1) / AFK_N : 0;
+  // this split's share of the tiles
+  const int j_lo = pbeg < pend ? pbeg / AFK_N : 0, j_hi = pbeg < pend ? (pend + AFK_N - 1) / AFK_N : 0;
   const int per = j_hi - j_lo;
-  const int j0 = j_lo + (int)((long long)per * split / sg.splits);
-  const int J = j_lo + (int)((long long)per * (split + 1) / sg.splits) - j0;
+  const int j0 = j_lo + (int)((long long)per * split / cl.splits);
+  const int J = j_lo + (int)((long long)per * (split + 1) / cl.splits) - j0;
 
   if (warp == 0) {
     if (lane == 0 && J > 0) {
       // ---------------- producer
-      const int kb = shared ? 0 : b;
       bool ok = true;
       int issued = 0;
       for (int j = 0; j < J && ok; ++j) {
-        const int s = j % ST, key0 = (j0 + j) * AFK_N;
+        const int s = j % ST, jj = j0 + j;
+        const int in_past = jj < np ? 1 : 0, key0 = (in_past ? jj : jj - np) * AFK_N;
+        const int kb = in_past && p.past_shared ? 0 : b;
         const uint32_t ph = (uint32_t)(j / ST - 1) & 1u;
         if (j >= ST && !mbar_wait(&k_empty[s], ph, err, DEV_TIMEOUT_PRODUCER)) ok = false;
         if (!ok) break;
         mbar_arrive_expect_tx(&k_full[s], KTILE);
 #pragma unroll
         for (int c = 0; c < NS; ++c)
-          tma_load_4d(s_k + s * KTILE + c * AFK_KSLAB, &sg.map_k, &k_full[s], 64 * c, key0, kvh, kb);
+          tma_load_4d(s_k + s * KTILE + c * AFK_KSLAB, &p.map_k[in_past], &k_full[s], 64 * c, key0, kvh, kb);
         issued = 2 * j + 1;
         if (j >= ST && !mbar_wait(&v_empty[s], ph, err, DEV_TIMEOUT_PRODUCER)) ok = false;
         if (!ok) break;
         mbar_arrive_expect_tx(&v_full[s], KTILE);
 #pragma unroll
         for (int c = 0; c < NS; ++c)
-          tma_load_4d(s_v + s * KTILE + c * AFK_KSLAB, &sg.map_v, &v_full[s], 64 * c, key0, kvh, kb);
+          tma_load_4d(s_v + s * KTILE + c * AFK_KSLAB, &p.map_v[in_past], &v_full[s], 64 * c, key0, kvh, kb);
         issued = 2 * j + 2;
       }
       if (!ok) {  // error path: let the copies in flight land before the CTA exits
@@ -301,7 +248,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         const int s = j % ST;
         bool ok = mbar_wait(&v_full[s], (uint32_t)(j / ST) & 1u, err, DEV_TIMEOUT_MMA);
         if (!__all_sync(0xffffffffu, ok)) break;
-        const int nv = kend - (j0 + j) * AFK_N;
+        const int nv = pend - (j0 + j) * AFK_N;
         if (nv < AFK_N) {  // keys past the last visible one: their values take no part
           for (int i = lane; i < (AFK_N - nv) * 8 * NS; i += 32) {
             const int c = i % (8 * NS), r = nv + i / (8 * NS);
@@ -336,24 +283,32 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const bool live = r < rows;
-    const RowId w = row_of(p, row0 + (live ? r : 0), kvh, b, shared);
+    const RowId w = row_of(row0 + (live ? r : 0), p.group, p.TQ, kvh, b, shared);
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    int row_end = row_keys;  // end of the keys this row may see
-    if (sg.limited && p.causal) row_end = min(row_end, w.t + 1);
+    const int row_end = p.causal ? min(keys, w.t + 1) : keys;  // end of the current keys this row may see
     const int64_t mrow = MASK == MASK_NONE ? 0 : w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st;
     float m_used = -INFINITY;  // reference of the exponentials, log2 units
     float l = 0.0f;            // sum of the fp16-rounded weights
     const float sc = p.scale_log2;
     const bool pos = sc > 0.0f;
+    const unsigned long long* words = MASK == MASK_BITS ? p.bits + mrow * p.words + (cl.past ? 0 : p.words_past) + j0 : nullptr;
+    unsigned long long word = MASK == MASK_BITS && J > 0 ? words[0] : 0ull;  // the next tile's, loaded a tile ahead
     bool ok = true;
     for (int j = 0; j < J && ok; ++j) {
-      const int sb = j & 1, key0 = (j0 + j) * AFK_N;
+      const int sb = j & 1, jj = j0 + j;
+      const bool in_past = jj < np;
+      const int key0 = (in_past ? jj : jj - np) * AFK_N;
       // visible keys of the tile, one bit each
       unsigned long long vis = ~0ull;
-      if (row_end - key0 < AFK_N) vis = row_end > key0 ? (1ull << (row_end - key0)) - 1 : 0ull;
-      if (MASK == MASK_BITS) vis &= p.bits[mrow * p.words + sg.word_off + (j0 + j)];
+      const int end = (in_past ? p.tp : row_end) - key0;
+      if (end < AFK_N) vis = end > 0 ? (1ull << end) - 1 : 0ull;
+      if (MASK == MASK_BITS) {
+        vis &= word;
+        if (j + 1 < J) word = words[j + 1];
+      }
+      const int mask_at = (in_past ? 0 : p.tp) + key0;  // the tile's first key in a mask row
       if (MASK == MASK_ADD) {  // keys past a short mask are not seen
-        const int left = p.mask_len - sg.mask_off - key0;
+        const int left = p.mask_len - mask_at;
         if (left < AFK_N) vis &= left > 0 ? (1ull << left) - 1 : 0ull;
       }
       ok = mbar_wait(&s_full[sb], (uint32_t)(j >> 1) & 1u, err, DEV_TIMEOUT_EPILOGUE);
@@ -389,7 +344,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       float mx;
       if (MASK == MASK_ADD) {
         // pass 1: -inf mask entries hide their key; the maximum of the masked scores (any value near it will do)
-        const int64_t at = mrow * p.mask_len + sg.mask_off + key0;
+        const int64_t at = mrow * p.mask_len + mask_at;
         mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -408,7 +363,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
               }
             } else {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) mk[e] = (half & (1u << (i + e))) ? mask_value(p, at + 32 * c + i + e) : 0.0f;
+              for (int e = 0; e < 8; ++e) mk[e] = (half & (1u << (i + e))) ? additive_entry(p.add, p.add_f32, at + 32 * c + i + e) : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -436,7 +391,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       uint32_t pw[2][16];
       float lp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       if (MASK == MASK_ADD) {
-        const int64_t at = mrow * p.mask_len + sg.mask_off + key0;
+        const int64_t at = mrow * p.mask_len + mask_at;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
@@ -454,7 +409,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
               }
             } else {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) mk[e] = (half & (1u << (i + e))) ? mask_value(p, at + 32 * c + i + e) : 0.0f;
+              for (int e = 0; e < 8; ++e) mk[e] = (half & (1u << (i + e))) ? additive_entry(p.add, p.add_f32, at + 32 * c + i + e) : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -527,8 +482,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       tc_fence_after();
       const bool part = p.part_o != nullptr;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int64_t row = ((int64_t)w.b * p.TQ + w.t) * p.HQ + w.h;
-      const int64_t slot_row = (int64_t)(sg.part0 + split) * ((int64_t)p.B * p.TQ * p.HQ) + row;
+      const int64_t row = ((int64_t)w.b * (int)p.TQ.d + w.t) * p.HQ + w.h;
+      const int64_t slot_row = (int64_t)(cl.part0 + split) * ((int64_t)p.B * (int)p.TQ.d * p.HQ) + row;
       uint16_t* orow = p.o + (int64_t)w.b * p.o_sb + (int64_t)w.h * p.o_sh + (int64_t)w.t * p.o_st;
       float* prow = part ? p.part_o + slot_row * p.DV : nullptr;
       if (part && live) p.part_ml[slot_row] = make_float2(m_used, l);
@@ -631,21 +586,29 @@ __global__ void __launch_bounds__(256) mask_pack_kernel(const uint8_t* __restric
   const int64_t row = blockIdx.x;
   const uint8_t* src = mask + row * len;
   int lo[2] = {0x7fffffff, 0x7fffffff}, hi[2] = {0, 0};
-#pragma unroll 4
-  for (int wd = warp; wd < words; wd += 8) {
-    const int seg = wd < words1 ? 1 : 0;
-    const int k0 = (seg ? wd : wd - words1) * 64;         // within the segment
-    const int n = seg ? past : keys, base = seg ? 0 : past;
-    const int ka = k0 + lane, kb = ka + 32;
-    const bool va = ka < n && base + ka < len && src[base + ka] != 0;
-    const bool vb = kb < n && base + kb < len && src[base + kb] != 0;
-    const uint32_t wa = __ballot_sync(0xffffffffu, va), wb = __ballot_sync(0xffffffffu, vb);
-    const unsigned long long w = (unsigned long long)wa | ((unsigned long long)wb << 32);
-    if (lane == 0) bits[row * words + wd] = w;
-    if (w) {
-      lo[seg] = min(lo[seg], k0 + __ffsll((long long)w) - 1);
-      hi[seg] = max(hi[seg], k0 + 64 - __clzll((long long)w));
+  // a warp takes eight consecutive words at a time and loads them all before the first ballot
+  for (int w0 = warp * 8; w0 < words; w0 += 64) {
+    bool v[8][2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int wd = w0 + i, seg = wd < words1 ? 1 : 0;
+      const int ka = (seg ? wd : wd - words1) * 64 + lane, n = seg ? past : keys, base = seg ? 0 : past;
+      v[i][0] = wd < words && ka < n && base + ka < len && src[base + ka] != 0;
+      v[i][1] = wd < words && ka + 32 < n && base + ka + 32 < len && src[base + ka + 32] != 0;
     }
+    unsigned long long mine = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t wa = __ballot_sync(0xffffffffu, v[i][0]), wb = __ballot_sync(0xffffffffu, v[i][1]);
+      const unsigned long long w = (unsigned long long)wa | ((unsigned long long)wb << 32);
+      if (lane == i) mine = w;
+      const int seg = w0 + i < words1 ? 1 : 0, k0 = (seg ? w0 + i : w0 + i - words1) * 64;
+      if (w) {
+        lo[seg] = min(lo[seg], k0 + __ffsll((long long)w) - 1);
+        hi[seg] = max(hi[seg], k0 + 64 - __clzll((long long)w));
+      }
+    }
+    if (lane < 8 && w0 + lane < words) bits[row * words + w0 + lane] = mine;
   }
   if (lane < 2 && hi[lane]) {
     atomicMin(&s_span[2 * lane], lo[lane]);
@@ -661,7 +624,7 @@ static size_t flash_smem(int ns) {
   return (size_t)ns * AFK_QSLAB + 2 * (size_t)st * ns * AFK_KSLAB + AFK_QSLAB + 256;
 }
 
-typedef void (*FlashKernel)(const FlashParams);
+typedef void (*FlashKernel)(const TileParams);
 
 static FlashKernel flash_kernel(int ns, int mask) {
   static const FlashKernel table[2][3] = {
@@ -678,6 +641,11 @@ int prepare_attention_flash(const PlanOp& op, void* const*, OpState*, int, char*
   const int64_t d = op.ip[AF_D], dv = op.ip[AF_DV];
   if (d < 8 || d > 128 || d % 8 || dv < 8 || dv > 128 || dv % 8)
     return fail(msg, n, 5, "Attention: head sizes %lld/%lld, needs multiples of 8 up to 128", (long long)d, (long long)dv);
+  if (op.ip[AF_K_ST] > 0x7fffffff || op.ip[AF_V_ST] > 0x7fffffff)
+    return fail(msg, n, 5, "Attention: key stride of more than 2^31 elements");
+  cudaError_t re = prepare_attention_rows();
+  if (re == cudaSuccess) re = prepare_attention_wide();
+  if (re != cudaSuccess) return fail(msg, n, 4, "cudaFuncSetAttribute: %s", cudaGetErrorString(re));
   for (int s = AF_Q_SB; s <= AF_O_ST; ++s)
     if (op.ip[s] % 8) return fail(msg, n, 5, "Attention: strides must be 16-byte multiples");
   for (int ns = 1; ns <= 2; ++ns)
@@ -690,14 +658,14 @@ int prepare_attention_flash(const PlanOp& op, void* const*, OpState*, int, char*
 }
 
 // 4-D map (d, t, h, b) over an fp16 tensor with element strides (1, st, sh, sb),
-// boxes of 64 d x 64 tokens.
+// boxes of 64 d x `tile_keys` tokens.
 static int make_tmap_kv(CUtensorMap* map, const void* base, int64_t d, int64_t t, int64_t heads, int64_t batch,
-                        int64_t st, int64_t sh, int64_t sb) {
+                        int64_t st, int64_t sh, int64_t sb, int tile_keys) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc || ((uintptr_t)base & 15u)) return 5;
   cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)t, (cuuint64_t)heads, (cuuint64_t)batch};
   cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)AFK_N, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)tile_keys, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -705,99 +673,144 @@ static int make_tmap_kv(CUtensorMap* map, const void* base, int64_t d, int64_t t
   return r == CUDA_SUCCESS ? 0 : 4;
 }
 
+// Fills what the tile pass needs beside the rows' parameters.
+static int tile_params(TileParams& p, const PlanOp& op, const RowsParams& r, const ItemClass* cls, int first1,
+                       int tile_keys) {
+  p.cls[0] = cls[0], p.cls[1] = cls[1], p.first1 = first1;
+  p.q = r.q, p.o = r.o, p.part_o = r.part_o, p.part_ml = r.part_ml;
+  p.q_sb = r.q_sb, p.q_sh = r.q_sh, p.q_st = r.q_st, p.o_sb = r.o_sb, p.o_sh = r.o_sh, p.o_st = r.o_st;
+  p.B = r.B, p.HQ = r.HQ, p.HKV = r.HKV, p.group = r.group, p.TQ = r.TQ, p.D = r.D, p.DV = r.DV;
+  p.causal = r.causal, p.tk = r.tk, p.tp = r.tp, p.past_shared = r.past_shared;
+  p.counts = r.counts;
+  p.mask_sb = r.mask_sb, p.mask_sh = r.mask_sh, p.mask_st = r.mask_st;
+  p.add = r.mask_add, p.add_f32 = r.add_f32, p.mask_len = r.mask_len;
+  // 16-byte reads of 8 fp16 entries: every row and both parts of the keys start on 16 bytes
+  p.add_vec = p.add && !p.add_f32 && p.mask_len % 8 == 0 && p.tp % 8 == 0 && ((uintptr_t)p.add & 15u) == 0;
+  p.scale_log2 = r.scale_log2;
+  p.err = r.err;
+  int rc = make_tmap_kv(&p.map_k[0], r.k, p.D, p.tk, p.HKV, p.B, r.k_st, r.k_sh, r.k_sb, tile_keys);
+  if (!rc) rc = make_tmap_kv(&p.map_v[0], r.v, p.DV, p.tk, p.HKV, p.B, r.v_st, r.v_sh, r.v_sb, tile_keys);
+  if (p.tp > 0) {
+    const int copies = p.past_shared ? 1 : p.B;
+    if (!rc)
+      rc = make_tmap_kv(&p.map_k[1], r.past_k, p.D, p.tp, p.HKV, copies, p.D, (int64_t)p.tp * p.D,
+                        (int64_t)p.HKV * p.tp * p.D, tile_keys);
+    if (!rc)
+      rc = make_tmap_kv(&p.map_v[1], r.past_v, p.DV, p.tp, p.HKV, copies, p.DV, (int64_t)p.tp * p.DV,
+                        (int64_t)p.HKV * p.tp * p.DV, tile_keys);
+  }
+  return rc;
+}
+
 int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, const LaunchCtx& ctx, int* launches) {
-  FlashParams p{};
+  RowsParams r{};
   const int64_t* s = &op.ip[AF_Q_SB];
   auto ptr = [&](int i) -> void* { return op.t[i] >= 0 ? ptrs[op.t[i]] : nullptr; };
-  p.B = (int)eff_batch(ctx, op, op.ip[AF_B]);
-  p.HQ = (int)op.ip[AF_HQ];
-  p.HKV = (int)op.ip[AF_HKV];
-  p.group = p.HQ / p.HKV;
-  p.TQ = (int)op.ip[AF_TQ];
-  p.D = (int)op.ip[AF_D];
-  p.DV = (int)op.ip[AF_DV];
-  p.causal = (int)op.ip[AF_CAUSAL];
-  p.scale_log2 = (float)(op.fp[AFF_SCALE] * 1.4426950408889634);
-  p.q = (const uint16_t*)ptr(0);
-  p.o = (uint16_t*)ptr(3);
-  p.q_sb = s[0], p.q_sh = s[1], p.q_st = s[2];
-  p.o_sb = s[9], p.o_sh = s[10], p.o_st = s[11];
-  p.err = ctx.d_error;
-  if (p.B <= 0 || p.TQ <= 0) return 0;
-  if (((uintptr_t)p.q | (uintptr_t)p.o) & 15u) return 5;
-  if ((uintptr_t)ptr(7) & 7u) return 5;
-  const int tk = (int)op.ip[AF_TK], tp = (int)op.ip[AF_TP];
-  const int64_t rows = (int64_t)p.B * p.TQ * p.HQ;
+  r.B = (int)eff_batch(ctx, op, op.ip[AF_B]);
+  r.HQ = (int)op.ip[AF_HQ];
+  r.HKV = (int)op.ip[AF_HKV];
+  const int64_t group = r.HQ / r.HKV, tq = op.ip[AF_TQ];
+  r.group = SmallDiv::of((uint32_t)group);
+  r.TQ = SmallDiv::of((uint32_t)tq);
+  r.D = (int)op.ip[AF_D];
+  r.DV = (int)op.ip[AF_DV];
+  r.causal = (int)op.ip[AF_CAUSAL];
+  r.tk = (int)op.ip[AF_TK];
+  r.tp = (int)op.ip[AF_TP];
+  r.past_shared = (int)op.ip[AF_PAST_SHARED];
+  r.scale_log2 = (float)(op.fp[AFF_SCALE] * 1.4426950408889634);
+  r.q = (const uint16_t*)ptr(0), r.k = (const uint16_t*)ptr(1), r.v = (const uint16_t*)ptr(2);
+  r.past_k = (const uint16_t*)ptr(5), r.past_v = (const uint16_t*)ptr(6);
+  r.o = (uint16_t*)ptr(3);
+  r.q_sb = s[0], r.q_sh = s[1], r.q_st = s[2], r.k_sb = s[3], r.k_sh = s[4], r.k_st = s[5];
+  r.v_sb = s[6], r.v_sh = s[7], r.v_st = s[8], r.o_sb = s[9], r.o_sh = s[10], r.o_st = s[11];
+  r.counts = (const long long*)ptr(7);
+  r.err = ctx.d_error;
+  if (r.B <= 0 || tq <= 0) return 0;
+  for (int i : {0, 1, 2, 3, 5, 6})
+    if ((uintptr_t)ptr(i) & 15u) return 5;
+  if ((uintptr_t)r.counts & 7u) return 5;
+  const int kind = (int)op.ip[AF_MASK_KIND];
+  const int variant = kind == AF_MASK_NONE ? MASK_NONE : kind == AF_MASK_BOOL ? MASK_BITS : MASK_ADD;
+  r.mask_sb = op.ip[AF_MASK_SB], r.mask_sh = op.ip[AF_MASK_SH], r.mask_st = op.ip[AF_MASK_ST];
+  r.mask_len = (int)op.ip[AF_MASK_LEN];
+  r.mask_bool = variant == MASK_BITS ? (const uint8_t*)ptr(4) : nullptr;
+  r.mask_add = variant == MASK_ADD ? ptr(4) : nullptr;
+  r.add_f32 = kind == AF_MASK_F32;
+  if (variant == MASK_ADD && ((uintptr_t)r.mask_add & (r.add_f32 ? 3u : 1u))) return 5;
 
-  FlashSegment& cur = p.seg[0];
-  cur.keys = tk;
-  cur.mask_off = tp;
-  cur.shared = 0;
-  cur.limited = 1;
-  cur.splits = (int)op.ip[AF_SPLITS_K];
-  cur.tiles = (p.TQ * p.group + AFK_M - 1) / AFK_M;
-  cur.part0 = 0;
-  int rc = make_tmap_kv(&cur.map_k, ptr(1), p.D, tk, p.HKV, p.B, s[5], s[4], s[3]);
-  if (!rc) rc = make_tmap_kv(&cur.map_v, ptr(2), p.DV, tk, p.HKV, p.B, s[8], s[7], s[6]);
-  int64_t items = (int64_t)p.B * p.HKV * cur.tiles * cur.splits;
-  int slots = cur.splits;
-  FlashSegment& past = p.seg[1];
-  if (tp > 0 && !rc) {
-    past.keys = tp;
-    past.shared = (int)op.ip[AF_PAST_SHARED];
-    past.splits = (int)op.ip[AF_SPLITS_P];
-    const int64_t packed = (int64_t)p.TQ * p.group * (past.shared ? p.B : 1);
-    past.tiles = (int)((packed + AFK_M - 1) / AFK_M);
-    past.part0 = cur.splits;
-    const int copies = past.shared ? 1 : p.B;
-    rc = make_tmap_kv(&past.map_k, ptr(5), p.D, tp, p.HKV, copies, p.D, (int64_t)tp * p.D, (int64_t)p.HKV * tp * p.D);
-    if (!rc)
-      rc = make_tmap_kv(&past.map_v, ptr(6), p.DV, tp, p.HKV, copies, p.DV, (int64_t)tp * p.DV,
-                        (int64_t)p.HKV * tp * p.DV);
-    p.first1 = copies * p.HKV * past.tiles * past.splits;
-    items += p.first1;
-    slots += past.splits;
+  // ---------------- work items of the two classes
+  const int64_t rows = (int64_t)r.B * tq * r.HQ;
+  const int pass_own = (int)op.ip[AF_PASS_OWN], pass_past = (int)op.ip[AF_PASS_PAST];
+  const bool apart = r.tp > 0 && pass_past != AF_PASS_NONE;  // a shared past in items of its own
+  auto tiles_of = [](int64_t n, int pass) {
+    const int m = pass == AF_PASS_ROWS8 ? 8 : pass == AF_PASS_ROWS16 ? 16 : pass == AF_PASS_WIDE ? 2 * AFK_M : AFK_M;
+    return (int)((n + m - 1) / m);
+  };
+  ItemClass cls[2] = {};
+  cls[0].splits = (int)op.ip[AF_SPLITS_K];
+  cls[0].tiles = tiles_of(tq * group, pass_own);
+  cls[0].past = r.tp > 0 && !apart;
+  int64_t items[2] = {(int64_t)r.B * r.HKV * cls[0].tiles * cls[0].splits, 0};
+  int slots = cls[0].splits;
+  if (apart) {
+    cls[1].splits = (int)op.ip[AF_SPLITS_P];
+    cls[1].tiles = tiles_of(r.B * tq * group, pass_past);
+    cls[1].part0 = slots;
+    cls[1].past = 1;
+    items[1] = (int64_t)r.HKV * cls[1].tiles * cls[1].splits;
+    slots += cls[1].splits;
   }
-  if (rc) return rc;
-  if (items > 0x7fffffff) return 5;
+  // (SmallDiv: rows divided by the group, and, against a shared past, by the tokens)
+  if (items[0] + items[1] > 0x7fffffff || (apart ? r.B : 1) * tq * group * group > 0xffffffffll ||
+      (apart && r.B * tq * tq > 0xffffffffll))
+    return 5;
   if (slots > 1) {
     // (m, l) pairs behind the outputs, both sized for the compiled batch
-    p.part_o = (float*)ptr(8);
-    p.part_ml = (float2*)(p.part_o + (int64_t)slots * rows * p.DV);
+    r.part_o = (float*)ptr(8);
+    r.part_ml = (float2*)(r.part_o + (int64_t)slots * rows * r.DV);
   }
-  p.counts = (const long long*)ptr(7);
-  int variant = MASK_NONE;
-  const int kind = (int)op.ip[AF_MASK_KIND];
-  p.mask_sb = op.ip[AF_MASK_SB], p.mask_sh = op.ip[AF_MASK_SH], p.mask_st = op.ip[AF_MASK_ST];
-  p.mask_len = (int)op.ip[AF_MASK_LEN];
-  if (kind == AF_MASK_BOOL) {
-    variant = MASK_BITS;
-    const int words1 = (tp + 63) / 64, words = words1 + (tk + 63) / 64;
-    const int64_t mrows = p.mask_sb ? p.mask_sb * p.B : op.ip[AF_MASK_ROWS];
-    cur.word_off = words1;
-    p.words = words;
-    p.spans = (const int4*)ptr(9);
-    p.bits = (const unsigned long long*)(p.spans + mrows);
-    cudaError_t e = launch_pdl(mask_pack_kernel, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, (const uint8_t*)ptr(4),
-                               p.mask_len, tp, tk, words1, words, (unsigned long long*)p.bits, (int4*)p.spans);
+
+  // ---------------- passes: one kernel for both classes, or the past's first and the own keys' beside it
+  auto is_rows = [](int pass) { return pass == AF_PASS_ROWS8 || pass == AF_PASS_ROWS16; };
+  const bool together = !apart || pass_own == pass_past;
+  cudaError_t e = cudaSuccess;
+  for (int step = together ? 1 : 0; step < 2 && e == cudaSuccess; ++step) {
+    const int pass = together ? pass_own : (step == 0 ? pass_past : pass_own);
+    const int64_t n1 = together ? items[1] : (step == 0 ? items[1] : 0);
+    const int64_t n0 = together || step == 1 ? items[0] : 0;
+    if (is_rows(pass)) {
+      r.cls[0] = cls[0], r.cls[1] = cls[1], r.first1 = (int)n1;
+      r.late_wait = !together;
+      e = launch_attention_rows(r, pass == AF_PASS_ROWS8 ? 1 : 2, variant, (int)op.ip[AF_WARPS], (unsigned)(n0 + n1), ctx.stream);
+    } else {
+      TileParams p{};
+      const int tile_keys = pass == AF_PASS_WIDE ? 128 : AFK_N;
+      if (pass == AF_PASS_WIDE && variant == MASK_ADD) return 5;  // (never planned)
+      int rc = tile_params(p, op, r, cls, (int)n1, tile_keys);
+      if (rc) return rc;
+      if (variant == MASK_BITS) {
+        const int64_t mrows = p.mask_sb ? p.mask_sb * p.B : op.ip[AF_MASK_ROWS];
+        p.words_past = (p.tp + tile_keys - 1) / tile_keys * (tile_keys / 64);
+        p.words = p.words_past + (p.tk + tile_keys - 1) / tile_keys * (tile_keys / 64);
+        p.spans = (const int4*)ptr(9);
+        p.bits = (const unsigned long long*)(p.spans + mrows);
+        e = launch_pdl(mask_pack_kernel, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, r.mask_bool, p.mask_len, p.tp,
+                       p.tk, p.words_past, p.words, (unsigned long long*)p.bits, (int4*)p.spans);
+        ++*launches;
+        if (e != cudaSuccess) return 4;
+      }
+      const int ns = flash_slabs(op);
+      e = pass == AF_PASS_WIDE ? launch_attention_wide(p, ns, variant, (unsigned)(n0 + n1), ctx.stream)
+                               : launch_pdl(flash_kernel(ns, variant), dim3((unsigned)(n0 + n1)), dim3(AFK_THREADS),
+                                            flash_smem(ns), ctx.stream, p);
+    }
     ++*launches;
-    if (e != cudaSuccess) return 4;
-  } else if (kind != AF_MASK_NONE) {
-    variant = MASK_ADD;
-    p.add = ptr(4);
-    p.add_f32 = kind == AF_MASK_F32;
-    if ((uintptr_t)p.add & (p.add_f32 ? 3u : 1u)) return 5;
-    // 16-byte reads of 8 fp16 entries: every row and both segments start on 16 bytes
-    p.add_vec = kind == AF_MASK_F16 && p.mask_len % 8 == 0 && tp % 8 == 0 && ((uintptr_t)p.add & 15u) == 0;
   }
-  const int ns = flash_slabs(op);
-  cudaError_t e = launch_pdl(flash_kernel(ns, variant), dim3((unsigned)items), dim3(AFK_THREADS), flash_smem(ns),
-                             ctx.stream, p);
-  ++*launches;
   if (e == cudaSuccess && slots > 1) {
     e = launch_pdl(attention_combine_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx.stream,
-                   (const float*)p.part_o, (const float2*)p.part_ml, slots, rows, p.TQ, p.HQ, p.DV, p.o, p.o_sb, p.o_sh,
-                   p.o_st);
+                   (const float*)r.part_o, (const float2*)r.part_ml, slots, rows, (int)tq, r.HQ, r.DV, r.o, r.o_sb, r.o_sh,
+                   r.o_st);
     ++*launches;
   }
   return e == cudaSuccess ? 0 : 4;

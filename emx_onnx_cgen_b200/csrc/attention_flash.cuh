@@ -1,0 +1,112 @@
+// What the passes of K_ATTENTION_FLASH share: how query rows are packed, the
+// additive mask's entries, and the few-row pass (attention_rows.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace emx {
+
+constexpr float AFK_RESCALE = 8.0f;  // the output is rescaled when a row's maximum grows by more (log2 units)
+constexpr float AFK_LOG2E = 1.4426950408889634f;
+
+enum { MASK_NONE = 0, MASK_BITS = 1, MASK_ADD = 2 };  // kernel variants
+
+struct RowId {
+  int b, h, t;
+};
+
+// Division of the rows' small numbers by a launch's constant: n / d = (n * magic) >> 32 with magic = 2^32 / d + 1 is
+// exact while n * d < 2^32 (checked by the host; d = 1 has no 32-bit magic and is its own case).
+struct SmallDiv {
+  uint32_t d, magic;
+  __host__ static SmallDiv of(uint32_t d) { return {d, d > 1 ? (uint32_t)((1ull << 32) / d + 1) : 0u}; }
+  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, magic); }
+};
+
+// Row r of a work item's rows: (token, head of the group), tokens slowest, of
+// sequence b, or of every sequence one after the other.
+__device__ __forceinline__ RowId row_of(int r, const SmallDiv& group, const SmallDiv& TQ, int kvh, int b,
+                                        bool all_sequences) {
+  const int bt = group.div(r), g = r - bt * (int)group.d;
+  RowId id;
+  id.h = kvh * (int)group.d + g;
+  id.b = b, id.t = bt;
+  if (all_sequences) {
+    id.b = TQ.div(bt);
+    id.t = bt - id.b * (int)TQ.d;
+  }
+  return id;
+}
+
+__device__ __forceinline__ float additive_entry(const void* mask, int f32, int64_t at) {
+  if (f32) {
+    // Finite entries beyond 2^24 count as 2^24: no score reaches across that, and the differences formed
+    // from them stay finite.  -inf (and NaN) stay.
+    const float v = __ldg(static_cast<const float*>(mask) + at);
+    return v > 0x1p24f ? 0x1p24f : (v < -0x1p24f && v > -INFINITY ? -0x1p24f : v);
+  }
+  return __half2float(__ldg(static_cast<const __half*>(mask) + at));
+}
+
+// The work items of a pass come in two classes: 0, the rows of one sequence
+// against its own keys (behind its past where `past` is set: one list of key
+// tiles, the past's first), and 1, the rows of every sequence against a past
+// that they share.  Items of class 1 have the lower block indices.
+struct ItemClass {
+  int splits;  // items along the keys
+  int tiles;   // row tiles per key/value head (and sequence)
+  int part0;   // first slot of partial results
+  int past;
+};
+
+// The keys that the rows of a tile-pass item see, as a list of KT-key tiles.
+struct TileParams {
+  CUtensorMap map_k[2], map_v[2];  // current keys, past: 4-D (d, key, head, batch), box (64, KT, 1, 1), 128-byte swizzle
+  ItemClass cls[2];
+  int first1;
+  const uint16_t* q;
+  uint16_t* o;
+  float* part_o;    // [slot][row][DV], null: one item per row, written to o
+  float2* part_ml;  // [slot][row] (m, l)
+  int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
+  int B, HQ, HKV, D, DV, causal, tk, tp, past_shared;
+  SmallDiv group, TQ;
+  const long long* counts;  // valid current keys of each sequence, or null
+  int64_t mask_sb, mask_sh, mask_st;  // mask row of (b, h, t): b * sb + h * sh + t * st
+  const unsigned long long* bits;     // packed boolean mask [row][words], the past's words first
+  const int4* spans;                  // per mask row: first and end visible current key, first and end visible past key
+  const void* add;                    // additive mask [row][mask_len]
+  int words, words_past, mask_len, add_f32, add_vec;
+  float scale_log2;
+  int* err;
+};
+
+struct RowsParams {
+  ItemClass cls[2];
+  int first1;
+  const uint16_t *q, *k, *v, *past_k, *past_v;
+  uint16_t* o;
+  float* part_o;
+  float2* part_ml;
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, o_sb, o_sh, o_st;
+  int B, HQ, HKV, D, DV, causal, tp, tk, past_shared;
+  SmallDiv group, TQ;
+  const long long* counts;
+  int64_t mask_sb, mask_sh, mask_st;
+  const uint8_t* mask_bool;
+  const void* mask_add;
+  int mask_len, add_f32;
+  float scale_log2;
+  int late_wait;  // launched behind a pass whose results it does not read
+  int* err;
+};
+
+cudaError_t prepare_attention_wide();
+cudaError_t launch_attention_wide(const TileParams& p, int slabs, int mask, unsigned items, cudaStream_t stream);
+cudaError_t prepare_attention_rows();
+cudaError_t launch_attention_rows(const RowsParams& p, int row_tiles, int mask, int warps, unsigned items,
+                                  cudaStream_t stream);
+
+}  // namespace emx

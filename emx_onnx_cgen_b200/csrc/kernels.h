@@ -102,16 +102,20 @@ enum { ATF_SCALE };
 
 // ---- K_ATTENTION_FLASH: t[0]=Q, t[1]=K, t[2]=V, t[3]=Y (fp16), t[4]=mask|-1, t[5]=past K|-1, t[6]=past V|-1,
 //      t[7]=valid key counts i64 [B]|-1, t[8]=partial results f32|-1 (slots x rows x (DV + 2), slots = AF_SPLITS_K +
-//      AF_SPLITS_P, rows = B*TQ*HQ), t[9]=packed boolean mask|-1 (16 bytes per mask row, then 8 per 64 keys of each
-//      segment).  Element (b, h, t, d) of Q, K, V, Y sits at b*SB + h*SH + t*ST + d; the past is contiguous
+//      AF_SPLITS_P, rows = B*TQ*HQ), t[9]=packed boolean mask|-1 (16 bytes per mask row, then 8 per 64 keys of the past,
+//      a multiple of 128, and of the current keys).  Element (b, h, t, d) of Q, K, V, Y sits at b*SB + h*SH + t*ST + d; the past is contiguous
 //      [B or 1][HKV][TP][D].  Mask row of query (b, h, t): b*SB + h*SH + t*ST, each of AF_MASK_LEN keys, past first.
 enum {
   AF_B, AF_HQ, AF_HKV, AF_TQ, AF_TK, AF_TP, AF_D, AF_DV, AF_CAUSAL,
   AF_Q_SB, AF_Q_SH, AF_Q_ST, AF_K_SB, AF_K_SH, AF_K_ST, AF_V_SB, AF_V_SH, AF_V_ST, AF_O_SB, AF_O_SH, AF_O_ST,
-  AF_PAST_SHARED /*one past for every sequence*/, AF_SPLITS_K, AF_SPLITS_P /*work items along the keys*/,
-  AF_MASK_KIND, AF_MASK_SB, AF_MASK_SH, AF_MASK_ST, AF_MASK_ROWS, AF_MASK_LEN
+  AF_PAST_SHARED /*one past for every sequence*/, AF_PASS_OWN /*pass that runs a sequence's rows on its own keys*/,
+  AF_PASS_PAST /*pass of a shared past's items, NONE: the past's keys come first in a sequence's own items*/,
+  AF_SPLITS_K, AF_SPLITS_P /*work items along the keys*/, AF_WARPS /*of an item of attention_rows.cu*/, AF_MASK_KIND,
+  AF_MASK_SB, AF_MASK_SH, AF_MASK_ST, AF_MASK_ROWS, AF_MASK_LEN
 };
 enum { AFF_SCALE };
+enum { AF_PASS_NONE = 0, AF_PASS_ROWS8 = 1, AF_PASS_ROWS16 = 2 /*attention_rows.cu*/, AF_PASS_TILES = 3 /*attention_flash.cu*/,
+       AF_PASS_WIDE = 4 /*attention_wide.cu*/ };
 enum { AF_MASK_NONE = 0, AF_MASK_BOOL = 1, AF_MASK_F16 = 2, AF_MASK_F32 = 3 };
 
 // ---- K_RMS_NORM: t[0]=x, t[1]=scale, t[2]=y; rows of RN_N contiguous elements

@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "f32x2.cuh"
 #include "host_util.h"
 #include "kernels.h"
 #include "tc100.cuh"
@@ -41,7 +42,9 @@ struct RopeParams {
   const void *cos, *sin;
   const long long* pos;
   int64_t tokens;
-  int T, D, rot, interleaved, heads /*of both items*/, groups /*lane groups per token*/;
+  int T, D, rot, interleaved, heads /*of both items*/;
+  int groups[2];  // lane groups per token of each item
+  float inv_d;
   int64_t positions;
   int* err;
 };
@@ -96,9 +99,18 @@ __device__ __forceinline__ int64_t table_row(const RopeParams& p, int64_t token)
   return -1;
 }
 
+// 1 / sqrt(v) to fp32 accuracy: the hardware estimate and one Newton step.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float y = rsqrtf(v);
+  return fmaf(y * 0.5f, fmaf(-v * y, y, 1.0f), y);
+}
+
 // Vector form: D and the rotated halves are whole 16-byte pieces, every row starts on 16 bytes.
-template <typename T, int LPR, int HPG>
-__global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ RopeParams p) {
+// A lane's two pieces hold V pairs (f, s): (piece 0, piece 1) element by element, or neighbours of one piece
+// (INTER).  Norm scale and rotation make one 2 x 2 matrix per pair, formed once for the group's rows:
+//   f' = inv (f wf cos - s ws sin),  s' = inv (f wf sin + s ws cos).
+template <typename T, int LPR, int HPG, bool INTER>
+__global__ void __launch_bounds__(256, 3) norm_rope_kernel(const __grid_constant__ RopeParams p) {
   constexpr int V = Chunk<T>::N;
   pdl_wait();
   pdl_launch_dependents();
@@ -106,97 +118,117 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
   const int u = threadIdx.x % LPR;
   // lanes of one group take the same path throughout and shuffle among themselves only
   const uint32_t group_mask = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << (threadIdx.x & 31 & ~(LPR - 1));
-  const uint32_t token = gi / (uint32_t)p.groups;
+  const uint32_t per_token = (uint32_t)(p.groups[0] + p.groups[1]);
+  const uint32_t token = gi / per_token;
   if (token >= p.tokens) return;
-  const int j = (int)(gi - token * (uint32_t)p.groups);
+  int j = (int)(gi - token * per_token);
+  const int sel = j >= p.groups[0] ? 1 : 0;  // a group's rows are of one tensor
+  const RopeItem& it = p.item[sel];
+  const int step = p.groups[sel];
+  if (sel) j -= p.groups[0];
   const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * (uint32_t)p.T);
   const int nc = p.D / V, rc = p.rot / V;
-  // this lane's two pieces and how they rotate
-  int c0, c1;
-  bool turn;
-  if (p.interleaved) {
-    c0 = 2 * u, c1 = 2 * u + 1;
-    turn = c0 < rc;
-  } else {
+  // this lane's two pieces and whether they rotate
+  int c0 = 2 * u, c1 = 2 * u + 1;
+  bool turn = c0 < rc;
+  if (!INTER) {
     turn = u < rc / 2;
     c0 = turn ? u : rc + 2 * (u - rc / 2);
     c1 = turn ? u + rc / 2 : c0 + 1;
   }
   const bool has0 = c0 < nc, has1 = c1 < nc;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   uint4 xv[HPG][2];
+  {
+    const T* x = static_cast<const T*>(it.x) + b * it.x_sb + t * it.x_st + j * it.x_sh;
+    const int64_t hop = step * it.x_sh;
 #pragma unroll
-  for (int i = 0; i < HPG; ++i) {
-    int h = j + i * p.groups;
-    xv[i][0] = xv[i][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (h >= p.heads) continue;
-    const bool second = h >= p.item[0].heads;
-    const RopeItem& it = p.item[second ? 1 : 0];
-    if (second) h -= p.item[0].heads;
-    const T* x = static_cast<const T*>(it.x) + b * it.x_sb + t * it.x_st + h * it.x_sh;
-    if (has0) xv[i][0] = __ldcs(reinterpret_cast<const uint4*>(x + c0 * V));
-    if (has1) xv[i][1] = __ldcs(reinterpret_cast<const uint4*>(x + c1 * V));
-  }
-  // cosines and sines of the V pairs of this lane's pieces (interleaved pieces 2u, 2u+1 use entries uV .. uV+V-1)
-  float cs[V], sn[V];
-  if (turn) {
-    const int64_t row = table_row(p, token);
-    if (row >= 0) {
-      const int64_t at = row * (p.rot / 2) + u * V;
-      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.cos) + at), cs);
-      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.sin) + at), sn);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
+    for (int i = 0; i < HPG; ++i) {
+      const bool in = j + i * step < it.heads;
+      xv[i][0] = in && has0 ? __ldcs(reinterpret_cast<const uint4*>(x + c0 * V)) : zero;
+      xv[i][1] = in && has1 ? __ldcs(reinterpret_cast<const uint4*>(x + c1 * V)) : zero;
+      x += hop;
     }
   }
-  float w0[V], w1[V];
-  int loaded = -1;
+  const bool norm = it.scale != nullptr;
+  F2 ff[V / 2], fs[V / 2], sf[V / 2], ss[V / 2];  // f' = inv (ff f - fs s), s' = inv (sf f + ss s), two pairs each
+  {
+    float w0[V], w1[V], cs[V], sn[V];
+    if (norm) {
+      const T* sc = static_cast<const T*>(it.scale);
+      Chunk<T>::unpack(has0 ? *reinterpret_cast<const uint4*>(sc + c0 * V) : zero, w0);
+      Chunk<T>::unpack(has1 ? *reinterpret_cast<const uint4*>(sc + c1 * V) : zero, w1);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) w0[e] = w1[e] = 1.0f;
+    }
+    // cosines and sines of the V pairs: entries uV .. uV + V - 1 of the token's rows
+#pragma unroll
+    for (int e = 0; e < V; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
+    if (turn) {
+      const int64_t row = table_row(p, token);
+      if (row >= 0) {
+        const int64_t at = row * (p.rot / 2) + u * V;
+        Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.cos) + at), cs);
+        Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.sin) + at), sn);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float(&w)[V] = 2 * e < V ? w0 : w1;  // INTER: pairs e, e + 1 are four neighbours of one piece
+      const int at = (2 * e) % V;
+      const F2 wf = INTER ? F2(w[at], w[at + 2]) : F2(w0[e], w0[e + 1]);
+      const F2 ws = INTER ? F2(w[at + 1], w[at + 3]) : F2(w1[e], w1[e + 1]);
+      const F2 c2(cs[e], cs[e + 1]), s2(sn[e], sn[e + 1]), m2(-sn[e], -sn[e + 1]);
+      ff[e / 2] = mul2(wf, c2), fs[e / 2] = mul2(ws, m2), sf[e / 2] = mul2(wf, s2), ss[e / 2] = mul2(ws, c2);
+    }
+  }
+  T* y = static_cast<T*>(it.y) + b * it.y_sb + t * it.y_st + j * it.y_sh;
+  const int64_t hop = step * it.y_sh;
 #pragma unroll
   for (int i = 0; i < HPG; ++i) {
-    int h = j + i * p.groups;
-    if (h >= p.heads) continue;
-    const int sel = h >= p.item[0].heads ? 1 : 0;
-    const RopeItem& it = p.item[sel];
-    if (sel) h -= p.item[0].heads;
+    if (j + i * step >= it.heads) break;
     float a[V], c[V];
     Chunk<T>::unpack(xv[i][0], a);
     Chunk<T>::unpack(xv[i][1], c);
-    if (it.scale) {
-      float ss = 0.0f;
+    F2 f[V / 2], s[V / 2];
 #pragma unroll
-      for (int e = 0; e < V; ++e) ss = fmaf(a[e], a[e], fmaf(c[e], c[e], ss));
-#pragma unroll
-      for (int d = LPR / 2; d; d >>= 1) ss += __shfl_xor_sync(group_mask, ss, d, LPR);
-      const float inv = 1.0f / sqrtf(ss / (float)p.D + it.eps);
-      if (loaded != sel) {
-        const T* sc = static_cast<const T*>(it.scale);
-        uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        Chunk<T>::unpack(has0 ? *reinterpret_cast<const uint4*>(sc + c0 * V) : z, w0);
-        Chunk<T>::unpack(has1 ? *reinterpret_cast<const uint4*>(sc + c1 * V) : z, w1);
-        loaded = sel;
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) a[e] = a[e] * inv * w0[e], c[e] = c[e] * inv * w1[e];
+    for (int e = 0; e < V; e += 2) {
+      const float(&x)[V] = 2 * e < V ? a : c;
+      const int at = (2 * e) % V;
+      f[e / 2] = INTER ? F2(x[at], x[at + 2]) : F2(a[e], a[e + 1]);
+      s[e / 2] = INTER ? F2(x[at + 1], x[at + 3]) : F2(c[e], c[e + 1]);
     }
-    if (turn && p.interleaved) {
+    float inv = 1.0f;
+    if (norm) {
+      F2 q0 = mul2(f[0], f[0]), q1 = mul2(s[0], s[0]);
 #pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float re = a[e] * cs[e / 2] - a[e + 1] * sn[e / 2], im = a[e] * sn[e / 2] + a[e + 1] * cs[e / 2];
-        a[e] = re, a[e + 1] = im;
-        const float re1 = c[e] * cs[V / 2 + e / 2] - c[e + 1] * sn[V / 2 + e / 2];
-        const float im1 = c[e] * sn[V / 2 + e / 2] + c[e + 1] * cs[V / 2 + e / 2];
-        c[e] = re1, c[e + 1] = im1;
-      }
-    } else if (turn) {
+      for (int e = 1; e < V / 2; ++e) q0 = fma2(f[e], f[e], q0), q1 = fma2(s[e], s[e], q1);
+      float sum = (q0.lo() + q0.hi()) + (q1.lo() + q1.hi());
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float re = a[e] * cs[e] - c[e] * sn[e], im = a[e] * sn[e] + c[e] * cs[e];
-        a[e] = re, c[e] = im;
-      }
+      for (int d = LPR / 2; d; d >>= 1) sum += __shfl_xor_sync(group_mask, sum, d, LPR);
+      inv = inv_sqrt(fmaf(sum, p.inv_d, it.eps));
     }
-    T* y = static_cast<T*>(it.y) + b * it.y_sb + t * it.y_st + h * it.y_sh;
+    const F2 inv2(inv, inv);
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) {
+      F2 f1 = mul2(ff[e], f[e]), s1 = mul2(ss[e], s[e]);
+      if (turn) {  // elements behind the rotation stay apart, whatever they hold
+        f1 = fma2(fs[e], s[e], f1);
+        s1 = fma2(sf[e], f[e], s1);
+      }
+      f1 = mul2(f1, inv2), s1 = mul2(s1, inv2);
+      float(&x)[V] = 4 * e < V ? a : c;
+      const int at = (4 * e) % V;
+      (INTER ? x[at] : a[2 * e]) = f1.lo(), (INTER ? x[at + 2] : a[2 * e + 1]) = f1.hi();
+      (INTER ? x[at + 1] : c[2 * e]) = s1.lo(), (INTER ? x[at + 3] : c[2 * e + 1]) = s1.hi();
+    }
     if (has0) *reinterpret_cast<uint4*>(y + c0 * V) = Chunk<T>::pack(a);
     if (has1) *reinterpret_cast<uint4*>(y + c1 * V) = Chunk<T>::pack(c);
+    y += hop;
   }
 }
 
@@ -226,7 +258,7 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const __grid_constan
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    inv = 1.0f / sqrtf(ss / (float)p.D + it.eps);
+    inv = inv_sqrt(fmaf(ss, p.inv_d, it.eps));
   }
   const int64_t at = table_row(p, token);
   const int half = p.rot / 2;
@@ -244,21 +276,20 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const __grid_constan
   for (int e = p.rot + lane; e < p.D; e += 32) from_f32(to_f32(x[e]) * inv * (sc ? to_f32(sc[e]) : 1.0f), y[e]);
 }
 
+template <typename T, int LPR, int HPG>
+static cudaError_t launch_vec_rows(RopeParams p, cudaStream_t stream) {
+  for (int i = 0; i < 2; ++i) p.groups[i] = (p.item[i].heads + HPG - 1) / HPG;
+  const int64_t groups = p.tokens * (p.groups[0] + p.groups[1]), blocks = (groups * LPR + 255) / 256;
+  if (groups > 0xffff0000ll || blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  auto kernel = p.interleaved ? norm_rope_kernel<T, LPR, HPG, true> : norm_rope_kernel<T, LPR, HPG, false>;
+  return launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+}
+
 template <typename T, int LPR>
-static void launch_vec(const RopeParams& p0, const LaunchCtx& ctx, cudaError_t* e) {
-  RopeParams p = p0;
+static cudaError_t launch_vec(const RopeParams& p, const LaunchCtx& ctx) {
   // Four rows per lane group once that still fills every SM's threads: fewer table loads and more bytes in flight
-  const bool four = p.tokens * p.heads * LPR >= (int64_t)ctx.num_sms * 2048 * 4;
-  p.groups = four ? (p.heads + 3) / 4 : p.heads;
-  const int64_t blocks = (p.tokens * p.groups * LPR + 255) / 256;
-  if (p.tokens * p.groups > 0xffff0000ll || blocks > 0x7fffffff) {
-    *e = cudaErrorInvalidConfiguration;
-    return;
-  }
-  if (four)
-    *e = launch_pdl(norm_rope_kernel<T, LPR, 4>, dim3((unsigned)blocks), dim3(256), 0, ctx.stream, p);
-  else
-    *e = launch_pdl(norm_rope_kernel<T, LPR, 1>, dim3((unsigned)blocks), dim3(256), 0, ctx.stream, p);
+  return p.tokens * p.heads * LPR >= (int64_t)ctx.num_sms * 2048 * 4 ? launch_vec_rows<T, LPR, 4>(p, ctx.stream)
+                                                                     : launch_vec_rows<T, LPR, 1>(p, ctx.stream);
 }
 
 template <typename T>
@@ -278,10 +309,10 @@ static int launch_rope_t(const RopeParams& p, int items, const LaunchCtx& ctx, i
   cudaError_t e;
   if (vec) {
     const int pairs = (nc + 1) / 2;
-    if (pairs <= 4) launch_vec<T, 4>(p, ctx, &e);
-    else if (pairs <= 8) launch_vec<T, 8>(p, ctx, &e);
-    else if (pairs <= 16) launch_vec<T, 16>(p, ctx, &e);
-    else launch_vec<T, 32>(p, ctx, &e);
+    if (pairs <= 4) e = launch_vec<T, 4>(p, ctx);
+    else if (pairs <= 8) e = launch_vec<T, 8>(p, ctx);
+    else if (pairs <= 16) e = launch_vec<T, 16>(p, ctx);
+    else e = launch_vec<T, 32>(p, ctx);
   } else {
     const int64_t blocks = (p.tokens * p.heads + 7) / 8;
     if (blocks > 0x7fffffff) return 5;
@@ -300,6 +331,7 @@ int launch_norm_rope(const PlanOp& op, void* const* ptrs, const OpState*, const 
   p.T = (int)op.ip[NR_T];
   p.tokens = eff_batch(ctx, op, op.ip[NR_B]) * p.T;
   p.D = (int)op.ip[NR_D];
+  p.inv_d = 1.0f / (float)p.D;
   p.rot = (int)op.ip[NR_ROT];
   p.interleaved = (int)op.ip[NR_INTERLEAVED];
   p.positions = op.ip[NR_POSITIONS];
@@ -356,7 +388,7 @@ __global__ void __launch_bounds__(256) rms_norm_kernel(const T* __restrict__ x, 
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) ss += s_sum[i];
   }
-  const float inv = 1.0f / sqrtf(ss / (float)n + eps);
+  const float inv = inv_sqrt(ss / (float)n + eps);
   for (int64_t e = (int64_t)tid * V; e < n; e += 32 * WARPS * V) {
     if (VEC) {
       float f[Chunk<T>::N], w[Chunk<T>::N];

@@ -268,18 +268,70 @@ def lstm_persistent_fits(b: int, isz: int, h: int, sms: int) -> bool:
             and smem <= K.LP_SMEM_LIMIT and grid <= sms)
 
 
-FLASH_ROWS, FLASH_KEYS = 128, 64   # packed query rows of a work item, keys of a tile (attention_flash.cu)
-FLASH_CTAS = 2 * K.LP_PLAN_SMS     # two work items run on an SM at a time
+FLASH_ROWS, FLASH_KEYS = 128, 64   # query rows and keys of a tile of attention_flash.cu
 
 
-def flash_splits(items_tiles) -> list[int]:
-    """Work items along the keys for each (items, key tiles of one item) of
-    attention_flash.cu: none while the items fill the device, else as many as
-    keep every item resident at once with about the same number of tiles (at
-    least 4: a shorter item is mostly set-up)."""
+def flash_splits(items_tiles, resident: int, least: int) -> list[int]:
+    """Work items along the keys for each (items, key tiles of one item): none
+    while the items fill the ``resident`` places of the device, else as many
+    as keep every item resident at once with about the same number of tiles
+    (at least ``least``: a shorter item is mostly set-up)."""
     total = sum(n * t for n, t in items_tiles)
-    target = max(4, -(-total // FLASH_CTAS))
+    target = max(least, -(-total // resident))
     return [max(1, t // target) for _, t in items_tiles]
+
+
+@dataclass
+class FlashSchedule:
+    """How attention_flash.cu's passes divide an Attention (see there)."""
+    own: int         # AF_PASS_* of a sequence's rows on its own keys
+    past: int        # AF_PASS_* of a shared past's items, AF_PASS_NONE: no past, or first in the own items' keys
+    splits_own: int
+    splits_past: int
+    warps: int = 8   # of an item of the few-row pass
+
+    @property
+    def slots(self) -> int:
+        """Partial results per row (1: written straight to the output)."""
+        return self.splits_own + self.splits_past
+
+
+def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, additive: bool = False) -> FlashSchedule:
+    """``rows``: query rows of one sequence per key/value head."""
+    tiles = lambda n, m: -(-n // m)
+    sms = K.LP_PLAN_SMS
+    few = rows <= 16
+
+    def tile_pass(parts):
+        """Pass and splits for [(rows, heads, keys)]: two row tiles a work item
+        where all rows fill more than one (attention_wide.cu has no additive
+        masks), one item per SM then, else one tile and two items."""
+        wide = not additive and all(n > FLASH_ROWS for n, _, _ in parts)
+        m, n_keys, per_sm, least = (2 * FLASH_ROWS, 2 * FLASH_KEYS, 1, 4) if wide else (FLASH_ROWS, FLASH_KEYS, 2, 4)
+        return (K.AF_PASS_WIDE if wide else K.AF_PASS_TILES,
+                flash_splits([(h * tiles(n, m), tiles(t, n_keys)) for n, h, t in parts], per_sm * sms, least))
+
+    # A sequence with at least a tile of rows reads a shared past for itself: packing other sequences' rows beside
+    # them would save no read of it, and cost the merge.
+    apart = tp > 0 and shared and b > 1 and rows < FLASH_ROWS
+    keys = tk if apart else tp + tk
+    if few:
+        packed = b * rows
+        own = K.AF_PASS_ROWS8 if rows <= 8 and not (apart and packed > 8) else K.AF_PASS_ROWS16
+        m = 8 if own == K.AF_PASS_ROWS8 else 16
+        work = [(b * hkv, tiles(keys, 64))]
+        if not apart:
+            return FlashSchedule(own, K.AF_PASS_NONE, flash_splits(work, 2 * sms, 8)[0], 0)
+        if packed <= 64:
+            # up to four tiles of 16 rows read the past's keys from L2 once each: less than a second kernel costs
+            work.append((hkv * tiles(packed, m), tiles(tp, 64)))
+            so, sp = flash_splits(work, 2 * sms, 8)
+            return FlashSchedule(own, own, so, sp)
+        so = flash_splits(work, 4 * sms, 8)[0]
+        past, sp = tile_pass([(packed, hkv, tp)])
+        return FlashSchedule(K.AF_PASS_ROWS8 if rows <= 8 else K.AF_PASS_ROWS16, past, so, sp[0], 4)
+    own, splits = tile_pass([(rows, b * hkv, keys)] + ([(b * rows, hkv, tp)] if apart else []))
+    return FlashSchedule(own, own if apart else K.AF_PASS_NONE, splits[0], splits[1] if apart else 0)
 
 
 def qconv_int_requant_ok(w: np.ndarray, bias: np.ndarray, scale: np.ndarray, a_signed: int) -> int:
@@ -1521,32 +1573,30 @@ class B200PlanEmitter:
                        K.AF_MASK_ST: 1 if mt > 1 else 0, K.AF_MASK_ROWS: mb * mh * mt, K.AF_MASK_LEN: ms[-1]})
             t_mask = self._src(op.input_attn_mask)
             batched = batched and self._fixed_or_batched(op.input_attn_mask, len(ms) == 4 and mb == self._batch)
-            if kind == K.AF_MASK_BOOL:
-                words = -(-tp // FLASH_KEYS) + -(-tk // FLASH_KEYS)
-                t_bits = self._b.arena_tensor(T_TEMP, "u8", (mb * mh * mt, 16 + 8 * words), name="attention:mask-bits")
         nonpad = getattr(op, "input_nonpad_kv_seqlen", None)
         if nonpad:
             t_count = self._src(nonpad)
             batched = batched and self._fixed_or_batched(nonpad, True)
-        row_tiles = lambda rows: -(-rows // FLASH_ROWS)
-        group = hq // hkv
-        work = [(b * hkv * row_tiles(tq * group), -(-tk // FLASH_KEYS))]
         if tp:
             names = self._shared_past[i] if shared else (op.input_past_key, op.input_past_value)
             t_pk, t_pv = (self._src(n) for n in names)
             if not shared:
                 batched = batched and all(self._fixed_or_batched(n, True) for n in names)
-            work.append(((1 if shared else b) * hkv * row_tiles(tq * group * (b if shared else 1)), -(-tp // FLASH_KEYS)))
-        splits = flash_splits(work)
-        ip.update({K.AF_SPLITS_K: splits[0], K.AF_SPLITS_P: splits[1] if tp else 0})
-        if sum(splits) > 1:
-            t_part = self._b.arena_tensor(T_TEMP, "f32", (sum(splits), b * tq * hq, dv + 2), name="attention:partials")
+        sch = flash_schedule(b, hkv, tq * (hq // hkv), tk, tp, shared,
+                             t_mask >= 0 and kind != K.AF_MASK_BOOL)
+        ip.update({K.AF_PASS_OWN: sch.own, K.AF_PASS_PAST: sch.past, K.AF_SPLITS_K: sch.splits_own,
+                   K.AF_SPLITS_P: sch.splits_past, K.AF_WARPS: sch.warps})
+        if sch.slots > 1:
+            t_part = self._b.arena_tensor(T_TEMP, "f32", (sch.slots, b * tq * hq, dv + 2), name="attention:partials")
+        if t_mask >= 0 and kind == K.AF_MASK_BOOL and not {K.AF_PASS_TILES, K.AF_PASS_WIDE}.isdisjoint((sch.own, sch.past)):
+            words = 2 * (-(-tp // (2 * FLASH_KEYS)) + -(-tk // (2 * FLASH_KEYS)))
+            t_bits = self._b.arena_tensor(T_TEMP, "u8", (mb * mh * mt, 16 + 8 * words), name="attention:mask-bits")
         q, k, v = self._src(op.input_q), self._src(op.input_k), self._src(op.input_v)
         y = self._dest(op.output, "f16", tuple(self._shape(op.output)))
         what = "shared past, " if shared and tp else ("past, " if tp else "")
         self._b.op(K.K_ATTENTION_FLASH, [q, k, v, y, t_mask, t_pk, t_pv, t_count, t_part, t_bits], ip,
                    {K.AFF_SCALE: float(op.scale)},
-                   label=f"{op.output} ({what}tensor cores, fp32 online softmax, key splits {'+'.join(map(str, splits))})",
+                   label=f"{op.output} ({what}fp32 online softmax, {sch.slots} key range{'s' if sch.slots > 1 else ''})",
                    batched=batched)
 
     @staticmethod

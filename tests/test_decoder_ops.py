@@ -11,7 +11,7 @@ from emx_onnx_cgen_b200 import workloads as W
 from emx_onnx_cgen_b200.lowering import UnsupportedOpError
 from emx_onnx_cgen_b200.onnx_reader import infer_types, read_onnx
 from emx_onnx_cgen_b200.onnx_writer import write_onnx
-from emx_onnx_cgen_b200.plan import B200PlanEmitter, flash_splits
+from emx_onnx_cgen_b200.plan import B200PlanEmitter, flash_schedule, flash_splits
 from emx_onnx_cgen_b200.spec import GraphSpec, NodeSpec, TensorSpec
 
 
@@ -196,17 +196,40 @@ def test_shape_and_output_refusals():
 
 
 def test_splits_keep_every_item_resident():
-    assert flash_splits([(1, 100)]) == [25]                   # four tiles an item at least
-    assert flash_splits([(296, 100)]) == [1]
-    assert flash_splits([(148, 64)]) == [2]
-    assert flash_splits([(4000, 3)]) == [1]
-    assert flash_splits([(1, 1)]) == [1]
+    assert flash_splits([(1, 100)], 296, 4) == [25]                   # four tiles an item at least
+    assert flash_splits([(296, 100)], 296, 4) == [1]
+    assert flash_splits([(148, 64)], 296, 4) == [2]
+    assert flash_splits([(4000, 3)], 296, 4) == [1]
+    assert flash_splits([(1, 1)], 296, 4) == [1]
     for items in range(1, 400, 7):
         for tiles in (1, 2, 7, 33, 250):
-            (s,) = flash_splits([(items, tiles)])
+            (s,) = flash_splits([(items, tiles)], 296, 4)
             assert 1 <= s <= tiles and (s == 1 or items * s <= 296)
-    a, b = flash_splits([(128, 1), (32, 128)])
+    a, b = flash_splits([(128, 1), (32, 128)], 296, 4)
     assert a == 1 and 1 < b <= 128
+
+
+def test_schedules():
+    rows8, rows16, tiles, wide, none = (K.AF_PASS_ROWS8, K.AF_PASS_ROWS16, K.AF_PASS_TILES, K.AF_PASS_WIDE,
+                                        K.AF_PASS_NONE)
+    pick = lambda *a: (lambda s: (s.own, s.past))(flash_schedule(*a))
+    assert pick(16, 16, 1, 1500, 0, False) == (rows8, none)
+    assert pick(2, 2, 12, 1500, 0, False) == (rows16, none)
+    assert pick(2, 2, 17, 1500, 0, False) == (tiles, none)
+    assert pick(4, 2, 4, 10, 500, False) == (rows8, none)       # a past of its own is part of the row's keys
+    assert pick(16, 8, 4, 33, 2048, True) == (rows16, rows16)   # 64 packed rows
+    assert pick(2, 8, 4, 33, 2048, True) == (rows8, rows8)
+    assert pick(17, 8, 4, 33, 2048, True) == (rows8, tiles)
+    assert pick(33, 8, 4, 33, 2048, True) == (rows8, wide)
+    assert pick(33, 8, 4, 33, 2048, True, True) == (rows8, tiles)  # additive masks: no wide form
+    assert pick(2, 2, 129, 1500, 0, False) == (wide, none)
+    assert pick(2, 2, 129, 1500, 0, False, True) == (tiles, none)
+    assert pick(1, 8, 4, 33, 2048, True) == (rows8, none)       # nobody to share with
+    assert pick(3, 8, 100, 33, 2048, True) == (tiles, tiles)
+    assert pick(3, 8, 128, 33, 2048, True) == (tiles, none)
+    for args in ((1, 1, 1, 5000, 0, False), (128, 8, 4, 256, 8192, True), (7, 4, 9, 40, 1001, True)):
+        s = flash_schedule(*args)
+        assert s.slots == s.splits_own + s.splits_past and (s.splits_past > 0) == (s.past != none)
 
 
 def test_partials_are_reserved_for_split_or_two_part_keys():
@@ -217,6 +240,7 @@ def test_partials_are_reserved_for_split_or_two_part_keys():
     assert s > 1 and plan.tensors[t(plan)].shape == (s, 2 * 1 * 2, 66)
     plan = plan_of(W.decoder_attention(batch=2, q_heads=2, kv_heads=2, q_seq=1, past=64, kv_seq=5))
     assert plan.tensors[t(plan)].shape == (2, 4, 66)
+    assert t(plan_of(W.decoder_attention(batch=2, q_heads=2, kv_heads=2, q_seq=1, past=64, kv_seq=5, shared_past=False))) == -1
 
 
 def test_batched_operands():

@@ -61,18 +61,20 @@ def test_lengths_heads_layouts(kw):
 
 @pytest.mark.parametrize("shape", ["seq", "query", "head", "full", "rank2", "rank3", "short", "short_query"])
 @pytest.mark.parametrize("mask", ["bool", "f16", "f32"])
-@pytest.mark.parametrize("past", [0, 72, 101])
-def test_masks(mask, shape, past):
+@pytest.mark.parametrize("past,tq,d", [(0, 35, 64), (72, 35, 64), (101, 35, 128), (0, 3, 64), (72, 3, 128), (101, 7, 64),
+                                       (40, 1, 128)])
+def test_masks(mask, shape, past, tq, d):
     require_gpu()
-    b, h, tq, tk = 2, 4, 35, 136
+    b, h, tk = 2, 4, 136
     t = past + tk
     ms = {"seq": (b, 1, 1, t), "query": (b, 1, tq, t), "head": (1, h, 1, t), "full": (b, h, tq, t), "rank2": (tq, t),
           "rank3": (h, tq, t), "short": (b, 1, 1, t - 70), "short_query": (1, 1, tq, max(past // 2, 60))}[shape]
-    verify(dict(batch=b, q_heads=h, kv_heads=2, q_seq=tq, kv_seq=tk, mask=mask, mask_shape=ms, past=past))
+    verify(dict(batch=b, q_heads=h, kv_heads=2, q_seq=tq, kv_seq=tk, mask=mask, mask_shape=ms, past=past, head_dim=d,
+                shared_past=past != 101))
 
 
 @pytest.mark.parametrize("mask", ["bool", "f16", "f32"])
-@pytest.mark.parametrize("kv_seq,q_seq", [(150, 40), (3000, 2)])
+@pytest.mark.parametrize("kv_seq,q_seq", [(150, 40), (3000, 2), (3000, 20)])
 def test_rows_that_see_nothing(mask, kv_seq, q_seq):
     """Such rows give 0, whether one of a tile, a whole sequence, or only in
     some of the key ranges; so do their neighbours' values stay as they are."""
@@ -89,12 +91,15 @@ def test_rows_that_see_nothing(mask, kv_seq, q_seq):
     assert not got[1].any() and not got[0, :, q_seq // 2].any()
 
 
+@pytest.mark.parametrize("heads", [2, 40])
 @pytest.mark.parametrize("mask", ["f16", "f32"])
-def test_lowest_value_masks(mask):
+def test_lowest_value_masks(mask, heads):
     """Padding at the type's lowest value; a row of nothing else is a softmax of
     its scores, with all their digits."""
     require_gpu()
-    kw = dict(batch=2, q_heads=2, kv_heads=1, q_seq=20, kv_seq=200, mask=mask, mask_shape=(2, 1, 20, 200))
+    # 20 queries of two heads to a key/value head, or eight of one
+    kw = dict(batch=2, q_heads=heads, kv_heads=heads // 2 if heads == 2 else heads, q_seq=20 if heads == 2 else 8, kv_seq=200,
+              mask=mask, mask_shape=(2, 1, 20 if heads == 2 else 8, 200))
     wl = W.decoder_attention(**kw)
     x = wl.make_inputs(6)
     low = float(np.finfo(np.float16).min)
@@ -106,15 +111,16 @@ def test_lowest_value_masks(mask):
     if mask == "f32":  # the fp32 type's own lowest value
         x["mask"][:, :, :, 120:] = np.finfo(np.float32).min
         x["mask"][1, 0, 4, 130:] = 0
-        want = decoder_attention(wl, dict(x, mask=np.where(np.arange(20)[:, None] == 7, 0, x["mask"]).astype(np.float32)))
+        want = decoder_attention(wl, dict(x, mask=np.where(np.arange(kw["q_seq"])[:, None] == 7, 0, x["mask"]).astype(np.float32)))
         x["mask"][:, 0, 7, :] = np.finfo(np.float32).min  # one constant over a whole row changes nothing
         check(run(wl, x), *want, str(kw))
 
 
-def test_counts():
+@pytest.mark.parametrize("q_seq,d", [(9, 64), (1, 128), (5, 64)])
+def test_counts(q_seq, d):
     """Valid counts from none to all; what the padding holds reaches nothing."""
     require_gpu()
-    kw = dict(batch=7, q_heads=4, kv_heads=2, q_seq=9, kv_seq=200, count=True)
+    kw = dict(batch=7, q_heads=4, kv_heads=2, q_seq=q_seq, kv_seq=200, count=True, head_dim=d)
     wl = W.decoder_attention(**kw)
     x = wl.make_inputs(7)
     x["count"][:] = [200, 0, 1, 63, 64, 65, 130]
@@ -134,16 +140,19 @@ def test_counts():
     check(sess.run(x)["Y"], *want, "after the errors")
 
 
-def test_padding_behind_a_boolean_mask():
-    """Keys past the last that any row of a sequence sees are not read."""
+@pytest.mark.parametrize("q_seq", [50, 2])
+def test_padding_behind_a_boolean_mask(q_seq):
+    """Keys past the last that any row of a sequence sees are not read; below 17
+    rows, 16- or 32-key blocks that no row sees are not."""
     require_gpu()
-    kw = dict(batch=3, q_heads=2, kv_heads=2, q_seq=50, kv_seq=300, mask="bool")
+    kw = dict(batch=3, q_heads=2, kv_heads=2, q_seq=q_seq, kv_seq=300, mask="bool")
     wl = W.decoder_attention(**kw)
     x = wl.make_inputs(8)
     ends = [300, 77, 128]
     x["mask"][:] = np.arange(300)[None, None, None, :] < np.array(ends)[:, None, None, None]
     want = decoder_attention(wl, x)
     for b, n in enumerate(ends):
+        n = n if q_seq > 16 else -(-n // 32) * 32
         x["K"][b, :, n:] = np.nan
         x["V"][b, :, n:] = np.inf
     check(run(wl, x), *want, str(kw))
@@ -152,8 +161,8 @@ def test_padding_behind_a_boolean_mask():
 def test_scores_of_hidden_keys_do_not_matter():
     """Infinite and NaN scores of keys that a row does not see leave it alone."""
     require_gpu()
-    for mask in ("bool", "f16"):
-        kw = dict(batch=1, q_heads=2, kv_heads=2, q_seq=30, kv_seq=150, mask=mask, mask_shape=(1, 1, 30, 150))
+    for mask, tq in (("bool", 30), ("f16", 30), ("bool", 6), ("f16", 6)):
+        kw = dict(batch=1, q_heads=2, kv_heads=2, q_seq=tq, kv_seq=150, mask=mask, mask_shape=(1, 1, tq, 150))
         wl = W.decoder_attention(**kw)
         x = wl.make_inputs(9)
         x["mask"][..., [3, 70, 149]] = False if mask == "bool" else -np.inf
@@ -171,18 +180,23 @@ def test_scores_of_hidden_keys_do_not_matter():
     dict(batch=1, q_heads=2, kv_heads=1, q_seq=4, kv_seq=4, past=1, causal=True, head_dim=32, v_dim=64),
     dict(batch=3, q_heads=4, kv_heads=2, q_seq=2, kv_seq=70, past=130, rank=3),
     dict(batch=3, q_heads=4, kv_heads=2, q_seq=1, kv_seq=20, past=9000, head_dim=128),  # split prefix
+    dict(batch=130, q_heads=8, kv_heads=2, q_seq=1, kv_seq=300, past=700, head_dim=128),
+    dict(batch=4, q_heads=8, kv_heads=2, q_seq=3, kv_seq=50, past=300, head_dim=128),   # 12 rows a sequence
+    dict(batch=2, q_heads=4, kv_heads=2, q_seq=30, kv_seq=30, past=300, causal=True),   # 60 rows a sequence
+    dict(batch=2, q_heads=4, kv_heads=2, q_seq=3, kv_seq=3, past=100, causal=True, head_dim=24),
 ])
 def test_past(kw, shared):
     require_gpu()
     verify(dict(kw, shared_past=shared))
 
 
+@pytest.mark.parametrize("batch", [6, 40])
 @pytest.mark.parametrize("shared", [True, False])
-def test_past_with_masks(shared):
+def test_past_with_masks(shared, batch):
     """A mask over prefix and suffix: hidden prefix keys, hidden suffixes, a row
     that sees the prefix alone, the suffix alone, or nothing."""
     require_gpu()
-    kw = dict(batch=6, q_heads=4, kv_heads=2, q_seq=2, kv_seq=70, past=321, mask="bool", mask_shape=(6, 1, 2, 391),
+    kw = dict(batch=batch, q_heads=4, kv_heads=2, q_seq=2, kv_seq=70, past=321, mask="bool", mask_shape=(batch, 1, 2, 391),
               shared_past=shared)
     wl = W.decoder_attention(**kw)
     x = wl.make_inputs(11)
