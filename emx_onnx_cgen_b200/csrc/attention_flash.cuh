@@ -61,11 +61,10 @@ struct ItemClass {
   int past;
 };
 
-// The keys that the rows of a tile-pass item see, as a list of KT-key tiles.
 struct TileParams {
-  CUtensorMap map_k[2], map_v[2];  // current keys, past: 4-D (d, key, head, batch), box (64, KT, 1, 1), 128-byte swizzle
+  CUtensorMap map_k[2], map_v[2];  // current keys, past: 4-D (d, key, head, batch), box (64, 64, 1, 1), 128-byte swizzle
   ItemClass cls[2];
-  int first1;
+  int first1, items;  // items of class 1, of both
   const uint16_t* q;
   uint16_t* o;
   float* part_o;    // [slot][row][DV], null: one item per row, written to o
@@ -104,7 +103,7 @@ struct RowsParams {
 };
 
 cudaError_t prepare_attention_wide();
-cudaError_t launch_attention_wide(const TileParams& p, int slabs, int mask, unsigned items, cudaStream_t stream);
+cudaError_t launch_attention_wide(const TileParams& p, int slabs, int mask, int num_sms, cudaStream_t stream);
 cudaError_t prepare_attention_rows();
 cudaError_t launch_attention_rows(const RowsParams& p, int row_tiles, int mask, int warps, unsigned items,
                                   cudaStream_t stream);

@@ -307,9 +307,9 @@ def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, 
         where all rows fill more than one (attention_wide.cu has no additive
         masks), one item per SM then, else one tile and two items."""
         wide = not additive and all(n > FLASH_ROWS for n, _, _ in parts)
-        m, n_keys, per_sm, least = (2 * FLASH_ROWS, 2 * FLASH_KEYS, 1, 4) if wide else (FLASH_ROWS, FLASH_KEYS, 2, 4)
+        m, per_sm, least = (2 * FLASH_ROWS, 1, 8) if wide else (FLASH_ROWS, 2, 4)
         return (K.AF_PASS_WIDE if wide else K.AF_PASS_TILES,
-                flash_splits([(h * tiles(n, m), tiles(t, n_keys)) for n, h, t in parts], per_sm * sms, least))
+                flash_splits([(h * tiles(n, m), tiles(t, FLASH_KEYS)) for n, h, t in parts], per_sm * sms, least))
 
     # A sequence with at least a tile of rows reads a shared past for itself: packing other sequences' rows beside
     # them would save no read of it, and cost the merge.
@@ -1589,7 +1589,7 @@ class B200PlanEmitter:
         if sch.slots > 1:
             t_part = self._b.arena_tensor(T_TEMP, "f32", (sch.slots, b * tq * hq, dv + 2), name="attention:partials")
         if t_mask >= 0 and kind == K.AF_MASK_BOOL and not {K.AF_PASS_TILES, K.AF_PASS_WIDE}.isdisjoint((sch.own, sch.past)):
-            words = 2 * (-(-tp // (2 * FLASH_KEYS)) + -(-tk // (2 * FLASH_KEYS)))
+            words = -(-tp // FLASH_KEYS) + -(-tk // FLASH_KEYS)
             t_bits = self._b.arena_tensor(T_TEMP, "u8", (mb * mh * mt, 16 + 8 * words), name="attention:mask-bits")
         q, k, v = self._src(op.input_q), self._src(op.input_k), self._src(op.input_v)
         y = self._dest(op.output, "f16", tuple(self._shape(op.output)))
