@@ -658,14 +658,14 @@ int prepare_attention_flash(const PlanOp& op, void* const*, OpState*, int, char*
 }
 
 // 4-D map (d, t, h, b) over an fp16 tensor with element strides (1, st, sh, sb),
-// boxes of 64 d x 64 tokens.
+// boxes of 64 d x `tile_keys` tokens.
 static int make_tmap_kv(CUtensorMap* map, const void* base, int64_t d, int64_t t, int64_t heads, int64_t batch,
-                        int64_t st, int64_t sh, int64_t sb) {
+                        int64_t st, int64_t sh, int64_t sb, int tile_keys) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc || ((uintptr_t)base & 15u)) return 5;
   cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)t, (cuuint64_t)heads, (cuuint64_t)batch};
   cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)AFK_N, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)tile_keys, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -673,8 +673,25 @@ static int make_tmap_kv(CUtensorMap* map, const void* base, int64_t d, int64_t t
   return r == CUDA_SUCCESS ? 0 : 4;
 }
 
+// Query rows as 5-D tiles of 64 d x 128 rows (token, head of the group), for the
+// class whose rows run over one sequence, or over all of them: possible where a
+// group divides 128 and tokens (and sequences) lie evenly.  Returns whether.
+static int make_tmap_q(CUtensorMap* map, const RowsParams& r, int64_t tokens, int64_t st, int64_t sequences, int64_t sb) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  const int64_t group = r.group.d;
+  if (!enc || 128 % group) return 0;
+  cuuint64_t dims[5] = {(cuuint64_t)r.D, (cuuint64_t)group, (cuuint64_t)tokens, (cuuint64_t)r.HKV, (cuuint64_t)sequences};
+  cuuint64_t strides[4] = {(cuuint64_t)r.q_sh * 2, (cuuint64_t)st * 2, (cuuint64_t)(group * r.q_sh) * 2, (cuuint64_t)sb * 2};
+  cuuint32_t box[5] = {64, (cuuint32_t)group, (cuuint32_t)(128 / group), 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<uint16_t*>(r.q), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Fills what the tile pass needs beside the rows' parameters.
-static int tile_params(TileParams& p, const RowsParams& r, const ItemClass* cls, int first1, int items) {
+static int tile_params(TileParams& p, const RowsParams& r, const ItemClass* cls, int first1, int items,
+                       int tile_keys) {
   p.cls[0] = cls[0], p.cls[1] = cls[1], p.first1 = first1, p.items = items;
   p.q = r.q, p.o = r.o, p.part_o = r.part_o, p.part_ml = r.part_ml;
   p.q_sb = r.q_sb, p.q_sh = r.q_sh, p.q_st = r.q_st, p.o_sb = r.o_sb, p.o_sh = r.o_sh, p.o_st = r.o_st;
@@ -687,16 +704,20 @@ static int tile_params(TileParams& p, const RowsParams& r, const ItemClass* cls,
   p.add_vec = p.add && !p.add_f32 && p.mask_len % 8 == 0 && p.tp % 8 == 0 && ((uintptr_t)p.add & 15u) == 0;
   p.scale_log2 = r.scale_log2;
   p.err = r.err;
-  int rc = make_tmap_kv(&p.map_k[0], r.k, p.D, p.tk, p.HKV, p.B, r.k_st, r.k_sh, r.k_sb);
-  if (!rc) rc = make_tmap_kv(&p.map_v[0], r.v, p.DV, p.tk, p.HKV, p.B, r.v_st, r.v_sh, r.v_sb);
+  const int64_t tq = r.TQ.d;
+  p.q_boxes[0] = make_tmap_q(&p.map_q[0], r, tq, r.q_st, r.B, r.q_sb);
+  if (tq == 1 || r.q_sb == tq * r.q_st)
+    p.q_boxes[1] = make_tmap_q(&p.map_q[1], r, r.B * tq, tq == 1 ? r.q_sb : r.q_st, 1, (int64_t)r.B * r.q_sb);
+  int rc = make_tmap_kv(&p.map_k[0], r.k, p.D, p.tk, p.HKV, p.B, r.k_st, r.k_sh, r.k_sb, tile_keys);
+  if (!rc) rc = make_tmap_kv(&p.map_v[0], r.v, p.DV, p.tk, p.HKV, p.B, r.v_st, r.v_sh, r.v_sb, tile_keys);
   if (p.tp > 0) {
     const int copies = p.past_shared ? 1 : p.B;
     if (!rc)
       rc = make_tmap_kv(&p.map_k[1], r.past_k, p.D, p.tp, p.HKV, copies, p.D, (int64_t)p.tp * p.D,
-                        (int64_t)p.HKV * p.tp * p.D);
+                        (int64_t)p.HKV * p.tp * p.D, tile_keys);
     if (!rc)
       rc = make_tmap_kv(&p.map_v[1], r.past_v, p.DV, p.tp, p.HKV, copies, p.DV, (int64_t)p.tp * p.DV,
-                        (int64_t)p.HKV * p.tp * p.DV);
+                        (int64_t)p.HKV * p.tp * p.DV, tile_keys);
   }
   return rc;
 }
@@ -784,13 +805,14 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
       e = launch_attention_rows(r, pass == AF_PASS_ROWS8 ? 1 : 2, variant, (int)op.ip[AF_WARPS], (unsigned)(n0 + n1), ctx.stream);
     } else {
       TileParams p{};
+      const int tile_keys = pass == AF_PASS_WIDE ? 128 : AFK_N;
       if (pass == AF_PASS_WIDE && variant == MASK_ADD) return 5;  // (never planned)
-      int rc = tile_params(p, r, cls, (int)n1, (int)(n0 + n1));
+      int rc = tile_params(p, r, cls, (int)n1, (int)(n0 + n1), tile_keys);
       if (rc) return rc;
       if (variant == MASK_BITS) {
         const int64_t mrows = p.mask_sb ? p.mask_sb * p.B : op.ip[AF_MASK_ROWS];
-        p.words_past = (p.tp + 63) / 64;
-        p.words = p.words_past + (p.tk + 63) / 64;
+        p.words_past = (p.tp + tile_keys - 1) / tile_keys * (tile_keys / 64);
+        p.words = p.words_past + (p.tk + tile_keys - 1) / tile_keys * (tile_keys / 64);
         p.spans = (const int4*)ptr(9);
         p.bits = (const unsigned long long*)(p.spans + mrows);
         e = launch_pdl(mask_pack_kernel, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, r.mask_bool, p.mask_len, p.tp,

@@ -62,7 +62,9 @@ struct ItemClass {
 };
 
 struct TileParams {
-  CUtensorMap map_k[2], map_v[2];  // current keys, past: 4-D (d, key, head, batch), box (64, 64, 1, 1), 128-byte swizzle
+  CUtensorMap map_k[2], map_v[2];  // current keys, past: 4-D (d, key, head, batch), box (64, tile keys, 1, 1), 128-byte swizzle
+  CUtensorMap map_q[2];  // per class: 5-D (d, head of the group, token, key/value head, sequence), 128 rows a box
+  int q_boxes[2];        // whether 128 consecutive rows of the class are such a box
   ItemClass cls[2];
   int first1, items;  // items of class 1, of both
   const uint16_t* q;

@@ -1589,7 +1589,7 @@ class B200PlanEmitter:
         if sch.slots > 1:
             t_part = self._b.arena_tensor(T_TEMP, "f32", (sch.slots, b * tq * hq, dv + 2), name="attention:partials")
         if t_mask >= 0 and kind == K.AF_MASK_BOOL and not {K.AF_PASS_TILES, K.AF_PASS_WIDE}.isdisjoint((sch.own, sch.past)):
-            words = -(-tp // FLASH_KEYS) + -(-tk // FLASH_KEYS)
+            words = 2 * (-(-tp // (2 * FLASH_KEYS)) + -(-tk // (2 * FLASH_KEYS)))
             t_bits = self._b.arena_tensor(T_TEMP, "u8", (mb * mh * mt, 16 + 8 * words), name="attention:mask-bits")
         q, k, v = self._src(op.input_q), self._src(op.input_k), self._src(op.input_v)
         y = self._dest(op.output, "f16", tuple(self._shape(op.output)))
