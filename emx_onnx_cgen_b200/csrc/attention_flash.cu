@@ -60,6 +60,31 @@ constexpr uint32_t AFK_KSLAB = AFK_N * 128u;  // 64 fp16 columns of a K or V til
 constexpr uint32_t AFK_TMEM_COLS = 256;       // scores at columns 0 and 64, output at 128
 constexpr uint32_t AFK_O_COL = 128;
 
+// Eight entries of an additive mask; `see`: which of them may be read (the others are 0).
+__device__ __forceinline__ void additive8(const TileParams& p, int64_t at, uint32_t see, float (&mk)[8]) {
+  if (p.add_vec && (p.add_padded || see == 0xffu)) {
+    if (p.add_f32) {
+      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.add) + at);
+      const float4 a = __ldg(src), b = __ldg(src + 1);
+      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mk[e] = additive_bounded(v[e]);
+    } else {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.add) + at));
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+        mk[2 * e] = f.x;
+        mk[2 * e + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mk[e] = (see >> e) & 1u ? additive_entry(p.add, p.add_f32, at + e) : 0.0f;
+  }
+}
+
 template <int NS, int MASK>
 __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const __grid_constant__ TileParams p) {
   constexpr uint32_t QTILE = NS * AFK_QSLAB, KTILE = NS * AFK_KSLAB;
@@ -86,7 +111,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
   uint32_t* holder = reinterpret_cast<uint32_t*>(s_full + 8);
   int* span = reinterpret_cast<int*>(holder + 1);  // [2] first and end key of the work item's rows
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   int* const err = p.err;
 
   // ---------------- work item
@@ -173,7 +198,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *holder;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *holder, 0);
   if (MASK == MASK_BITS) {
     pbeg = span[0];
     pend = min(pend, span[1]);
@@ -217,32 +242,42 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && J > 0) {
-      // ---------------- S issuer
+    if (J > 0) {
+      // ---------------- S issuer.  The warp goes through the waits together and an elected thread issues: operands
+      // known to be uniform cost a product the tensor pipe's time, not some 100 clocks of issue an instruction.
       const uint32_t idesc = make_idesc(1u, 0u, 0u, AFK_M, AFK_N);
       const int nks = (p.D + 15) / 16;
+      const uint64_t q = smem_desc_k_sw128(smem_u32(s_q), 1024), k = smem_desc_k_sw128(smem_u32(s_k), 1024);
       for (int j = 0; j < J; ++j) {
         const int s = j % ST, sb = j & 1;
-        if (!mbar_wait(&k_full[s], (uint32_t)(j / ST) & 1u, err, DEV_TIMEOUT_MMA)) break;
-        if (j >= 2 && !mbar_wait(&s_empty[sb], (uint32_t)((j >> 1) - 1) & 1u, err, DEV_TIMEOUT_MMA)) break;
+        bool ok = mbar_wait(&k_full[s], (uint32_t)(j / ST) & 1u, err, DEV_TIMEOUT_MMA);
+        if (ok && j >= 2) ok = mbar_wait(&s_empty[sb], (uint32_t)((j >> 1) - 1) & 1u, err, DEV_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        const uint32_t qa = smem_u32(s_q), kb = smem_u32(s_k + s * KTILE);
-        for (int ks = 0; ks < nks; ++ks) {
-          const uint32_t qoff = (uint32_t)(ks >> 2) * AFK_QSLAB + (uint32_t)(ks & 3) * 32u;
-          const uint32_t koff = (uint32_t)(ks >> 2) * AFK_KSLAB + (uint32_t)(ks & 3) * 32u;
-          mma_f16(tmem + (uint32_t)(sb * AFK_N), smem_desc_k_sw128(qa + qoff, 1024), smem_desc_k_sw128(kb + koff, 1024),
-                  idesc, ks > 0 ? 1u : 0u);
+        if (elect_one()) {
+          // descriptors hold addresses in 16-byte units in their low bits: a step along d is an addition
+          const uint64_t kt = k + s * (KTILE >> 4);
+#pragma unroll
+          for (int ks = 0; ks < 4 * NS; ++ks)
+            if (ks < nks)
+              mma_f16(tmem + (uint32_t)(sb * AFK_N), q + ((ks >> 2) * AFK_QSLAB + (ks & 3) * 32u) / 16u,
+                      kt + ((ks >> 2) * AFK_KSLAB + (ks & 3) * 32u) / 16u, idesc, ks > 0 ? 1u : 0u);
+          tc_commit(&s_full[sb]);
+          tc_commit(&k_empty[s]);
         }
-        tc_commit(&s_full[sb]);
-        tc_commit(&k_empty[s]);
+        __syncwarp();
       }
       // every MMA this thread issued completes before TMEM is released
-      tc_commit(&drain[0]);
-      (void)mbar_wait(&drain[0], 0, nullptr, 0);
+      if (elect_one()) {
+        tc_commit(&drain[0]);
+        (void)mbar_wait(&drain[0], 0, nullptr, 0);
+      }
+      __syncwarp();
     }
   } else if (warp == 2) {
     if (J > 0) {
-      // ---------------- P.V issuer (all lanes wait; lane 0 issues)
+      // ---------------- P.V issuer (as the S issuer)
+      const uint64_t pd = smem_desc_k_sw128(smem_u32(s_p), 1024), v = smem_desc_mn_sw128(smem_u32(s_v), AFK_KSLAB, 1024u);
       const uint32_t idesc = make_idesc(1u, 0u, 0u, AFK_M, (uint32_t)((p.DV + 15) & ~15)) | (1u << 16);
       for (int j = 0; j < J; ++j) {
         const int s = j % ST;
@@ -260,23 +295,22 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         }
         ok = mbar_wait(p_full, (uint32_t)j & 1u, err, DEV_TIMEOUT_MMA);
         if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) {
-          tc_fence_after();
-          const uint32_t pa = smem_u32(s_p), vb = smem_u32(s_v + s * KTILE);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vt = v + s * (KTILE >> 4);
 #pragma unroll
           for (int kk = 0; kk < AFK_N / 16; ++kk)
-            mma_f16(tmem + AFK_O_COL, smem_desc_k_sw128(pa + (uint32_t)kk * 32u, 1024),
-                    smem_desc_mn_sw128(vb + (uint32_t)kk * 16u * 128u, AFK_KSLAB, 1024u), idesc,
-                    (j > 0 || kk > 0) ? 1u : 0u);
+            mma_f16(tmem + AFK_O_COL, pd + kk * 2u, vt + kk * (16u * 128u / 16u), idesc, (j > 0 || kk > 0) ? 1u : 0u);
           tc_commit(o_done);
           tc_commit(&v_empty[s]);
         }
         __syncwarp();
       }
-      if (lane == 0) {
+      if (elect_one()) {
         tc_commit(&drain[1]);
         (void)mbar_wait(&drain[1], 0, nullptr, 0);
       }
+      __syncwarp();
     }
   } else if (warp >= 4 && warp - 4 < nact) {
     // ---------------- softmax and epilogue: thread = query row (warp % 4 = TMEM lane quarter)
@@ -307,7 +341,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         if (j + 1 < J) word = words[j + 1];
       }
       const int mask_at = (in_past ? 0 : p.tp) + key0;  // the tile's first key in a mask row
-      if (MASK == MASK_ADD) {  // keys past a short mask are not seen
+      if (MASK == MASK_ADD && !p.add_padded) {  // keys past a short mask are not seen (padded: -inf)
         const int left = p.mask_len - mask_at;
         if (left < AFK_N) vis &= left > 0 ? (1ull << left) - 1 : 0ull;
       }
@@ -344,7 +378,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       float mx;
       if (MASK == MASK_ADD) {
         // pass 1: -inf mask entries hide their key; the maximum of the masked scores (any value near it will do)
-        const int64_t at = mrow * p.mask_len + mask_at;
+        const int64_t at = mrow * p.add_pitch + (p.add_padded ? ((cl.past ? 0 : p.words_past) + jj) * AFK_N : mask_at);
         mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -352,19 +386,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float mk[8];
-            if (p.add_vec && half == ~0u) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.add) + at + 32 * c + i));
-              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vw[e]));
-                mk[2 * e] = f.x;
-                mk[2 * e + 1] = f.y;
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) mk[e] = (half & (1u << (i + e))) ? additive_entry(p.add, p.add_f32, at + 32 * c + i + e) : 0.0f;
-            }
+            additive8(p, at + 32 * c + i, (half >> i) & 0xffu, mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               if (mk[e] == -INFINITY) sv[c][i + e] = 0xff800000u;
@@ -391,26 +413,14 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       uint32_t pw[2][16];
       float lp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       if (MASK == MASK_ADD) {
-        const int64_t at = mrow * p.mask_len + mask_at;
+        const int64_t at = mrow * p.add_pitch + (p.add_padded ? ((cl.past ? 0 : p.words_past) + jj) * AFK_N : mask_at);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float mk[8];
-            if (p.add_vec && half == ~0u) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.add) + at + 32 * c + i));
-              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vw[e]));
-                mk[2 * e] = f.x;
-                mk[2 * e + 1] = f.y;
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) mk[e] = (half & (1u << (i + e))) ? additive_entry(p.add, p.add_f32, at + 32 * c + i + e) : 0.0f;
-            }
+            additive8(p, at + 32 * c + i, (half >> i) & 0xffu, mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               // a hidden key's score is -inf; its mask entry must not turn that into NaN
@@ -618,6 +628,23 @@ __global__ void __launch_bounds__(256) mask_pack_kernel(const uint8_t* __restric
   if (threadIdx.x == 0) spans[row] = make_int4(s_span[0], s_span[1], s_span[2], s_span[3]);
 }
 
+// ------------------------------------------------------------------ whole tiles of additive masks
+// y[row][tile][64]: the past's tiles, then the current keys', -inf past the mask's length and each part's keys.
+template <typename T>
+__global__ void __launch_bounds__(256) mask_pad_kernel(const T* __restrict__ mask, int len, int past, int keys, int words1,
+                                                       int words, T* __restrict__ y) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x;
+  const T* src = mask + row * len;
+  T* dst = y + row * words * 64;
+  const T low = (T)-INFINITY;
+  for (int i = threadIdx.x; i < words * 64; i += 256) {
+    const int seg = i < words1 * 64 ? 1 : 0, k = seg ? i : i - words1 * 64, at = seg ? k : past + k;
+    dst[i] = k < (seg ? past : keys) && at < len ? src[at] : low;
+  }
+}
+
 // ------------------------------------------------------------------ host side
 static size_t flash_smem(int ns) {
   const int st = ns == 1 ? 4 : 2;
@@ -700,8 +727,9 @@ static int tile_params(TileParams& p, const RowsParams& r, const ItemClass* cls,
   p.counts = r.counts;
   p.mask_sb = r.mask_sb, p.mask_sh = r.mask_sh, p.mask_st = r.mask_st;
   p.add = r.mask_add, p.add_f32 = r.add_f32, p.mask_len = r.mask_len;
-  // 16-byte reads of 8 fp16 entries: every row and both parts of the keys start on 16 bytes
-  p.add_vec = p.add && !p.add_f32 && p.mask_len % 8 == 0 && p.tp % 8 == 0 && ((uintptr_t)p.add & 15u) == 0;
+  p.add_pitch = p.mask_len;
+  const int entries = p.add_f32 ? 4 : 8;  // of 16 bytes: every row and both parts of the keys start on 16 bytes
+  p.add_vec = p.add && p.mask_len % entries == 0 && p.tp % entries == 0 && ((uintptr_t)p.add & 15u) == 0;
   p.scale_log2 = r.scale_log2;
   p.err = r.err;
   const int64_t tq = r.TQ.d;
@@ -809,17 +837,28 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
       if (pass == AF_PASS_WIDE && variant == MASK_ADD) return 5;  // (never planned)
       int rc = tile_params(p, r, cls, (int)n1, (int)(n0 + n1), tile_keys);
       if (rc) return rc;
+      const int64_t mrows = p.mask_sb ? p.mask_sb * p.B : op.ip[AF_MASK_ROWS];
+      p.words_past = (p.tp + tile_keys - 1) / tile_keys * (tile_keys / 64);
+      p.words = p.words_past + (p.tk + tile_keys - 1) / tile_keys * (tile_keys / 64);
       if (variant == MASK_BITS) {
-        const int64_t mrows = p.mask_sb ? p.mask_sb * p.B : op.ip[AF_MASK_ROWS];
-        p.words_past = (p.tp + tile_keys - 1) / tile_keys * (tile_keys / 64);
-        p.words = p.words_past + (p.tk + tile_keys - 1) / tile_keys * (tile_keys / 64);
         p.spans = (const int4*)ptr(9);
         p.bits = (const unsigned long long*)(p.spans + mrows);
         e = launch_pdl(mask_pack_kernel, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, r.mask_bool, p.mask_len, p.tp,
                        p.tk, p.words_past, p.words, (unsigned long long*)p.bits, (int4*)p.spans);
         ++*launches;
-        if (e != cudaSuccess) return 4;
+      } else if (variant == MASK_ADD && op.ip[AF_MASK_PADDED]) {
+        if (p.add_f32)
+          e = launch_pdl(mask_pad_kernel<float>, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, (const float*)p.add,
+                         p.mask_len, p.tp, p.tk, p.words_past, p.words, (float*)ptr(9));
+        else
+          e = launch_pdl(mask_pad_kernel<__half>, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, (const __half*)p.add,
+                         p.mask_len, p.tp, p.tk, p.words_past, p.words, (__half*)ptr(9));
+        ++*launches;
+        p.add = ptr(9);
+        p.add_pitch = (int64_t)p.words * 64;
+        p.add_vec = p.add_padded = 1;
       }
+      if (e != cudaSuccess) return 4;
       const int ns = flash_slabs(op);
       e = pass == AF_PASS_WIDE ? launch_attention_wide(p, ns, variant, ctx.num_sms, ctx.stream)
                                : launch_pdl(flash_kernel(ns, variant), dim3((unsigned)(n0 + n1)), dim3(AFK_THREADS),

@@ -40,13 +40,14 @@ __device__ __forceinline__ RowId row_of(int r, const SmallDiv& group, const Smal
   return id;
 }
 
+// Finite fp32 entries beyond 2^24 count as 2^24: no score reaches across that, and the differences formed from
+// them stay finite.  -inf (and NaN) stay.
+__device__ __forceinline__ float additive_bounded(float v) {
+  return v > 0x1p24f ? 0x1p24f : (v < -0x1p24f && v > -INFINITY ? -0x1p24f : v);
+}
+
 __device__ __forceinline__ float additive_entry(const void* mask, int f32, int64_t at) {
-  if (f32) {
-    // Finite entries beyond 2^24 count as 2^24: no score reaches across that, and the differences formed
-    // from them stay finite.  -inf (and NaN) stay.
-    const float v = __ldg(static_cast<const float*>(mask) + at);
-    return v > 0x1p24f ? 0x1p24f : (v < -0x1p24f && v > -INFINITY ? -0x1p24f : v);
-  }
+  if (f32) return additive_bounded(__ldg(static_cast<const float*>(mask) + at));
   return __half2float(__ldg(static_cast<const __half*>(mask) + at));
 }
 
@@ -78,8 +79,11 @@ struct TileParams {
   int64_t mask_sb, mask_sh, mask_st;  // mask row of (b, h, t): b * sb + h * sh + t * st
   const unsigned long long* bits;     // packed boolean mask [row][words], the past's words first
   const int4* spans;                  // per mask row: first and end visible current key, first and end visible past key
-  const void* add;                    // additive mask [row][mask_len]
-  int words, words_past, mask_len, add_f32, add_vec;
+  // additive mask [row][add_pitch]: as given, or, padded, every 64-key tile of the past and of the current keys whole
+  // (-inf past the mask) and in the tiles' order; add_vec: groups of 8 entries start on 16 bytes
+  const void* add;
+  int64_t add_pitch;
+  int words, words_past, mask_len, add_f32, add_vec, add_padded;
   float scale_log2;
   int* err;
 };

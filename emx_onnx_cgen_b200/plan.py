@@ -1588,9 +1588,16 @@ class B200PlanEmitter:
                    K.AF_SPLITS_P: sch.splits_past, K.AF_WARPS: sch.warps})
         if sch.slots > 1:
             t_part = self._b.arena_tensor(T_TEMP, "f32", (sch.slots, b * tq * hq, dv + 2), name="attention:partials")
-        if t_mask >= 0 and kind == K.AF_MASK_BOOL and not {K.AF_PASS_TILES, K.AF_PASS_WIDE}.isdisjoint((sch.own, sch.past)):
-            words = 2 * (-(-tp // (2 * FLASH_KEYS)) + -(-tk // (2 * FLASH_KEYS)))
-            t_bits = self._b.arena_tensor(T_TEMP, "u8", (mb * mh * mt, 16 + 8 * words), name="attention:mask-bits")
+        if t_mask >= 0 and not {K.AF_PASS_TILES, K.AF_PASS_WIDE}.isdisjoint((sch.own, sch.past)):
+            if kind == K.AF_MASK_BOOL:
+                words = 2 * (-(-tp // (2 * FLASH_KEYS)) + -(-tk // (2 * FLASH_KEYS)))
+                t_bits = self._b.arena_tensor(T_TEMP, "u8", (mb * mh * mt, 16 + 8 * words), name="attention:mask-bits")
+            elif ms[-1] % 8 or tp % 8:
+                # rows or the two parts of the keys start off 16 bytes: a copy in whole tiles, read 16 bytes at a time
+                ip[K.AF_MASK_PADDED] = 1
+                words = -(-tp // FLASH_KEYS) + -(-tk // FLASH_KEYS)
+                t_bits = self._b.arena_tensor(T_TEMP, self._dtype(op.input_attn_mask), (mb * mh * mt, 64 * words),
+                                              name="attention:mask-tiles")
         q, k, v = self._src(op.input_q), self._src(op.input_k), self._src(op.input_v)
         y = self._dest(op.output, "f16", tuple(self._shape(op.output)))
         what = "shared past, " if shared and tp else ("past, " if tp else "")
