@@ -45,6 +45,8 @@
 #include <cuda_fp16.h>
 
 #include "attention_flash.cuh"
+#include <algorithm>
+
 #include "host_util.h"
 #include "kernels.h"
 #include "tc100.cuh"
@@ -828,7 +830,23 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
     const int64_t n1 = together ? items[1] : (step == 0 ? items[1] : 0);
     const int64_t n0 = together || step == 1 ? items[0] : 0;
     if (is_rows(pass)) {
+      // a work item's boolean mask has to fit the kernel's bits
+      auto most_keys = [](int64_t tp, int64_t tk, int splits) {
+        const int64_t blocks = (tp + 15) / 16 + (tk + 15) / 16;
+        return (blocks + splits - 1) / splits * 16;
+      };
+      if (variant == MASK_BITS &&
+          ((n0 && most_keys(cls[0].past ? r.tp : 0, r.tk, cls[0].splits) > AF_ROWS_MASK_KEYS) ||
+           (n1 && most_keys(r.tp, 0, cls[1].splits) > AF_ROWS_MASK_KEYS)))
+        return 5;
       r.cls[0] = cls[0], r.cls[1] = cls[1], r.first1 = (int)n1;
+      for (int c = 0; c < 2; ++c) {
+        // (an absent class divides by 1)
+        r.by[c][0] = SmallDiv::of(cls[c].splits ? cls[c].splits : 1), r.by[c][1] = SmallDiv::of(cls[c].tiles ? cls[c].tiles : 1);
+        const int64_t largest = std::max<int64_t>(std::max(cls[c].splits, cls[c].tiles), r.HKV);
+        if (std::max<int64_t>(n0 + n1, most_keys(r.tp, r.tk, 1)) * largest > 0xffffffffll) return 5;
+      }
+      r.by_hkv = SmallDiv::of(r.HKV);
       r.late_wait = !together;
       e = launch_attention_rows(r, pass == AF_PASS_ROWS8 ? 1 : 2, variant, (int)op.ip[AF_WARPS], (unsigned)(n0 + n1), ctx.stream);
     } else {

@@ -90,6 +90,7 @@ struct TileParams {
 
 struct RowsParams {
   ItemClass cls[2];
+  SmallDiv by[2][2], by_hkv;  // by a class's splits and tiles, by the key/value heads
   int first1;
   const uint16_t *q, *k, *v, *past_k, *past_v;
   uint16_t* o;

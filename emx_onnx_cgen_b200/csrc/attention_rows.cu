@@ -3,27 +3,32 @@
 // operator and its mathematics; this kernel is one of its passes).
 //
 // What bounds it is the read of K and V: up to 16 query rows share every key,
-// 4 flops a byte and row at most, so nothing is staged -- a warp loads the
-// K and V of its key block from global memory straight into the operand
-// registers of mma.sync.m16n8k16, 16 bytes a thread and load, and hides the
-// latency behind the other warps of the SM.  (The tcgen05 form needs a 128-row
-// tile, tensor maps, barriers and TMEM set up per work item; at these sizes a
-// work item is over before that has paid off.)  Both products run transposed,
+// 4 flops a byte and row at most.  Each warp copies its 16-key blocks of K and V
+// into a ring of its own in shared memory (cp.async, 24 KB a warp), two to five
+// blocks ahead of the one it works on: with the blocks in registers, one ahead,
+// a block cost a memory latency (1.2 us).  The products are mma.sync.m16n8k16:
+// a tcgen05 form needs a 128-row tile, tensor maps, barriers and TMEM set up per
+// work item, and at these sizes a work item is over before that has paid off.
+// Both products run transposed,
 //   S^T [16 keys x 8 rows] = K Q^T,   O^T [16 d x 8 rows] += V^T P^T,
 // so the row tiles are 8 wide and the big operands are the A side:
 //   * the contraction over d may take d in any order, so thread t of a quad
 //     takes the 16-byte pieces t, t + 4, ... of a key's row, which serve two
 //     k-steps each, and the same pieces of the query rows;
-//   * the rows of O^T (d) may be in any order as well: thread group g loads
+//   * the rows of O^T (d) may be in any order as well: thread group g reads
 //     16-byte piece g of four keys' V rows and pairs up the keys' halves;
 //   * P^T reaches its operand layout through two 8 x 8 register transposes.
+// Piece c of key row r lies at place c ^ (r & 6) ^ 4 (r & 1) of the row, which
+// keeps both operands' reads free of bank conflicts.
 //
-// One work item is (sequence, key/value head, range of 16-key blocks); its 2 to
-// 8 warps take the blocks in turn and merge through shared memory.  The past and
+// One work item is (sequence, key/value head, range of 16-key blocks); its
+// warps take the blocks in turn and merge through shared memory.  The past and
 // the current keys of a sequence are one list of blocks, or, when the past is
 // shared by the batch, two kinds of items: rows of several sequences against
-// the past, each sequence's rows against its own keys.  Blocks whose keys a
-// boolean mask hides from every row are not loaded.
+// the past, each sequence's rows against its own keys.  The item's part of a
+// boolean mask is first turned into bits in shared memory, beside the first
+// blocks' copies; blocks before its first and after its last visible key are
+// not read.
 #include <cuda_fp16.h>
 
 #include "attention_flash.cuh"
@@ -34,7 +39,9 @@
 
 namespace emx {
 
-constexpr int AR_WARPS = 8;  // most warps of a work item
+constexpr int AR_WARPS = 8;        // most warps of a work item
+constexpr int AR_KB = 16;          // keys per block
+constexpr int AR_RING = 24 * 1024; // bytes of a warp's ring
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -49,28 +56,37 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   return r;
 }
 
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
+// 16 bytes global -> shared, or 16 zero bytes
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
 
+// Where piece c of key row r lies in its row.
+__device__ __forceinline__ int rows_place(int r, int c) { return c ^ (r & 6) ^ ((r & 1) << 2); }
+
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// NS: 64-wide slabs of the head size; NT: tiles of 8 query rows; MASK: AF_MASK_* folded to none / boolean / additive
+// NS: 64-wide slabs of the head size; NT: tiles of 8 query rows; MASK: MASK_*
 template <int NS, int NT, int MASK>
-__global__ void __launch_bounds__(32 * AR_WARPS, NS == 2 && NT == 2 ? 1 : 2)
-    attention_rows_kernel(const __grid_constant__ RowsParams p) {
-  constexpr int KM = NS == 2 ? 1 : 2;  // 16-key groups per block: 8 KB of K and V per warp at either head size
-  constexpr int KB = 16 * KM;
-  constexpr int NC = 2 * NS;           // 16-byte pieces of a key row per thread
-  constexpr int OW = 64 * NS + 4;      // padded row of the merge buffer
-  extern __shared__ __align__(16) float s_all[];  // rows_smem() bytes
+__global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const __grid_constant__ RowsParams p) {
+  constexpr int NC = 2 * NS;                      // 16-byte pieces of a key row per thread
+  constexpr int ROW = 128 * NS;                   // bytes of a key row in the ring
+  constexpr int STAGE = 2 * AR_KB * ROW;          // K and V of a block
+  constexpr int ST = AR_RING / STAGE;             // 6 or 3 blocks
+  constexpr int OW = 64 * NS + 4;                 // padded row of the merge buffer
+  extern __shared__ __align__(128) uint8_t s_all[];  // rows_smem() bytes
+  __shared__ uint32_t s_bits[MASK == MASK_BITS ? 8 * NT * AF_ROWS_MASK_KEYS / 32 : 1];  // [row][32 keys]
+  __shared__ int s_range[2];
+  __shared__ float2 s_row[8 * NT];
   const int warps = blockDim.x >> 5;
-  float(*s_o)[8 * NT][OW] = reinterpret_cast<float(*)[8 * NT][OW]>(s_all);
-  float(*s_m)[8 * NT] = reinterpret_cast<float(*)[8 * NT]>(s_all + warps * 8 * NT * OW);
+  float(*s_o)[8 * NT][OW] = reinterpret_cast<float(*)[8 * NT][OW]>(s_all);  // once the ring is done with
+  float(*s_m)[8 * NT] = reinterpret_cast<float(*)[8 * NT]>(s_all + (size_t)warps * 8 * NT * OW * 4);
   float(*s_l)[8 * NT] = s_m + warps;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (!p.late_wait) pdl_wait();
@@ -80,11 +96,9 @@ __global__ void __launch_bounds__(32 * AR_WARPS, NS == 2 && NT == 2 ? 1 : 2)
   const bool past_item = (int)blockIdx.x < p.first1;
   const ItemClass& cl = p.cls[past_item ? 1 : 0];
   int id = (int)blockIdx.x - (past_item ? 0 : p.first1);
-  const int split = id % cl.splits;
-  id /= cl.splits;
-  const int tile = id % cl.tiles;
-  id /= cl.tiles;
-  const int kvh = id % p.HKV, b = id / p.HKV;
+  const SmallDiv *by = p.by[past_item ? 1 : 0];  // splits, tiles
+  const int id1 = by[0].div(id), split = id - id1 * cl.splits, id2 = by[1].div(id1), tile = id1 - id2 * cl.tiles;
+  const int b = p.by_hkv.div(id2), kvh = id2 - b * p.HKV;
   const int rows_all = (int)(p.TQ.d * p.group.d) * (past_item ? p.B : 1);
   const int row0 = tile * 8 * NT, rows = min(8 * NT, rows_all - row0);
   const bool two = NT == 2 && rows > 8;
@@ -98,17 +112,44 @@ __global__ void __launch_bounds__(32 * AR_WARPS, NS == 2 && NT == 2 ? 1 : 2)
     }
   }
   const int past = cl.past ? p.tp : 0;
-  const int pblocks = (past + KB - 1) / KB, blocks = pblocks + (keys + KB - 1) / KB;
-  const int blk0 = (int)((long long)blocks * split / cl.splits), blk1 = (int)((long long)blocks * (split + 1) / cl.splits);
+  const int pblocks = (past + AR_KB - 1) / AR_KB, blocks = pblocks + (keys + AR_KB - 1) / AR_KB;
+  const int share = by[0].div(blocks + cl.splits - 1);  // (blocks * splits < 2^32 as well)
+  const int blk0 = min(blocks, share * split);
+  int blk1 = min(blocks, share * (split + 1));
 
   const uint16_t* kc = p.k + (int64_t)b * p.k_sb + (int64_t)kvh * p.k_sh;
   const uint16_t* vc = p.v + (int64_t)b * p.v_sb + (int64_t)kvh * p.v_sh;
   const int64_t ph = ((int64_t)(p.past_shared ? 0 : b) * p.HKV + kvh) * p.tp;
   const uint16_t* kp = p.past_k + ph * p.D;
   const uint16_t* vp = p.past_v + ph * p.DV;
-  // this thread's first piece: K of key g, V of key 2t
-  kc += (int64_t)g * p.k_st + 8 * t, kp += g * p.D + 8 * t;
-  vc += (int64_t)(2 * t) * p.v_st + 8 * g, vp += 2 * t * p.DV + 8 * g;
+
+  // ---------------- copies: this warp's n-th block is blk0 + warp + n * warps, in stage n % ST
+  const uint32_t ring = smem_u32(s_all) + warp * AR_RING;
+  auto issue = [&](int blk, int stage) {
+    if (blk < blk1) {
+      const bool is_past = blk < pblocks;
+      const int k0 = (is_past ? blk : blk - pblocks) * AR_KB, n = (is_past ? past : keys) - k0;
+      const int ks = is_past ? p.D : (int)p.k_st, vs = is_past ? p.DV : (int)p.v_st;
+      constexpr int PIECES = 8 * NS, STEP = 32 / PIECES;
+      const int c = lane % PIECES, r0 = lane / PIECES;
+      const uint16_t* ksrc = (is_past ? kp : kc) + (int64_t)k0 * ks + 8 * c;
+      const uint16_t* vsrc = (is_past ? vp : vc) + (int64_t)k0 * vs + 8 * c;
+      const uint32_t dst = ring + stage * STAGE;
+      const bool k_in = 8 * c < p.D, v_in = 8 * c < p.DV;
+#pragma unroll
+      for (int i = 0; i < AR_KB; i += STEP) {
+        const int r = r0 + i;
+        const bool in = r < n;
+        const uint32_t at = dst + r * ROW + rows_place(r, c) * 16;
+        // rows past the keys and pieces past the head size are zero (what is not taken is not read either)
+        cp_async16_or_zero(at, in && k_in ? ksrc + (int64_t)r * ks : p.k, in && k_in);
+        cp_async16_or_zero(at + AR_KB * ROW, in && v_in ? vsrc + (int64_t)r * vs : p.v, in && v_in);
+      }
+    }
+    cp_async_commit();  // (an empty group keeps the count)
+  };
+#pragma unroll 1  // (straight-line copies cost more in instruction fetches than they gain)
+  for (int n = 0; n < ST - 1; ++n) issue(blk0 + warp + n * warps, n);
 
   // ---------------- the rows whose scores this thread holds (2t, 2t + 1 of each tile): mask row and key limit
   int64_t mrow[NT][2];
@@ -120,7 +161,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, NS == 2 && NT == 2 ? 1 : 2)
     for (int e = 0; e < 2; ++e) {
       const int r = 8 * n + 2 * t + e;
       const RowId w = row_of(row0 + min(r, rows - 1), p.group, p.TQ, kvh, b, past_item);
-      mrow[n][e] = MASK == MASK_NONE ? 0 : (w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st) * (int64_t)p.mask_len;
+      mrow[n][e] = MASK != MASK_ADD ? 0 : (w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st) * (int64_t)p.mask_len;
       lim[n][e] = r >= rows || past_item ? 0x7fffffff : p.tp + (p.causal ? min(keys, w.t + 1) : keys);
       lim_all = min(lim_all, lim[n][e]);
     }
@@ -142,77 +183,70 @@ __global__ void __launch_bounds__(32 * AR_WARPS, NS == 2 && NT == 2 ? 1 : 2)
     }
   }
 
-  uint4 k[KM][2][NC], v[KM][4][NS];
-  // pieces past the head size stay zero; a whole block's loads have no other condition
-  bool k_in[NC], v_in[NS];
+  // ---------------- boolean mask: bits of the item's keys, counted through its blocks; the blocks worth reading
+  const bool one_row = p.mask_sh == 0 && p.mask_st == 0 && !past_item;  // every row of the tile has the same mask row
+  int first = blk0;  // bits of block i start at bit (i - blk0) * AR_KB
+  if (MASK == MASK_BITS) {
+    if (threadIdx.x < 2) s_range[threadIdx.x] = threadIdx.x ? 0 : 0x7fffffff;
+    __syncthreads();
+    const int words = ((blk1 - blk0) * AR_KB + 31) / 32, mask_rows = one_row ? 1 : rows;
+    int lo = 0x7fffffff, hi = 0;
+    // a warp takes 256 keys of a row at a time, eight loads in flight
+    constexpr int LOADS = 8;
+    const int groups = (words + LOADS - 1) / LOADS;
+#pragma unroll 1
+    for (int i = warp; i < groups * mask_rows; i += warps) {
+      const int r = i / groups, w4 = (i - r * groups) * LOADS;
+      const RowId w = row_of(row0 + r, p.group, p.TQ, kvh, b, past_item);
+      const uint8_t* src = p.mask_bool + (w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st) * (int64_t)p.mask_len;
+      uint8_t v[LOADS];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) k_in[c] = 8 * (t + 4 * c) < p.D;
-#pragma unroll
-  for (int s = 0; s < NS; ++s) v_in[s] = 64 * s + 8 * g < p.DV;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  auto load_k = [&](int blk) {
-    const bool is_past = blk < pblocks;
-    const int k0 = (is_past ? blk : blk - pblocks) * KB, n = (is_past ? past : keys) - k0;
-    const int ks = is_past ? p.D : (int)p.k_st;
-    const uint16_t* src = (is_past ? kp : kc) + (int64_t)k0 * ks;
-    const int64_t step = (int64_t)ks * 8;
-    const bool whole = n >= KB;
-#pragma unroll
-    for (int m = 0; m < KM; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool in = whole || 16 * m + 8 * h + g < n;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) k[m][h][c] = in && k_in[c] ? ld_stream(src + (2 * m + h) * step + 32 * c) : zero;
+      for (int u = 0; u < LOADS; ++u) {
+        const int blk = blk0 + ((w4 + u) * 32 + lane) / AR_KB, in_blk = lane % AR_KB;
+        const bool is_past = blk < pblocks;
+        const int k = (is_past ? blk : blk - pblocks) * AR_KB + in_blk, pos = (is_past ? 0 : p.tp) + k;
+        v[u] = blk < blk1 && k < (is_past ? past : keys) && pos < p.mask_len ? __ldg(src + pos) : (uint8_t)0;
       }
-  };
-  auto load_v = [&](int blk) {
-    const bool is_past = blk < pblocks;
-    const int k0 = (is_past ? blk : blk - pblocks) * KB, n = (is_past ? past : keys) - k0;
-    const int vs = is_past ? p.DV : (int)p.v_st;
-    const uint16_t* src = (is_past ? vp : vc) + (int64_t)k0 * vs;
-    const int64_t step = (int64_t)vs * 8;
-    const bool whole = n >= KB;
 #pragma unroll
-    for (int m = 0; m < KM; ++m)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool in = whole || 16 * m + 8 * (e >> 1) + 2 * t + (e & 1) < n;
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-          v[m][e][s] = in && v_in[s] ? ld_stream(src + (2 * m + (e >> 1)) * step + (e & 1) * vs + 64 * s) : zero;
+      for (int u = 0; u < LOADS; ++u) {
+        const uint32_t bits = __ballot_sync(0xffffffffu, v[u] != 0);
+        if (w4 + u >= words) break;
+        if (lane == 0) s_bits[r * (AF_ROWS_MASK_KEYS / 32) + w4 + u] = bits;
+        if (bits) {
+          lo = min(lo, (w4 + u) * 32 + __ffs(bits) - 1);
+          hi = max(hi, (w4 + u) * 32 + 32 - __clz(bits));
+        }
       }
-  };
-  // mask entries of a block at this thread's scores: [m][half][n][e]; returns whether any lane sees any key
-  float mk[MASK == MASK_ADD ? KM * 4 * NT : 1];
-  auto load_mask = [&](int blk) -> uint32_t {
+    }
+    if (lane == 0 && hi) {
+      atomicMin(&s_range[0], lo);
+      atomicMax(&s_range[1], hi);
+    }
+    __syncthreads();
+    const int lo_blk = s_range[1] ? blk0 + s_range[0] / AR_KB : blk1;
+    const int hi_blk = s_range[1] ? blk0 + (s_range[1] + AR_KB - 1) / AR_KB : blk0;
+    // later copies stop at the last block with a visible key; the blocks before the first are passed over below
+    blk1 = min(blk1, hi_blk);
+    first = lo_blk;
+  }
+
+  // additive mask entries of a block at this thread's scores, loaded a block ahead
+  float mk[MASK == MASK_ADD ? 4 * NT : 1], mk_next[MASK == MASK_ADD ? 4 * NT : 1];
+  auto load_add = [&](int blk) {
+    if (MASK != MASK_ADD || blk >= blk1) return;
     const bool is_past = blk < pblocks;
-    const int k0 = (is_past ? blk : blk - pblocks) * KB, pos0 = (is_past ? 0 : p.tp) + k0;
-    const int seg_end = is_past ? past : p.tp + keys;
-    if (MASK == MASK_NONE && pos0 + KB <= min(lim_all, seg_end)) return ~0u;
-    uint32_t see = 0;
+    const int k0 = (is_past ? blk : blk - pblocks) * AR_KB, pos0 = (is_past ? 0 : p.tp) + k0;
 #pragma unroll
-    for (int m = 0; m < KM; ++m)
+    for (int h = 0; h < 2; ++h) {
+      const int pos = pos0 + 8 * h + g;
+      const bool in = k0 + 8 * h + g < (is_past ? past : keys);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int pos = pos0 + 16 * m + 8 * h + g;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = ((m * 2 + h) * NT + n) * 2 + e;
-            bool ok = pos < min(lim[n][e], seg_end);
-            if (MASK != MASK_NONE) ok = ok && pos < p.mask_len;
-            if (MASK == MASK_BITS) ok = ok && __ldg(p.mask_bool + mrow[n][e] + pos) != 0;
-            if (MASK == MASK_ADD) {
-              mk[i] = ok ? additive_entry(p.mask_add, p.add_f32, mrow[n][e] + pos) : 0.0f;
-              ok = ok && mk[i] != -INFINITY;
-              if (!ok) mk[i] = 0.0f;
-            }
-            see |= (ok ? 1u : 0u) << i;
-          }
-      }
-    return see;
+        for (int e = 0; e < 2; ++e)
+          mk_next[(h * NT + n) * 2 + e] =
+              in && pos < p.mask_len ? additive_entry(p.mask_add, p.add_f32, mrow[n][e] + pos) : -INFINITY;
+    }
   };
 
   float o[NT][NS][4][4];  // O^T: [row tile][slab][d pair][(d, row), (d, row + 1), (d + 1, row), (d + 1, row + 1)]
@@ -229,150 +263,170 @@ __global__ void __launch_bounds__(32 * AR_WARPS, NS == 2 && NT == 2 ? 1 : 2)
         for (int e = 0; e < 4; ++e) o[n][s][j][e] = 0.0f;
   }
   const float sc = p.scale_log2;
+  bool any_block = false;
+  // operand addresses within a stage: K row g (and g + 8), V rows 2t, 2t + 1 (and + 8)
+  const uint32_t k_row = ring + g * ROW, v_row = ring + AR_KB * ROW + 2 * t * ROW;
+  const int k_swz = rows_place(g, 0), v_swz0 = rows_place(2 * t, 0), v_swz1 = rows_place(2 * t + 1, 0);
 
-  int blk = blk0 + warp;
-  uint32_t see = 0;
-  bool need = false;
-  const bool any_block = blk < blk1;
-  if (any_block) {  // the first block is loaded beside its mask
-    load_k(blk);
-    load_v(blk);
-    see = load_mask(blk);
-    need = MASK == MASK_NONE || __any_sync(0xffffffffu, see != 0);
-  }
-  for (; blk < blk1; blk += warps) {
-    const int next = blk + warps;
-    uint32_t see_next = 0;
-    bool need_next = false;
+  load_add(blk0 + warp);
+  for (int n = 0, blk = blk0 + warp; blk < blk1; ++n, blk += warps) {
+    cp_async_wait_group<ST - 2>();  // this block's copies (one group a block) are done, for every lane
+    __syncwarp();
+    issue(blk + (ST - 1) * warps, (n + ST - 1) % ST);  // into the stage of the block before this one
+    if (MASK == MASK_ADD) {
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) mk[i] = mk_next[i];
+      load_add(blk + warps);
+    }
+    if (MASK == MASK_BITS && blk < first) continue;
+    any_block = true;
+    const uint32_t stage = (uint32_t)(n % ST) * STAGE;
+    // ---------------- which of this thread's scores count: [half][tile][row]
+    const bool is_past = blk < pblocks;
+    const int k0 = (is_past ? blk : blk - pblocks) * AR_KB, pos0 = (is_past ? 0 : p.tp) + k0;
+    const int seg_end = is_past ? past : p.tp + keys;
+    uint32_t see = ~0u;
+    if (MASK != MASK_NONE || pos0 + AR_KB > min(lim_all, seg_end)) {
+      see = 0;
+      const int bit = (blk - blk0) * AR_KB;
+#pragma unroll
+      for (int n2 = 0; n2 < NT; ++n2)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t bits = 0xffffu;
+          if (MASK == MASK_BITS)
+            bits = s_bits[(one_row ? 0 : min(8 * n2 + 2 * t + e, rows - 1)) * (AF_ROWS_MASK_KEYS / 32) + (bit >> 5)] >> (bit & 31);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int pos = pos0 + 8 * h + g, i = (h * NT + n2) * 2 + e;
+            bool ok = pos < min(lim[n2][e], seg_end) && ((bits >> (8 * h + g)) & 1u);
+            if (MASK == MASK_ADD) {
+              ok = ok && mk[i] != -INFINITY;
+              if (!ok) mk[i] = 0.0f;
+            }
+            see |= (ok ? 1u : 0u) << i;
+          }
+        }
+    }
     // ---------------- S^T
-    float s[KM][NT][4];
-    if (need) {
+    uint4 k[2][NC];
 #pragma unroll
-      for (int m = 0; m < KM; ++m)
+    for (int c = 0; c < NC; ++c) {
+      const uint32_t at = k_row + stage + (((t + 4 * c) ^ k_swz) << 4);
+      k[0][c] = lds128(at);
+      k[1][c] = lds128(at + 8 * ROW);
+    }
+    float s[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+    for (int n2 = 0; n2 < NT; ++n2) {
+      float s2[4];  // two chains of products
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][n][e] = 0.0f;
-          if (n == 1 && !two) continue;
+      for (int e = 0; e < 4; ++e) s[n2][e] = s2[e] = 0.0f;
+      if (n2 == 1 && !two) continue;
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            mma_16816(s[m][n], k[m][0][c].x, k[m][1][c].x, k[m][0][c].y, k[m][1][c].y, q[n][c].x, q[n][c].y);
-            mma_16816(s[m][n], k[m][0][c].z, k[m][1][c].z, k[m][0][c].w, k[m][1][c].w, q[n][c].z, q[n][c].w);
-          }
-        }
-      // scores in log2 units; entries the row does not see are -inf
-#pragma unroll
-      for (int m = 0; m < KM; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][n][e] *= sc;
-      if (MASK != MASK_NONE || see != ~0u) {
-#pragma unroll
-        for (int m = 0; m < KM; ++m)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int i = ((m * 2 + (e >> 1)) * NT + n) * 2 + (e & 1);
-              if (!((see >> i) & 1u)) s[m][n][e] = -INFINITY;
-            }
+      for (int c = 0; c < NC; ++c) {
+        mma_16816(s[n2], k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, q[n2][c].x, q[n2][c].y);
+        mma_16816(s2, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, q[n2][c].z, q[n2][c].w);
       }
-      bool grow = false;
-      float top[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int e = 0; e < 4; ++e) s[n2][e] = (s[n2][e] + s2[e]) * sc;
+    }
+    // V in K's registers, on its way during the softmax
+    uint4 v[NS][4];
+#pragma unroll
+    for (int sl = 0; sl < NS; ++sl) {
+      const uint32_t at = v_row + stage;
+      v[sl][0] = lds128(at + (((8 * sl + g) ^ v_swz0) << 4));
+      v[sl][1] = lds128(at + ROW + (((8 * sl + g) ^ v_swz1) << 4));
+      v[sl][2] = lds128(at + 8 * ROW + (((8 * sl + g) ^ v_swz0) << 4));
+      v[sl][3] = lds128(at + 9 * ROW + (((8 * sl + g) ^ v_swz1) << 4));
+    }
+    // scores in log2 units; entries the row does not see are -inf
+    if (see != ~0u) {
+#pragma unroll
+      for (int n2 = 0; n2 < NT; ++n2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!((see >> (((e >> 1) * NT + n2) * 2 + (e & 1))) & 1u)) s[n2][e] = -INFINITY;
+    }
+    bool grow = false;
+    float top[NT][2];
+#pragma unroll
+    for (int n2 = 0; n2 < NT; ++n2)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (n2 == 1 && !two) continue;
+        float x0 = s[n2][e], x1 = s[n2][2 + e];
+        if (MASK == MASK_ADD) {
+          x0 = fmaf(mk[n2 * 2 + e], AFK_LOG2E, x0);
+          x1 = fmaf(mk[(NT + n2) * 2 + e], AFK_LOG2E, x1);
+        }
+        const float x = fmaxf(x0, x1);
+        top[n2][e] = x;
+        grow = grow || x > m_ref[n2][e] + AFK_RESCALE || (m_ref[n2][e] == -INFINITY && x > -INFINITY);
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int n2 = 0; n2 < NT; ++n2)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (n == 1 && !two) continue;
-          float x = -INFINITY;
+          if (n2 == 1 && !two) continue;
+          float x = top[n2][e];
 #pragma unroll
-          for (int m = 0; m < KM; ++m)
+          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+          const float old = m_ref[n2][e];
+          if (x > old + AFK_RESCALE || old == -INFINITY) {
+            m_ref[n2][e] = x;
+            const float alpha = old == -INFINITY ? 0.0f : ex2_approx(old - x);
+            l[n2][e] *= alpha;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float y = s[m][n][2 * h + e];
-              if (MASK == MASK_ADD) y = fmaf(mk[((m * 2 + h) * NT + n) * 2 + e], AFK_LOG2E, y);
-              x = fmaxf(x, y);
-            }
-          top[n][e] = x;
-          grow = grow || x > m_ref[n][e] + AFK_RESCALE || (m_ref[n][e] == -INFINITY && x > -INFINITY);
-        }
-      if (__any_sync(0xffffffffu, grow)) {
+            for (int sl = 0; sl < NS; ++sl)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if (n == 1 && !two) continue;
-            float x = top[n][e];
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            const float old = m_ref[n][e];
-            if (x > old + AFK_RESCALE || old == -INFINITY) {
-              m_ref[n][e] = x;
-              const float alpha = old == -INFINITY ? 0.0f : ex2_approx(old - x);
-              l[n][e] *= alpha;
-#pragma unroll
-              for (int sl = 0; sl < NS; ++sl)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  o[n][sl][j][e] *= alpha;
-                  o[n][sl][j][e + 2] *= alpha;
-                }
-            }
+              for (int j = 0; j < 4; ++j) {
+                o[n2][sl][j][e] *= alpha;
+                o[n2][sl][j][e + 2] *= alpha;
+              }
           }
-      }
-      // weights
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (n == 1 && !two) continue;
-          const float neg = m_ref[n][e] == -INFINITY ? 0.0f : -m_ref[n][e];
-#pragma unroll
-          for (int m = 0; m < KM; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float off = neg;
-              if (MASK == MASK_ADD) off = fmaf(mk[((m * 2 + h) * NT + n) * 2 + e], AFK_LOG2E, neg);
-              s[m][n][2 * h + e] = ex2_approx(s[m][n][2 * h + e] + off);
-              l[n][e] += s[m][n][2 * h + e];
-            }
         }
     }
-    // ---------------- the next block's mask and K, then O^T += V^T P^T
-    if (next < blk1) {
-      see_next = load_mask(next);
-      need_next = MASK == MASK_NONE || __any_sync(0xffffffffu, see_next != 0);
-      if (need_next) load_k(next);
+    // ---------------- weights, as the B operand of the second product
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int n2 = 0; n2 < NT; ++n2) {
+      if (n2 == 1 && !two) continue;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float neg = m_ref[n2][e] == -INFINITY ? 0.0f : -m_ref[n2][e];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float off = neg;
+          if (MASK == MASK_ADD) off = fmaf(mk[(h * NT + n2) * 2 + e], AFK_LOG2E, neg);
+          s[n2][2 * h + e] = ex2_approx(s[n2][2 * h + e] + off);
+          l[n2][e] += s[n2][2 * h + e];
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) pb[n2][h] = transpose_8x8(pack_f16x2(s[n2][2 * h], s[n2][2 * h + 1]));
     }
-    if (need) {
+    // ---------------- O^T += V^T P^T
 #pragma unroll
-      for (int m = 0; m < KM; ++m) {
-        uint32_t pb[NT][2];
+    for (int sl = 0; sl < NS; ++sl) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (n == 0 || two) pb[n][h] = transpose_8x8(pack_f16x2(s[m][n][2 * h], s[m][n][2 * h + 1]));
-#pragma unroll
-        for (int sl = 0; sl < NS; ++sl)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t w0 = word_of(v[m][0][sl], j), w1 = word_of(v[m][1][sl], j);
-            const uint32_t w2 = word_of(v[m][2][sl], j), w3 = word_of(v[m][3][sl], j);
-            const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
-            const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
-            mma_16816(o[0][sl][j], a0, a1, a2, a3, pb[0][0], pb[0][1]);
-            if (NT == 2 && two) mma_16816(o[NT - 1][sl][j], a0, a1, a2, a3, pb[NT - 1][0], pb[NT - 1][1]);
-          }
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w0 = word_of(v[sl][0], j), w1 = word_of(v[sl][1], j);
+        const uint32_t w2 = word_of(v[sl][2], j), w3 = word_of(v[sl][3], j);
+        const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
+        const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
+        mma_16816(o[0][sl][j], a0, a1, a2, a3, pb[0][0], pb[0][1]);
+        if (NT == 2 && two) mma_16816(o[NT - 1][sl][j], a0, a1, a2, a3, pb[NT - 1][0], pb[NT - 1][1]);
       }
     }
-    if (need_next) load_v(next);
-    see = see_next;
-    need = need_next;
+    __syncwarp();  // the stage's readers are done before its next copies
   }
+  cp_async_wait_group<0>();
 
-  // ---------------- merge the warps, write the rows
+  // ---------------- merge the warps (over the rings), write the rows
+  __syncthreads();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     if (n == 1 && !two) continue;
@@ -395,27 +449,46 @@ __global__ void __launch_bounds__(32 * AR_WARPS, NS == 2 && NT == 2 ? 1 : 2)
     }
   }
   __syncthreads();
+  // thread (row, warp): that warp's factor 2^(m - M) in place of its m, the row's M and sum beside them
+  {
+    const int r = threadIdx.x >> 3, w = threadIdx.x & 7;
+    if (r < 8 * NT) {  // whole groups of eight lanes; CTAs of fewer threads than rows x 8 go around below
+      for (int rr = r; rr < 8 * NT; rr += blockDim.x >> 3) {
+        const bool in = w < warps && rr < rows;
+        const float lw = in ? s_l[w][rr] : 0.0f, mw = in && lw != 0.0f ? s_m[w][rr] : -INFINITY;
+        float m = mw, sum;
+#pragma unroll
+        for (int d = 4; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d, 8));
+        const float f = lw != 0.0f ? ex2_approx(mw - m) : 0.0f;
+        sum = f * lw;
+#pragma unroll
+        for (int d = 4; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d, 8);
+        if (in) s_m[w][rr] = f;
+        if (w == 0 && rr < rows) s_row[rr] = make_float2(m, sum);
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
   for (int i = threadIdx.x; i < rows * 16 * NS; i += blockDim.x) {
     const int r = i / (16 * NS), d = (i % (16 * NS)) * 4;
-    float m = -INFINITY, sum = 0.0f;
-    for (int w = 0; w < warps; ++w)
-      if (s_l[w][r] != 0.0f) m = fmaxf(m, s_m[w][r]);
+    if (d >= p.DV) continue;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < warps; ++w) {
-      if (s_l[w][r] == 0.0f) continue;
-      const float f = ex2_approx(s_m[w][r] - m);
+#pragma unroll
+    for (int w = 0; w < AR_WARPS; ++w) {
+      const float f = w < warps ? s_m[w][r] : 0.0f;
+      if (f == 0.0f) continue;  // a warp without keys has written no output
       const float4 x = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
-      sum += f * s_l[w][r];
       acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
     }
-    if (d >= p.DV) continue;
+    const float2 ms = s_row[r];
     const RowId w = row_of(row0 + r, p.group, p.TQ, kvh, b, past_item);
     if (p.part_o) {
       const int64_t at = (int64_t)(cl.part0 + split) * ((int64_t)p.B * (int)p.TQ.d * p.HQ) + ((int64_t)w.b * (int)p.TQ.d + w.t) * p.HQ + w.h;
-      if (d == 0) p.part_ml[at] = make_float2(m, sum);
+      if (d == 0) p.part_ml[at] = ms;
       *reinterpret_cast<float4*>(p.part_o + at * p.DV + d) = acc;
     } else {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float inv = ms.y == 0.0f ? 0.0f : 1.0f / ms.y;
       *reinterpret_cast<uint2*>(p.o + (int64_t)w.b * p.o_sb + (int64_t)w.h * p.o_sh + (int64_t)w.t * p.o_st + d) =
           make_uint2(pack_f16x2(acc.x * inv, acc.y * inv), pack_f16x2(acc.z * inv, acc.w * inv));
     }
@@ -428,34 +501,37 @@ __global__ void __launch_bounds__(32 * AR_WARPS, NS == 2 && NT == 2 ? 1 : 2)
 
 // ------------------------------------------------------------------ host side
 static size_t rows_smem(int ns, int nt, int warps) {
-  return (size_t)warps * 8 * nt * (64 * ns + 4 + 2) * sizeof(float);
+  const size_t merge = (size_t)warps * 8 * nt * (64 * ns + 4 + 2) * sizeof(float), ring = (size_t)warps * AR_RING;
+  return merge > ring ? merge : ring;
 }
 
 template <int NS, int NT>
-static cudaError_t launch_variant(const RowsParams& p, int mask, int warps, unsigned items, cudaStream_t stream) {
-  auto kernel = mask == MASK_NONE ? attention_rows_kernel<NS, NT, MASK_NONE>
-                : mask == MASK_BITS ? attention_rows_kernel<NS, NT, MASK_BITS>
-                                    : attention_rows_kernel<NS, NT, MASK_ADD>;
-  return launch_pdl(kernel, dim3(items), dim3(32 * warps), rows_smem(NS, NT, warps), stream, p);
+static const void* rows_kernel(int mask) {
+  return mask == MASK_NONE ? (const void*)attention_rows_kernel<NS, NT, MASK_NONE>
+         : mask == MASK_BITS ? (const void*)attention_rows_kernel<NS, NT, MASK_BITS>
+                             : (const void*)attention_rows_kernel<NS, NT, MASK_ADD>;
+}
+
+static const void* rows_kernel(bool wide, int row_tiles, int mask) {
+  if (row_tiles == 1) return wide ? rows_kernel<2, 1>(mask) : rows_kernel<1, 1>(mask);
+  return wide ? rows_kernel<2, 2>(mask) : rows_kernel<1, 2>(mask);
 }
 
 cudaError_t prepare_attention_rows() {
-  // only the widest form needs more than a launch's default shared memory
-  cudaError_t e = cudaSuccess;
-  for (auto kernel : {attention_rows_kernel<2, 2, MASK_NONE>, attention_rows_kernel<2, 2, MASK_BITS>,
-                      attention_rows_kernel<2, 2, MASK_ADD>})
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem(2, 2, AR_WARPS));
-  return e;
+  for (int i = 0; i < 12; ++i) {
+    cudaError_t e = cudaFuncSetAttribute(rows_kernel(i & 1, 1 + ((i >> 1) & 1), i >> 2),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, AR_WARPS * AR_RING);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 cudaError_t launch_attention_rows(const RowsParams& p, int row_tiles, int mask, int warps, unsigned items,
                                   cudaStream_t stream) {
   if (warps < 1 || warps > AR_WARPS) return cudaErrorInvalidValue;
   const bool wide = p.D > 64 || p.DV > 64;
-  if (row_tiles == 1)
-    return wide ? launch_variant<2, 1>(p, mask, warps, items, stream) : launch_variant<1, 1>(p, mask, warps, items, stream);
-  return wide ? launch_variant<2, 2>(p, mask, warps, items, stream) : launch_variant<1, 2>(p, mask, warps, items, stream);
+  auto kernel = reinterpret_cast<void (*)(const RowsParams)>(const_cast<void*>(rows_kernel(wide, row_tiles, mask)));
+  return launch_pdl(kernel, dim3(items), dim3(32 * warps), rows_smem(wide ? 2 : 1, row_tiles, warps), stream, p);
 }
 
 }  // namespace emx

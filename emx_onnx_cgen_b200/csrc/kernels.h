@@ -117,6 +117,7 @@ enum {
 enum { AFF_SCALE };
 enum { AF_PASS_NONE = 0, AF_PASS_ROWS8 = 1, AF_PASS_ROWS16 = 2 /*attention_rows.cu*/, AF_PASS_TILES = 3 /*attention_flash.cu*/,
        AF_PASS_WIDE = 4 /*attention_wide.cu*/ };
+enum { AF_ROWS_MASK_KEYS = 4096 };  // most keys of a few-row work item under a boolean mask
 enum { AF_MASK_NONE = 0, AF_MASK_BOOL = 1, AF_MASK_F16 = 2, AF_MASK_F32 = 3 };
 
 // ---- K_RMS_NORM: t[0]=x, t[1]=scale, t[2]=y; rows of RN_N contiguous elements

@@ -296,20 +296,24 @@ class FlashSchedule:
         return self.splits_own + self.splits_past
 
 
-def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, additive: bool = False) -> FlashSchedule:
-    """``rows``: query rows of one sequence per key/value head."""
+def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, mask: str = "", head: int = 128) -> FlashSchedule:
+    """``rows``: query rows of one sequence per key/value head; ``mask``: its dtype; ``head``: the head size."""
     tiles = lambda n, m: -(-n // m)
+    blocks = lambda *parts: sum(tiles(t, 16) for t in parts)
+    additive = mask not in ("", "bool")
+    # key ranges that the few-row pass needs at least: it keeps a range's boolean mask on chip
+    at_least = lambda n: tiles(n * 16, K.AF_ROWS_MASK_KEYS) if mask == "bool" else 1
     sms = K.LP_PLAN_SMS
     few = rows <= 16
 
-    def tile_pass(parts):
+    def tile_pass(parts, share=1.0):
         """Pass and splits for [(rows, heads, keys)]: two row tiles a work item
         where all rows fill more than one (attention_wide.cu has no additive
         masks), one item per SM then, else one tile and two items."""
         wide = not additive and all(n > FLASH_ROWS for n, _, _ in parts)
-        m, per_sm, least = (2 * FLASH_ROWS, 1, 8) if wide else (FLASH_ROWS, 2, 4)
+        m, per_sm, least = (2 * FLASH_ROWS, share, 8) if wide else (FLASH_ROWS, 2, 1 if additive else 4)
         return (K.AF_PASS_WIDE if wide else K.AF_PASS_TILES,
-                flash_splits([(h * tiles(n, m), tiles(t, FLASH_KEYS)) for n, h, t in parts], per_sm * sms, least))
+                flash_splits([(h * tiles(n, m), tiles(t, FLASH_KEYS)) for n, h, t in parts], int(per_sm * sms), least))
 
     # A sequence with at least a tile of rows reads a shared past for itself: packing other sequences' rows beside
     # them would save no read of it, and cost the merge.
@@ -317,19 +321,25 @@ def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, 
     keys = tk if apart else tp + tk
     if few:
         packed = b * rows
-        own = K.AF_PASS_ROWS8 if rows <= 8 and not (apart and packed > 8) else K.AF_PASS_ROWS16
-        m = 8 if own == K.AF_PASS_ROWS8 else 16
-        work = [(b * hkv, tiles(keys, 64))]
+        # A work item of eight warps fills an SM; with an item for every SM, two of four warps share one instead.
+        warps = lambda items: 4 if items >= sms else 8
+        own = K.AF_PASS_ROWS8 if rows <= 8 else K.AF_PASS_ROWS16
         if not apart:
-            return FlashSchedule(own, K.AF_PASS_NONE, flash_splits(work, 2 * sms, 8)[0], 0)
-        if packed <= 64:
-            # up to four tiles of 16 rows read the past's keys from L2 once each: less than a second kernel costs
-            work.append((hkv * tiles(packed, m), tiles(tp, 64)))
-            so, sp = flash_splits(work, 2 * sms, 8)
-            return FlashSchedule(own, own, so, sp)
-        so = flash_splits(work, 4 * sms, 8)[0]
-        past, sp = tile_pass([(packed, hkv, tp)])
-        return FlashSchedule(K.AF_PASS_ROWS8 if rows <= 8 else K.AF_PASS_ROWS16, past, so, sp[0], 4)
+            so = max(flash_splits([(b * hkv, tiles(keys, 64))], sms, 8)[0], at_least(blocks(tp, tk)))
+            return FlashSchedule(own, K.AF_PASS_NONE, so, 0, warps(b * hkv * so))
+        if packed <= (64 if head <= 64 else 32):
+            # Up to four row tiles read the past's keys from L2 once each, which costs less than a tile pass takes to
+            # set up (7 sequences x 9 rows, 1001 keys, D = 64: 14.4 against 16.4 us; 16 x 4, 2048 keys, D = 128: 18.5
+            # against 16.4 us).
+            own = K.AF_PASS_ROWS8 if packed <= 8 else K.AF_PASS_ROWS16
+            items = hkv * tiles(packed, 8 if packed <= 8 else 16)
+            sp = max(flash_splits([(items, tiles(tp, 64))], sms, 4)[0], at_least(blocks(tp)))
+            return FlashSchedule(own, own, max(1, at_least(blocks(tk))), sp, 8)
+        so = max(flash_splits([(b * hkv, tiles(keys, 64))], 2 * sms, 8)[0], at_least(blocks(tk)))
+        # the sequences' own keys run beside the past on the SMs it leaves: 3/5 of them give the shortest whole
+        # (128 sequences, 8192 + 256 keys: 68 us with 5 key ranges, 83 us with 9)
+        past, sp = tile_pass([(packed, hkv, tp)], 0.6)
+        return FlashSchedule(own, past, so, sp[0], 4)
     own, splits = tile_pass([(rows, b * hkv, keys)] + ([(b * rows, hkv, tp)] if apart else []))
     return FlashSchedule(own, own if apart else K.AF_PASS_NONE, splits[0], splits[1] if apart else 0)
 
@@ -1583,7 +1593,7 @@ class B200PlanEmitter:
             if not shared:
                 batched = batched and all(self._fixed_or_batched(n, True) for n in names)
         sch = flash_schedule(b, hkv, tq * (hq // hkv), tk, tp, shared,
-                             t_mask >= 0 and kind != K.AF_MASK_BOOL)
+                             self._dtype(op.input_attn_mask) if t_mask >= 0 else "", max(d, dv))
         ip.update({K.AF_PASS_OWN: sch.own, K.AF_PASS_PAST: sch.past, K.AF_SPLITS_K: sch.splits_own,
                    K.AF_SPLITS_P: sch.splits_past, K.AF_WARPS: sch.warps})
         if sch.slots > 1:

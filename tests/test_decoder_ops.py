@@ -217,19 +217,27 @@ def test_schedules():
     assert pick(2, 2, 12, 1500, 0, False) == (rows16, none)
     assert pick(2, 2, 17, 1500, 0, False) == (tiles, none)
     assert pick(4, 2, 4, 10, 500, False) == (rows8, none)       # a past of its own is part of the row's keys
-    assert pick(16, 8, 4, 33, 2048, True) == (rows16, rows16)   # 64 packed rows
+    assert pick(8, 8, 4, 33, 2048, True) == (rows16, rows16)    # 32 packed rows
+    assert pick(16, 8, 4, 33, 2048, True, "", 64) == (rows16, rows16)
+    assert pick(16, 8, 4, 33, 2048, True) == (rows8, tiles)
     assert pick(2, 8, 4, 33, 2048, True) == (rows8, rows8)
-    assert pick(17, 8, 4, 33, 2048, True) == (rows8, tiles)
     assert pick(33, 8, 4, 33, 2048, True) == (rows8, wide)
-    assert pick(33, 8, 4, 33, 2048, True, True) == (rows8, tiles)  # additive masks: no wide form
+    assert pick(33, 8, 4, 33, 2048, True, "f16") == (rows8, tiles)  # additive masks: no wide form
     assert pick(2, 2, 129, 1500, 0, False) == (wide, none)
-    assert pick(2, 2, 129, 1500, 0, False, True) == (tiles, none)
+    assert pick(2, 2, 129, 1500, 0, False, "f32") == (tiles, none)
     assert pick(1, 8, 4, 33, 2048, True) == (rows8, none)       # nobody to share with
     assert pick(3, 8, 100, 33, 2048, True) == (tiles, tiles)
     assert pick(3, 8, 128, 33, 2048, True) == (tiles, none)
     for args in ((1, 1, 1, 5000, 0, False), (128, 8, 4, 256, 8192, True), (7, 4, 9, 40, 1001, True)):
         s = flash_schedule(*args)
         assert s.slots == s.splits_own + s.splits_past and (s.splits_past > 0) == (s.past != none)
+    # the few-row pass holds a key range's boolean mask on chip
+    for b, tk, tp, shared in ((400, 9000, 0, False), (400, 4097, 0, False), (2, 9000, 20000, True), (300, 5000, 70000, False)):
+        s = flash_schedule(b, 8, 4, tk, tp, shared, "bool")
+        blocks = lambda *parts: sum(-(-t // 16) for t in parts)
+        own, past = (blocks(tk), blocks(tp)) if s.past != none else (blocks(tk, tp), 0)
+        assert -(-own // s.splits_own) * 16 <= K.AF_ROWS_MASK_KEYS
+        assert s.past not in (rows8, rows16) or -(-past // s.splits_past) * 16 <= K.AF_ROWS_MASK_KEYS
 
 
 def test_partials_are_reserved_for_split_or_two_part_keys():
