@@ -585,46 +585,51 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __r
 
 // ------------------------------------------------------------------ packing boolean masks
 // One CTA per mask row of `len` bytes (key k: past keys first); words of segment
-// 1 (the past) come first, then those of segment 0, each segment from a fresh word.
+// 1 (the past) come first, then those of segment 0, each segment from a fresh
+// word.  A thread makes 16 bits (2 bytes of a word) from 16 mask bytes: one load
+// where they lie on 16 bytes and within the row, else one by one.
 __global__ void __launch_bounds__(256) mask_pack_kernel(const uint8_t* __restrict__ mask, int len, int past, int keys,
-                                                        int words1, int words,
+                                                        int words1, int words, int vec,
                                                         unsigned long long* __restrict__ bits, int4* __restrict__ spans) {
   __shared__ int s_span[4];  // first and end of segment 0, first and end of segment 1
   pdl_wait();
   pdl_launch_dependents();
   if (threadIdx.x < 4) s_span[threadIdx.x] = threadIdx.x & 1 ? 0 : 0x7fffffff;
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x;
   const uint8_t* src = mask + row * len;
+  uint16_t* dst = reinterpret_cast<uint16_t*>(bits + row * words);
   int lo[2] = {0x7fffffff, 0x7fffffff}, hi[2] = {0, 0};
-  // a warp takes eight consecutive words at a time and loads them all before the first ballot
-  for (int w0 = warp * 8; w0 < words; w0 += 64) {
-    bool v[8][2];
+#pragma unroll 2
+  for (int i = threadIdx.x; i < words * 4; i += 256) {
+    const int seg = i < words1 * 4 ? 1 : 0;
+    const int k0 = (seg ? i : i - words1 * 4) * 16, at = (seg ? 0 : past) + k0;  // key of the segment, of the row
+    const int n = min((seg ? past : keys) - k0, len - at);                       // keys of these 16 that exist
+    uint32_t m = 0;
+    if (vec && n >= 16) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + at));
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      // bytes that are not 0 -> bits 0, 8, 16, 24 -> the top nibble in order
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int wd = w0 + i, seg = wd < words1 ? 1 : 0;
-      const int ka = (seg ? wd : wd - words1) * 64 + lane, n = seg ? past : keys, base = seg ? 0 : past;
-      v[i][0] = wd < words && ka < n && base + ka < len && src[base + ka] != 0;
-      v[i][1] = wd < words && ka + 32 < n && base + ka + 32 < len && src[base + ka + 32] != 0;
-    }
-    unsigned long long mine = 0;
+      for (int e = 0; e < 4; ++e) m |= (((__vcmpne4(w[e], 0u) & 0x01010101u) * 0x10204080u) >> 28) << (4 * e);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t wa = __ballot_sync(0xffffffffu, v[i][0]), wb = __ballot_sync(0xffffffffu, v[i][1]);
-      const unsigned long long w = (unsigned long long)wa | ((unsigned long long)wb << 32);
-      if (lane == i) mine = w;
-      const int seg = w0 + i < words1 ? 1 : 0, k0 = (seg ? w0 + i : w0 + i - words1) * 64;
-      if (w) {
-        lo[seg] = min(lo[seg], k0 + __ffsll((long long)w) - 1);
-        hi[seg] = max(hi[seg], k0 + 64 - __clzll((long long)w));
-      }
+      for (int e = 0; e < 16; ++e)
+        if (e < n && src[at + e] != 0) m |= 1u << e;
     }
-    if (lane < 8 && w0 + lane < words) bits[row * words + w0 + lane] = mine;
+    dst[i] = (uint16_t)m;
+    if (m) {
+      if (seg) lo[1] = min(lo[1], k0 + __ffs(m) - 1), hi[1] = max(hi[1], k0 + 32 - __clz(m));
+      else lo[0] = min(lo[0], k0 + __ffs(m) - 1), hi[0] = max(hi[0], k0 + 32 - __clz(m));
+    }
   }
-  if (lane < 2 && hi[lane]) {
-    atomicMin(&s_span[2 * lane], lo[lane]);
-    atomicMax(&s_span[2 * lane + 1], hi[lane]);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int l = __reduce_min_sync(0xffffffffu, lo[s]), h = __reduce_max_sync(0xffffffffu, hi[s]);
+    if ((threadIdx.x & 31) == 0 && h) {
+      atomicMin(&s_span[2 * s], l);
+      atomicMax(&s_span[2 * s + 1], h);
+    }
   }
   __syncthreads();
   if (threadIdx.x == 0) spans[row] = make_int4(s_span[0], s_span[1], s_span[2], s_span[3]);
@@ -862,7 +867,9 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
         p.spans = (const int4*)ptr(9);
         p.bits = (const unsigned long long*)(p.spans + mrows);
         e = launch_pdl(mask_pack_kernel, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, r.mask_bool, p.mask_len, p.tp,
-                       p.tk, p.words_past, p.words, (unsigned long long*)p.bits, (int4*)p.spans);
+                       p.tk, p.words_past, p.words,
+                       (int)(p.mask_len % 16 == 0 && p.tp % 16 == 0 && ((uintptr_t)r.mask_bool & 15u) == 0),
+                       (unsigned long long*)p.bits, (int4*)p.spans);
         ++*launches;
       } else if (variant == MASK_ADD && op.ip[AF_MASK_PADDED]) {
         if (p.add_f32)

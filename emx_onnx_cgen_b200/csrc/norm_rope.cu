@@ -109,24 +109,21 @@ __device__ __forceinline__ float inv_sqrt(float v) {
 // A lane's two pieces hold V pairs (f, s): (piece 0, piece 1) element by element, or neighbours of one piece
 // (INTER).  Norm scale and rotation make one 2 x 2 matrix per pair, formed once for the group's rows:
 //   f' = inv (f wf cos - s ws sin),  s' = inv (f wf sin + s ws cos).
-template <typename T, int LPR, int HPG, bool INTER>
-__global__ void __launch_bounds__(256, 3) norm_rope_kernel(const __grid_constant__ RopeParams p) {
+// RING > 0: lane groups stay and go from token to token; every lane copies its own pieces asynchronously to
+// shared memory, RING - 1 groups ahead, so that loads are under way all the time whatever the registers hold.
+template <typename T, int LPR, int HPG, int RING, bool INTER>
+__global__ void __launch_bounds__(256, RING ? 2 : 3) norm_rope_kernel(const __grid_constant__ RopeParams p) {
   constexpr int V = Chunk<T>::N;
+  constexpr int SLOTS = 2 * HPG;  // pieces of a lane per group
+  extern __shared__ uint4 s_ring[];  // [RING][SLOTS][256]
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t gi = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;  // lane group (their count fits 32 bits)
   const int u = threadIdx.x % LPR;
   // lanes of one group take the same path throughout and shuffle among themselves only
   const uint32_t group_mask = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << (threadIdx.x & 31 & ~(LPR - 1));
-  const uint32_t per_token = (uint32_t)(p.groups[0] + p.groups[1]);
-  const uint32_t token = gi / per_token;
-  if (token >= p.tokens) return;
-  int j = (int)(gi - token * per_token);
-  const int sel = j >= p.groups[0] ? 1 : 0;  // a group's rows are of one tensor
-  const RopeItem& it = p.item[sel];
-  const int step = p.groups[sel];
-  if (sel) j -= p.groups[0];
-  const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * (uint32_t)p.T);
+  const uint32_t per_token = (uint32_t)(p.groups[0] + p.groups[1]), total = (uint32_t)p.tokens * per_token;
+  const uint32_t stride = gridDim.x * (256u / LPR);
+  uint32_t gi = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;  // lane group (their count fits 32 bits)
   const int nc = p.D / V, rc = p.rot / V;
   // this lane's two pieces and whether they rotate
   int c0 = 2 * u, c1 = 2 * u + 1;
@@ -138,97 +135,150 @@ __global__ void __launch_bounds__(256, 3) norm_rope_kernel(const __grid_constant
   }
   const bool has0 = c0 < nc, has1 = c1 < nc;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  uint4 xv[HPG][2];
-  {
-    const T* x = static_cast<const T*>(it.x) + b * it.x_sb + t * it.x_st + j * it.x_sh;
-    const int64_t hop = step * it.x_sh;
+  // a group's token, tensor and first row
+  struct Place {
+    uint32_t token;
+    int sel, j, b, t;
+  };
+  auto place = [&](uint32_t at) {
+    Place w;
+    w.token = at / per_token;
+    w.j = (int)(at - w.token * per_token);
+    w.sel = w.j >= p.groups[0] ? 1 : 0;  // a group's rows are of one tensor
+    if (w.sel) w.j -= p.groups[0];
+    w.b = (int)(w.token / (uint32_t)p.T);
+    w.t = (int)(w.token - (uint32_t)w.b * (uint32_t)p.T);
+    return w;
+  };
+  auto fetch = [&](uint32_t at, int slot) {
+    if (at < total) {
+      const Place w = place(at);
+      const RopeItem& it = p.item[w.sel];
+      const int step = p.groups[w.sel];
+      const T* x = static_cast<const T*>(it.x) + w.b * it.x_sb + w.t * it.x_st + w.j * it.x_sh;
+      uint4* dst = s_ring + slot * SLOTS * 256 + threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < HPG; ++i) {
-      const bool in = j + i * step < it.heads;
-      xv[i][0] = in && has0 ? __ldcs(reinterpret_cast<const uint4*>(x + c0 * V)) : zero;
-      xv[i][1] = in && has1 ? __ldcs(reinterpret_cast<const uint4*>(x + c1 * V)) : zero;
-      x += hop;
+      for (int i = 0; i < HPG; ++i) {
+        if (w.j + i * step < it.heads) {
+          if (has0) cp_async16(dst + (2 * i) * 256, x + c0 * V);
+          if (has1) cp_async16(dst + (2 * i + 1) * 256, x + c1 * V);
+        }
+        x += step * it.x_sh;
+      }
     }
+    cp_async_commit();  // (an empty group keeps the count)
+  };
+  if (RING) {
+#pragma unroll
+    for (int n = 0; n < RING - 1; ++n) fetch(gi + n * stride, n);
   }
-  const bool norm = it.scale != nullptr;
-  F2 ff[V / 2], fs[V / 2], sf[V / 2], ss[V / 2];  // f' = inv (ff f - fs s), s' = inv (sf f + ss s), two pairs each
-  {
-    float w0[V], w1[V], cs[V], sn[V];
-    if (norm) {
-      const T* sc = static_cast<const T*>(it.scale);
-      Chunk<T>::unpack(has0 ? *reinterpret_cast<const uint4*>(sc + c0 * V) : zero, w0);
-      Chunk<T>::unpack(has1 ? *reinterpret_cast<const uint4*>(sc + c1 * V) : zero, w1);
-    } else {
+  int slot = 0;
+#pragma unroll 1
+  for (; gi < total; gi += stride) {
+    const Place w = place(gi);
+    const RopeItem& it = p.item[w.sel];
+    const int step = p.groups[w.sel];
+    uint4 xv[RING ? 1 : HPG][2];
+    if (!RING) {
+      const T* x = static_cast<const T*>(it.x) + w.b * it.x_sb + w.t * it.x_st + w.j * it.x_sh;
 #pragma unroll
-      for (int e = 0; e < V; ++e) w0[e] = w1[e] = 1.0f;
+      for (int i = 0; i < HPG; ++i) {
+        const bool in = w.j + i * step < it.heads;
+        xv[RING ? 0 : i][0] = in && has0 ? __ldcs(reinterpret_cast<const uint4*>(x + c0 * V)) : zero;
+        xv[RING ? 0 : i][1] = in && has1 ? __ldcs(reinterpret_cast<const uint4*>(x + c1 * V)) : zero;
+        x += step * it.x_sh;
+      }
     }
-    // cosines and sines of the V pairs: entries uV .. uV + V - 1 of the token's rows
-#pragma unroll
-    for (int e = 0; e < V; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
-    if (turn) {
-      const int64_t row = table_row(p, token);
-      if (row >= 0) {
-        const int64_t at = row * (p.rot / 2) + u * V;
-        Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.cos) + at), cs);
-        Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.sin) + at), sn);
+    const bool norm = it.scale != nullptr;
+    F2 ff[V / 2], fs[V / 2], sf[V / 2], ss[V / 2];  // f' = inv (ff f - fs s), s' = inv (sf f + ss s), two pairs each
+    {
+      float w0[V], w1[V], cs[V], sn[V];
+      if (norm) {
+        const T* sc = static_cast<const T*>(it.scale);
+        Chunk<T>::unpack(has0 ? *reinterpret_cast<const uint4*>(sc + c0 * V) : zero, w0);
+        Chunk<T>::unpack(has1 ? *reinterpret_cast<const uint4*>(sc + c1 * V) : zero, w1);
       } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
+        for (int e = 0; e < V; ++e) w0[e] = w1[e] = 1.0f;
+      }
+      // cosines and sines of the V pairs: entries uV .. uV + V - 1 of the token's rows
+#pragma unroll
+      for (int e = 0; e < V; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
+      if (turn) {
+        const int64_t row = table_row(p, w.token);
+        if (row >= 0) {
+          const int64_t at = row * (p.rot / 2) + u * V;
+          Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.cos) + at), cs);
+          Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.sin) + at), sn);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float(&wv)[V] = 2 * e < V ? w0 : w1;  // INTER: pairs e, e + 1 are four neighbours of one piece
+        const int at = (2 * e) % V;
+        const F2 wf = INTER ? F2(wv[at], wv[at + 2]) : F2(w0[e], w0[e + 1]);
+        const F2 ws = INTER ? F2(wv[at + 1], wv[at + 3]) : F2(w1[e], w1[e + 1]);
+        const F2 c2(cs[e], cs[e + 1]), s2(sn[e], sn[e + 1]), m2(-sn[e], -sn[e + 1]);
+        ff[e / 2] = mul2(wf, c2), fs[e / 2] = mul2(ws, m2), sf[e / 2] = mul2(wf, s2), ss[e / 2] = mul2(ws, c2);
       }
     }
-#pragma unroll
-    for (int e = 0; e < V; e += 2) {
-      const float(&w)[V] = 2 * e < V ? w0 : w1;  // INTER: pairs e, e + 1 are four neighbours of one piece
-      const int at = (2 * e) % V;
-      const F2 wf = INTER ? F2(w[at], w[at + 2]) : F2(w0[e], w0[e + 1]);
-      const F2 ws = INTER ? F2(w[at + 1], w[at + 3]) : F2(w1[e], w1[e + 1]);
-      const F2 c2(cs[e], cs[e + 1]), s2(sn[e], sn[e + 1]), m2(-sn[e], -sn[e + 1]);
-      ff[e / 2] = mul2(wf, c2), fs[e / 2] = mul2(ws, m2), sf[e / 2] = mul2(wf, s2), ss[e / 2] = mul2(ws, c2);
+    if (RING) {
+      cp_async_wait_group<RING ? RING - 2 : 0>();  // own copies of this group
+      fetch(gi + (RING - 1) * stride, (slot + RING - 1) % (RING ? RING : 1));
     }
-  }
-  T* y = static_cast<T*>(it.y) + b * it.y_sb + t * it.y_st + j * it.y_sh;
-  const int64_t hop = step * it.y_sh;
+    T* y = static_cast<T*>(it.y) + w.b * it.y_sb + w.t * it.y_st + w.j * it.y_sh;
+    const int64_t hop = step * it.y_sh;
 #pragma unroll
-  for (int i = 0; i < HPG; ++i) {
-    if (j + i * step >= it.heads) break;
-    float a[V], c[V];
-    Chunk<T>::unpack(xv[i][0], a);
-    Chunk<T>::unpack(xv[i][1], c);
-    F2 f[V / 2], s[V / 2];
-#pragma unroll
-    for (int e = 0; e < V; e += 2) {
-      const float(&x)[V] = 2 * e < V ? a : c;
-      const int at = (2 * e) % V;
-      f[e / 2] = INTER ? F2(x[at], x[at + 2]) : F2(a[e], a[e + 1]);
-      s[e / 2] = INTER ? F2(x[at + 1], x[at + 3]) : F2(c[e], c[e + 1]);
-    }
-    float inv = 1.0f;
-    if (norm) {
-      F2 q0 = mul2(f[0], f[0]), q1 = mul2(s[0], s[0]);
-#pragma unroll
-      for (int e = 1; e < V / 2; ++e) q0 = fma2(f[e], f[e], q0), q1 = fma2(s[e], s[e], q1);
-      float sum = (q0.lo() + q0.hi()) + (q1.lo() + q1.hi());
-#pragma unroll
-      for (int d = LPR / 2; d; d >>= 1) sum += __shfl_xor_sync(group_mask, sum, d, LPR);
-      inv = inv_sqrt(fmaf(sum, p.inv_d, it.eps));
-    }
-    const F2 inv2(inv, inv);
-#pragma unroll
-    for (int e = 0; e < V / 2; ++e) {
-      F2 f1 = mul2(ff[e], f[e]), s1 = mul2(ss[e], s[e]);
-      if (turn) {  // elements behind the rotation stay apart, whatever they hold
-        f1 = fma2(fs[e], s[e], f1);
-        s1 = fma2(sf[e], f[e], s1);
+    for (int i = 0; i < HPG; ++i) {
+      if (w.j + i * step >= it.heads) break;
+      if (RING) {
+        const uint4* src = s_ring + slot * SLOTS * 256 + threadIdx.x;
+        xv[0][0] = has0 ? src[(2 * i) * 256] : zero;
+        xv[0][1] = has1 ? src[(2 * i + 1) * 256] : zero;
       }
-      f1 = mul2(f1, inv2), s1 = mul2(s1, inv2);
-      float(&x)[V] = 4 * e < V ? a : c;
-      const int at = (4 * e) % V;
-      (INTER ? x[at] : a[2 * e]) = f1.lo(), (INTER ? x[at + 2] : a[2 * e + 1]) = f1.hi();
-      (INTER ? x[at + 1] : c[2 * e]) = s1.lo(), (INTER ? x[at + 3] : c[2 * e + 1]) = s1.hi();
+      float a[V], c[V];
+      Chunk<T>::unpack(xv[RING ? 0 : i][0], a);
+      Chunk<T>::unpack(xv[RING ? 0 : i][1], c);
+      F2 f[V / 2], s[V / 2];
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float(&x)[V] = 2 * e < V ? a : c;
+        const int at = (2 * e) % V;
+        f[e / 2] = INTER ? F2(x[at], x[at + 2]) : F2(a[e], a[e + 1]);
+        s[e / 2] = INTER ? F2(x[at + 1], x[at + 3]) : F2(c[e], c[e + 1]);
+      }
+      float inv = 1.0f;
+      if (norm) {
+        F2 q0 = mul2(f[0], f[0]), q1 = mul2(s[0], s[0]);
+#pragma unroll
+        for (int e = 1; e < V / 2; ++e) q0 = fma2(f[e], f[e], q0), q1 = fma2(s[e], s[e], q1);
+        float sum = (q0.lo() + q0.hi()) + (q1.lo() + q1.hi());
+#pragma unroll
+        for (int d = LPR / 2; d; d >>= 1) sum += __shfl_xor_sync(group_mask, sum, d, LPR);
+        inv = inv_sqrt(fmaf(sum, p.inv_d, it.eps));
+      }
+      const F2 inv2(inv, inv);
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) {
+        F2 f1 = mul2(ff[e], f[e]), s1 = mul2(ss[e], s[e]);
+        if (turn) {  // elements behind the rotation stay apart, whatever they hold
+          f1 = fma2(fs[e], s[e], f1);
+          s1 = fma2(sf[e], f[e], s1);
+        }
+        f1 = mul2(f1, inv2), s1 = mul2(s1, inv2);
+        float(&x)[V] = 4 * e < V ? a : c;
+        const int at = (4 * e) % V;
+        (INTER ? x[at] : a[2 * e]) = f1.lo(), (INTER ? x[at + 2] : a[2 * e + 1]) = f1.hi();
+        (INTER ? x[at + 1] : c[2 * e]) = s1.lo(), (INTER ? x[at + 3] : c[2 * e + 1]) = s1.hi();
+      }
+      if (has0) *reinterpret_cast<uint4*>(y + c0 * V) = Chunk<T>::pack(a);
+      if (has1) *reinterpret_cast<uint4*>(y + c1 * V) = Chunk<T>::pack(c);
+      y += hop;
     }
-    if (has0) *reinterpret_cast<uint4*>(y + c0 * V) = Chunk<T>::pack(a);
-    if (has1) *reinterpret_cast<uint4*>(y + c1 * V) = Chunk<T>::pack(c);
-    y += hop;
+    if (RING) slot = slot + 1 == RING ? 0 : slot + 1;
   }
 }
 
@@ -276,20 +326,32 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const __grid_constan
   for (int e = p.rot + lane; e < p.D; e += 32) from_f32(to_f32(x[e]) * inv * (sc ? to_f32(sc[e]) : 1.0f), y[e]);
 }
 
-template <typename T, int LPR, int HPG>
-static cudaError_t launch_vec_rows(RopeParams p, cudaStream_t stream) {
+constexpr int NR_RING = 3;  // groups of four rows a lane holds at once in shared memory: 96 KB a CTA, two CTAs an SM
+
+template <typename T, int LPR, int HPG, int RING>
+static cudaError_t launch_vec_rows(RopeParams p, int num_sms, cudaStream_t stream) {
   for (int i = 0; i < 2; ++i) p.groups[i] = (p.item[i].heads + HPG - 1) / HPG;
-  const int64_t groups = p.tokens * (p.groups[0] + p.groups[1]), blocks = (groups * LPR + 255) / 256;
-  if (groups > 0xffff0000ll || blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  auto kernel = p.interleaved ? norm_rope_kernel<T, LPR, HPG, true> : norm_rope_kernel<T, LPR, HPG, false>;
-  return launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+  const int64_t groups = p.tokens * (p.groups[0] + p.groups[1]);
+  int64_t blocks = (groups * LPR + 255) / 256;
+  // (the ring runs past the last group by less than a grid's worth)
+  if (groups > 0x7fff0000ll || blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (RING && blocks > 2 * num_sms) blocks = 2 * num_sms;
+  auto kernel = p.interleaved ? norm_rope_kernel<T, LPR, HPG, RING, true> : norm_rope_kernel<T, LPR, HPG, RING, false>;
+  const size_t smem = (size_t)RING * 2 * HPG * 256 * 16;
+  if (RING) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), smem, stream, p);
 }
 
 template <typename T, int LPR>
 static cudaError_t launch_vec(const RopeParams& p, const LaunchCtx& ctx) {
-  // Four rows per lane group once that still fills every SM's threads: fewer table loads and more bytes in flight
-  return p.tokens * p.heads * LPR >= (int64_t)ctx.num_sms * 2048 * 4 ? launch_vec_rows<T, LPR, 4>(p, ctx.stream)
-                                                                     : launch_vec_rows<T, LPR, 1>(p, ctx.stream);
+  // Four rows per lane group, in lane groups that stay, once there is work for each to go around more than once;
+  // before that, one row each at once.
+  return p.tokens * p.heads * LPR >= (int64_t)ctx.num_sms * 2048 * 4
+             ? launch_vec_rows<T, LPR, 4, NR_RING>(p, ctx.num_sms, ctx.stream)
+             : launch_vec_rows<T, LPR, 1, 0>(p, ctx.num_sms, ctx.stream);
 }
 
 template <typename T>
