@@ -168,9 +168,23 @@ __global__ void __launch_bounds__(256, RING ? 2 : 3) norm_rope_kernel(const __gr
     }
     cp_async_commit();  // (an empty group keeps the count)
   };
+  auto load_tables = [&](int64_t row, uint4& c4, uint4& s4) {
+    const int64_t at = row * (p.rot / 2) + u * V;
+    c4 = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.cos) + at);
+    s4 = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.sin) + at);
+  };
+  auto row_of_group = [&](uint32_t at) {
+    return turn && at < total ? table_row(p, at / per_token) : 0;
+  };
+  // The ring's table entries are read one group ahead, their row's number two (it may be a position to load).
+  int64_t row_now = 0, row_next = 0;
+  uint4 cos_next = zero, sin_next = zero;
   if (RING) {
 #pragma unroll
     for (int n = 0; n < RING - 1; ++n) fetch(gi + n * stride, n);
+    row_now = row_of_group(gi);
+    row_next = row_of_group(gi + stride);
+    if (turn && row_now >= 0) load_tables(row_now, cos_next, sin_next);
   }
   int slot = 0;
 #pragma unroll 1
@@ -202,17 +216,32 @@ __global__ void __launch_bounds__(256, RING ? 2 : 3) norm_rope_kernel(const __gr
         for (int e = 0; e < V; ++e) w0[e] = w1[e] = 1.0f;
       }
       // cosines and sines of the V pairs: entries uV .. uV + V - 1 of the token's rows
+      const uint4 tc = RING ? cos_next : zero, ts = RING ? sin_next : zero;
+      if (RING) {
+        cos_next = sin_next = zero;
+        if (turn && row_next >= 0) load_tables(row_next, cos_next, sin_next);
+        const bool bad = row_now < 0;
+        row_now = row_next;
+        row_next = row_of_group(gi + 2 * stride);
+        Chunk<T>::unpack(tc, cs);
+        Chunk<T>::unpack(ts, sn);
+        if (!turn || bad) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
-      if (turn) {
-        const int64_t row = table_row(p, w.token);
-        if (row >= 0) {
-          const int64_t at = row * (p.rot / 2) + u * V;
-          Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.cos) + at), cs);
-          Chunk<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.sin) + at), sn);
-        } else {
+          for (int e = 0; e < V; ++e) cs[e] = turn ? __int_as_float(0x7fc00000) : 1.0f, sn[e] = turn ? cs[e] : 0.0f;
+        }
+      } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
+        for (int e = 0; e < V; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
+        if (turn) {
+          const int64_t row = table_row(p, w.token);
+          uint4 c4 = zero, s4 = zero;
+          if (row >= 0) load_tables(row, c4, s4);
+          Chunk<T>::unpack(c4, cs);
+          Chunk<T>::unpack(s4, sn);
+          if (row < 0) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
+          }
         }
       }
 #pragma unroll
