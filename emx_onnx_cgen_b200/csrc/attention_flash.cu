@@ -207,9 +207,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
   }
   // this split's share of the tiles
   const int j_lo = pbeg < pend ? pbeg / AFK_N : 0, j_hi = pbeg < pend ? (pend + AFK_N - 1) / AFK_N : 0;
-  const int per = j_hi - j_lo;
-  const int j0 = j_lo + (int)((long long)per * split / cl.splits);
-  const int J = j_lo + (int)((long long)per * (split + 1) / cl.splits) - j0;
+  const int j0 = j_lo + split_start(j_hi - j_lo, split, cl.splits);
+  const int J = j_lo + split_start(j_hi - j_lo, split + 1, cl.splits) - j0;
 
   if (warp == 0) {
     if (lane == 0 && J > 0) {
@@ -552,26 +551,43 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __r
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  float m = -INFINITY;
-  for (int s = lane; s < slots; s += 32) {
-    const float2 ml = part_ml[(int64_t)s * rows + row];
+  // lane s: slot s0 + s; the first 32 slots' (m, l) are loaded once
+  const float2 none = make_float2(-INFINITY, 0.0f);
+  float2 ml = lane < slots ? part_ml[(int64_t)lane * rows + row] : none;
+  const float2 first = ml;
+  float m = ml.y != 0.0f ? ml.x : -INFINITY;
+  for (int s = lane + 32; s < slots; s += 32) {
+    ml = part_ml[(int64_t)s * rows + row];
     if (ml.y != 0.0f) m = fmaxf(m, ml.x);
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
   float l = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < slots; ++s) {
-    const float2 ml = part_ml[(int64_t)s * rows + row];
-    if (ml.y == 0.0f) continue;  // this item saw no key of the row (its output is not written)
-    const float wgt = ex2_approx(ml.x - m);
-    l += wgt * ml.y;
-    if (lane * 4 < DV) {
-      const float4 v = *reinterpret_cast<const float4*>(part_o + ((int64_t)s * rows + row) * DV + lane * 4);
-      acc.x += wgt * v.x;
-      acc.y += wgt * v.y;
-      acc.z += wgt * v.z;
-      acc.w += wgt * v.w;
+  for (int s0 = 0; s0 < slots; s0 += 32) {
+    ml = s0 == 0 ? first : s0 + lane < slots ? part_ml[(int64_t)(s0 + lane) * rows + row] : none;
+    const float wgt = ml.y != 0.0f ? ex2_approx(ml.x - m) : 0.0f;
+    const uint32_t seen = __ballot_sync(0xffffffffu, ml.y != 0.0f);  // the others saw no key: their output is not written
+    float part_l = ml.y != 0.0f ? wgt * ml.y : 0.0f;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) part_l += __shfl_xor_sync(0xffffffffu, part_l, d);
+    l += part_l;
+    // four slots' loads at once
+    for (int s = 0; s < 32 && s0 + s < slots; s += 4) {
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = (seen >> (s + i)) & 1u && lane * 4 < DV
+                   ? *reinterpret_cast<const float4*>(part_o + ((int64_t)(s0 + s + i) * rows + row) * DV + lane * 4)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float ws = __shfl_sync(0xffffffffu, wgt, s + i);
+        acc.x += ws * v[i].x;
+        acc.y += ws * v[i].y;
+        acc.z += ws * v[i].z;
+        acc.w += ws * v[i].w;
+      }
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;

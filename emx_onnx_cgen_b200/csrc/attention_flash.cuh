@@ -62,6 +62,13 @@ struct ItemClass {
   int past;
 };
 
+// Item `split` of `splits` takes floor(n split / splits) up to the next item's first of n tiles (32-bit: n may be
+// 2^25, splits some hundreds).
+__device__ __forceinline__ int split_start(int n, int split, int splits) {
+  const int whole = n / splits;
+  return whole * split + (n - whole * splits) * split / splits;
+}
+
 struct TileParams {
   CUtensorMap map_k[2], map_v[2];  // current keys, past: 4-D (d, key, head, batch), box (64, tile keys, 1, 1), 128-byte swizzle
   CUtensorMap map_q[2];  // per class: 5-D (d, head of the group, token, key/value head, sequence), 128 rows a box

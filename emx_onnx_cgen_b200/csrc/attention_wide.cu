@@ -245,13 +245,16 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
       int pbeg = 0, pend = keys > 0 ? np * AW_N + keys : (cl.past ? p.tp : 0);
       if (MASK == MASK_BITS) {
         int lo = 0x7fffffff, hi = 0;
+        int4 v[8];  // (lanes past the last row read that row's again: no branch between the loads)
 #pragma unroll
-        for (int i = 0; i < 2 * AW_M; i += 32) {
-          if (i + lane >= w.rows) continue;
-          const RowId r = row_of(w.row0 + i + lane, p.group, p.TQ, w.kvh, w.b, w.shared);
-          const int4 v = p.spans[r.b * p.mask_sb + r.h * p.mask_sh + r.t * p.mask_st];
-          if (cl.past && v.z < v.w) lo = min(lo, v.z), hi = max(hi, v.w);
-          if (!w.shared && v.x < v.y) lo = min(lo, np * AW_N + v.x), hi = max(hi, np * AW_N + v.y);
+        for (int i = 0; i < 8; ++i) {
+          const RowId r = row_of(w.row0 + min(32 * i + lane, w.rows - 1), p.group, p.TQ, w.kvh, w.b, w.shared);
+          v[i] = p.spans[r.b * p.mask_sb + r.h * p.mask_sh + r.t * p.mask_st];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (cl.past && v[i].z < v[i].w) lo = min(lo, v[i].z), hi = max(hi, v[i].w);
+          if (!w.shared && v[i].x < v[i].y) lo = min(lo, np * AW_N + v[i].x), hi = max(hi, np * AW_N + v[i].y);
         }
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
@@ -259,8 +262,8 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
       }
       const int j_lo = pbeg < pend ? pbeg / AW_N : 0, j_hi = pbeg < pend ? (pend + AW_N - 1) / AW_N : 0;
       WideKeys k;
-      k.j0 = j_lo + (int)((long long)(j_hi - j_lo) * w.split / cl.splits);
-      k.J = j_lo + (int)((long long)(j_hi - j_lo) * (w.split + 1) / cl.splits) - k.j0;
+      k.j0 = j_lo + split_start(j_hi - j_lo, w.split, cl.splits);
+      k.J = j_lo + split_start(j_hi - j_lo, w.split + 1, cl.splits) - k.j0;
       k.keys = keys;
       k.last = pend - (k.j0 + k.J - 1) * AW_N;
       if (n >= 2 && !__all_sync(0xffffffffu, mbar_wait(&info_empty[n & 1], (uint32_t)((n >> 1) - 1) & 1u, err,
