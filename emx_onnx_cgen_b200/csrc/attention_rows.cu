@@ -77,8 +77,10 @@ template <int NS, int NT, int MASK>
 __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const __grid_constant__ RowsParams p) {
   constexpr int NC = 2 * NS;                      // 16-byte pieces of a key row per thread
   constexpr int ROW = 128 * NS;                   // bytes of a key row in the ring
-  constexpr int STAGE = 2 * AR_KB * ROW;          // K and V of a block
-  constexpr int ST = AR_RING / STAGE;             // 6 or 3 blocks
+  constexpr int U = NS == 1 && NT == 1 ? 2 : 1;   // blocks of a step
+  constexpr int BLOCK = 2 * AR_KB * ROW;          // K and V of a block
+  constexpr int STAGE = U * BLOCK;
+  constexpr int ST = AR_RING / STAGE;             // 3 steps, or 6 at NS = 1, NT = 2
   constexpr int OW = 64 * NS + 4;                 // padded row of the merge buffer
   extern __shared__ __align__(128) uint8_t s_all[];  // rows_smem() bytes
   __shared__ uint32_t s_bits[MASK == MASK_BITS ? 8 * NT * AF_ROWS_MASK_KEYS / 32 : 1];  // [row][32 keys]
@@ -123,18 +125,21 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   const uint16_t* kp = p.past_k + ph * p.D;
   const uint16_t* vp = p.past_v + ph * p.DV;
 
-  // ---------------- copies: this warp's n-th block is blk0 + warp + n * warps, in stage n % ST
+  // ---------------- copies: this warp's n-th step takes the U blocks from blk0 + U (warp + n warps), in stage n % ST
   const uint32_t ring = smem_u32(s_all) + warp * AR_RING;
   auto issue = [&](int blk, int stage) {
-    if (blk < blk1) {
+#pragma unroll
+    for (int u = 0; u < U; ++u, ++blk) {
+      if (blk >= blk1) break;
       const bool is_past = blk < pblocks;
       const int k0 = (is_past ? blk : blk - pblocks) * AR_KB, n = (is_past ? past : keys) - k0;
       const int ks = is_past ? p.D : (int)p.k_st, vs = is_past ? p.DV : (int)p.v_st;
       constexpr int PIECES = 8 * NS, STEP = 32 / PIECES;
       const int c = lane % PIECES, r0 = lane / PIECES;
-      const uint16_t* ksrc = (is_past ? kp : kc) + (int64_t)k0 * ks + 8 * c;
-      const uint16_t* vsrc = (is_past ? vp : vc) + (int64_t)k0 * vs + 8 * c;
-      const uint32_t dst = ring + stage * STAGE;
+      const uint16_t* ksrc = (is_past ? kp : kc) + (int64_t)(k0 + r0) * ks + 8 * c;
+      const uint16_t* vsrc = (is_past ? vp : vc) + (int64_t)(k0 + r0) * vs + 8 * c;
+      const int64_t k_step = (int64_t)STEP * ks, v_step = (int64_t)STEP * vs;
+      const uint32_t dst = ring + stage * STAGE + u * BLOCK;
       const bool k_in = 8 * c < p.D, v_in = 8 * c < p.DV;
 #pragma unroll
       for (int i = 0; i < AR_KB; i += STEP) {
@@ -142,14 +147,15 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
         const bool in = r < n;
         const uint32_t at = dst + r * ROW + rows_place(r, c) * 16;
         // rows past the keys and pieces past the head size are zero (what is not taken is not read either)
-        cp_async16_or_zero(at, in && k_in ? ksrc + (int64_t)r * ks : p.k, in && k_in);
-        cp_async16_or_zero(at + AR_KB * ROW, in && v_in ? vsrc + (int64_t)r * vs : p.v, in && v_in);
+        cp_async16_or_zero(at, in && k_in ? ksrc : p.k, in && k_in);
+        cp_async16_or_zero(at + AR_KB * ROW, in && v_in ? vsrc : p.v, in && v_in);
+        ksrc += k_step, vsrc += v_step;
       }
     }
     cp_async_commit();  // (an empty group keeps the count)
   };
 #pragma unroll 1  // (straight-line copies cost more in instruction fetches than they gain)
-  for (int n = 0; n < ST - 1; ++n) issue(blk0 + warp + n * warps, n);
+  for (int n = 0; n < ST - 1; ++n) issue(blk0 + U * (warp + n * warps), n);
 
   // ---------------- the rows whose scores this thread holds (2t, 2t + 1 of each tile): mask row and key limit
   int64_t mrow[NT][2];
@@ -230,22 +236,24 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
     first = lo_blk;
   }
 
-  // additive mask entries of a block at this thread's scores, loaded a block ahead
-  float mk[MASK == MASK_ADD ? 4 * NT : 1], mk_next[MASK == MASK_ADD ? 4 * NT : 1];
+  // additive mask entries of a step at this thread's scores, loaded a step ahead
+  float mk[U][MASK == MASK_ADD ? 4 * NT : 1], mk_next[U][MASK == MASK_ADD ? 4 * NT : 1];
   auto load_add = [&](int blk) {
-    if (MASK != MASK_ADD || blk >= blk1) return;
-    const bool is_past = blk < pblocks;
-    const int k0 = (is_past ? blk : blk - pblocks) * AR_KB, pos0 = (is_past ? 0 : p.tp) + k0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int pos = pos0 + 8 * h + g;
-      const bool in = k0 + 8 * h + g < (is_past ? past : keys);
+    for (int u = 0; u < (MASK == MASK_ADD ? U : 0); ++u, ++blk) {
+      const bool is_past = blk < pblocks;
+      const int k0 = (is_past ? blk : blk - pblocks) * AR_KB, pos0 = (is_past ? 0 : p.tp) + k0;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int h = 0; h < 2; ++h) {
+        const int pos = pos0 + 8 * h + g;
+        const bool in = blk < blk1 && k0 + 8 * h + g < (is_past ? past : keys);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          mk_next[(h * NT + n) * 2 + e] =
-              in && pos < p.mask_len ? additive_entry(p.mask_add, p.add_f32, mrow[n][e] + pos) : -INFINITY;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            mk_next[u][(h * NT + n) * 2 + e] =
+                in && pos < p.mask_len ? additive_entry(p.mask_add, p.add_f32, mrow[n][e] + pos) : -INFINITY;
+      }
     }
   };
 
@@ -268,86 +276,108 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   const uint32_t k_row = ring + g * ROW, v_row = ring + AR_KB * ROW + 2 * t * ROW;
   const int k_swz = rows_place(g, 0), v_swz0 = rows_place(2 * t, 0), v_swz1 = rows_place(2 * t + 1, 0);
 
-  load_add(blk0 + warp);
-  for (int n = 0, blk = blk0 + warp; blk < blk1; ++n, blk += warps) {
-    cp_async_wait_group<ST - 2>();  // this block's copies (one group a block) are done, for every lane
+  load_add(blk0 + U * warp);
+  for (int n = 0, blk = blk0 + U * warp; blk < blk1; ++n, blk += U * warps) {
+    cp_async_wait_group<ST - 2>();  // this step's copies (one group a step) are done, for every lane
     __syncwarp();
-    issue(blk + (ST - 1) * warps, (n + ST - 1) % ST);  // into the stage of the block before this one
+    issue(blk + (ST - 1) * U * warps, (n + ST - 1) % ST);  // into the stage of the step before this one
     if (MASK == MASK_ADD) {
 #pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) mk[i] = mk_next[i];
-      load_add(blk + warps);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4 * NT; ++i) mk[u][i] = mk_next[u][i];
+      load_add(blk + U * warps);
     }
-    if (MASK == MASK_BITS && blk < first) continue;
+    if (MASK == MASK_BITS && blk + U - 1 < first) continue;
     any_block = true;
     const uint32_t stage = (uint32_t)(n % ST) * STAGE;
-    // ---------------- which of this thread's scores count: [half][tile][row]
-    const bool is_past = blk < pblocks;
-    const int k0 = (is_past ? blk : blk - pblocks) * AR_KB, pos0 = (is_past ? 0 : p.tp) + k0;
-    const int seg_end = is_past ? past : p.tp + keys;
+    // ---------------- which of this thread's scores count: [block][half][tile][row]
     uint32_t see = ~0u;
-    if (MASK != MASK_NONE || pos0 + AR_KB > min(lim_all, seg_end)) {
-      see = 0;
-      const int bit = (blk - blk0) * AR_KB;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool is_past = blk + u < pblocks;
+      const int k0 = (is_past ? blk + u : blk + u - pblocks) * AR_KB, pos0 = (is_past ? 0 : p.tp) + k0;
+      const int seg_end = blk + u >= blk1 ? 0 : is_past ? past : p.tp + keys;
+      if (MASK == MASK_NONE && pos0 + AR_KB <= min(lim_all, seg_end)) continue;
+      const int bit = (blk + u - blk0) * AR_KB;
 #pragma unroll
       for (int n2 = 0; n2 < NT; ++n2)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint32_t bits = 0xffffu;
-          if (MASK == MASK_BITS)
+          if (MASK == MASK_BITS && blk + u < blk1)
             bits = s_bits[(one_row ? 0 : min(8 * n2 + 2 * t + e, rows - 1)) * (AF_ROWS_MASK_KEYS / 32) + (bit >> 5)] >> (bit & 31);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int pos = pos0 + 8 * h + g, i = (h * NT + n2) * 2 + e;
             bool ok = pos < min(lim[n2][e], seg_end) && ((bits >> (8 * h + g)) & 1u);
             if (MASK == MASK_ADD) {
-              ok = ok && mk[i] != -INFINITY;
-              if (!ok) mk[i] = 0.0f;
+              ok = ok && mk[u][i] != -INFINITY;
+              if (!ok) mk[u][i] = 0.0f;
             }
-            see |= (ok ? 1u : 0u) << i;
+            if (!ok) see &= ~(1u << (4 * NT * u + i));
           }
         }
     }
     // ---------------- S^T
-    uint4 k[2][NC];
+    uint4 k[U][2][NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const uint32_t at = k_row + stage + (((t + 4 * c) ^ k_swz) << 4);
-      k[0][c] = lds128(at);
-      k[1][c] = lds128(at + 8 * ROW);
-    }
-    float s[NT][4];
-#pragma unroll
-    for (int n2 = 0; n2 < NT; ++n2) {
-      float s2[4];  // two chains of products
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[n2][e] = s2[e] = 0.0f;
-      if (n2 == 1 && !two) continue;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        mma_16816(s[n2], k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, q[n2][c].x, q[n2][c].y);
-        mma_16816(s2, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, q[n2][c].z, q[n2][c].w);
+        const uint32_t at = k_row + stage + u * BLOCK + (((t + 4 * c) ^ k_swz) << 4);
+        k[u][0][c] = lds128(at);
+        k[u][1][c] = lds128(at + 8 * ROW);
       }
+    float s[U][NT][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n2][e] = (s[n2][e] + s2[e]) * sc;
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int n2 = 0; n2 < NT; ++n2) {
+        float s2[4];  // two chains of products
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][n2][e] = s2[e] = 0.0f;
+        if (n2 == 1 && !two) continue;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          mma_16816(s[u][n2], k[u][0][c].x, k[u][1][c].x, k[u][0][c].y, k[u][1][c].y, q[n2][c].x, q[n2][c].y);
+          mma_16816(s2, k[u][0][c].z, k[u][1][c].z, k[u][0][c].w, k[u][1][c].w, q[n2][c].z, q[n2][c].w);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][n2][e] = (s[u][n2][e] + s2[e]) * sc;
+      }
     // V in K's registers, on its way during the softmax
-    uint4 v[NS][4];
+    uint4 v[U][NS][4];
 #pragma unroll
-    for (int sl = 0; sl < NS; ++sl) {
-      const uint32_t at = v_row + stage;
-      v[sl][0] = lds128(at + (((8 * sl + g) ^ v_swz0) << 4));
-      v[sl][1] = lds128(at + ROW + (((8 * sl + g) ^ v_swz1) << 4));
-      v[sl][2] = lds128(at + 8 * ROW + (((8 * sl + g) ^ v_swz0) << 4));
-      v[sl][3] = lds128(at + 9 * ROW + (((8 * sl + g) ^ v_swz1) << 4));
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int sl = 0; sl < NS; ++sl) {
+        const uint32_t at = v_row + stage + u * BLOCK;
+        v[u][sl][0] = lds128(at + (((8 * sl + g) ^ v_swz0) << 4));
+        v[u][sl][1] = lds128(at + ROW + (((8 * sl + g) ^ v_swz1) << 4));
+        v[u][sl][2] = lds128(at + 8 * ROW + (((8 * sl + g) ^ v_swz0) << 4));
+        v[u][sl][3] = lds128(at + 9 * ROW + (((8 * sl + g) ^ v_swz1) << 4));
+      }
+    if (U == 2) {  // a block without a visible key beside one with some takes no part, whatever its values hold
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      if (MASK == MASK_BITS && blk < first) {
+#pragma unroll
+        for (int i = 0; i < 4 * NS; ++i) v[0][i >> 2][i & 3] = zero;
+      }
+      if (blk + 1 >= blk1) {
+#pragma unroll
+        for (int i = 0; i < 4 * NS; ++i) v[U - 1][i >> 2][i & 3] = zero;
+      }
     }
     // scores in log2 units; entries the row does not see are -inf
     if (see != ~0u) {
 #pragma unroll
-      for (int n2 = 0; n2 < NT; ++n2)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!((see >> (((e >> 1) * NT + n2) * 2 + (e & 1))) & 1u)) s[n2][e] = -INFINITY;
+        for (int n2 = 0; n2 < NT; ++n2)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!((see >> (4 * NT * u + ((e >> 1) * NT + n2) * 2 + (e & 1))) & 1u)) s[u][n2][e] = -INFINITY;
     }
     bool grow = false;
     float top[NT][2];
@@ -356,12 +386,16 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (n2 == 1 && !two) continue;
-        float x0 = s[n2][e], x1 = s[n2][2 + e];
-        if (MASK == MASK_ADD) {
-          x0 = fmaf(mk[n2 * 2 + e], AFK_LOG2E, x0);
-          x1 = fmaf(mk[(NT + n2) * 2 + e], AFK_LOG2E, x1);
+        float x = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float x0 = s[u][n2][e], x1 = s[u][n2][2 + e];
+          if (MASK == MASK_ADD) {
+            x0 = fmaf(mk[u][n2 * 2 + e], AFK_LOG2E, x0);
+            x1 = fmaf(mk[u][(NT + n2) * 2 + e], AFK_LOG2E, x1);
+          }
+          x = fmaxf(x, fmaxf(x0, x1));
         }
-        const float x = fmaxf(x0, x1);
         top[n2][e] = x;
         grow = grow || x > m_ref[n2][e] + AFK_RESCALE || (m_ref[n2][e] == -INFINITY && x > -INFINITY);
       }
@@ -390,37 +424,41 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
         }
     }
     // ---------------- weights, as the B operand of the second product
-    uint32_t pb[NT][2];
+    uint32_t pb[U][NT][2];
 #pragma unroll
-    for (int n2 = 0; n2 < NT; ++n2) {
-      if (n2 == 1 && !two) continue;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float neg = m_ref[n2][e] == -INFINITY ? 0.0f : -m_ref[n2][e];
+      for (int n2 = 0; n2 < NT; ++n2) {
+        if (n2 == 1 && !two) continue;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float off = neg;
-          if (MASK == MASK_ADD) off = fmaf(mk[(h * NT + n2) * 2 + e], AFK_LOG2E, neg);
-          s[n2][2 * h + e] = ex2_approx(s[n2][2 * h + e] + off);
-          l[n2][e] += s[n2][2 * h + e];
+        for (int e = 0; e < 2; ++e) {
+          const float neg = m_ref[n2][e] == -INFINITY ? 0.0f : -m_ref[n2][e];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float off = neg;
+            if (MASK == MASK_ADD) off = fmaf(mk[u][(h * NT + n2) * 2 + e], AFK_LOG2E, neg);
+            s[u][n2][2 * h + e] = ex2_approx(s[u][n2][2 * h + e] + off);
+            l[n2][e] += s[u][n2][2 * h + e];
+          }
         }
-      }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) pb[n2][h] = transpose_8x8(pack_f16x2(s[n2][2 * h], s[n2][2 * h + 1]));
-    }
+        for (int h = 0; h < 2; ++h) pb[u][n2][h] = transpose_8x8(pack_f16x2(s[u][n2][2 * h], s[u][n2][2 * h + 1]));
+      }
     // ---------------- O^T += V^T P^T
 #pragma unroll
-    for (int sl = 0; sl < NS; ++sl) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w0 = word_of(v[sl][0], j), w1 = word_of(v[sl][1], j);
-        const uint32_t w2 = word_of(v[sl][2], j), w3 = word_of(v[sl][3], j);
-        const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
-        const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
-        mma_16816(o[0][sl][j], a0, a1, a2, a3, pb[0][0], pb[0][1]);
-        if (NT == 2 && two) mma_16816(o[NT - 1][sl][j], a0, a1, a2, a3, pb[NT - 1][0], pb[NT - 1][1]);
+      for (int sl = 0; sl < NS; ++sl) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w0 = word_of(v[u][sl][0], j), w1 = word_of(v[u][sl][1], j);
+          const uint32_t w2 = word_of(v[u][sl][2], j), w3 = word_of(v[u][sl][3], j);
+          const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
+          const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
+          mma_16816(o[0][sl][j], a0, a1, a2, a3, pb[u][0][0], pb[u][0][1]);
+          if (NT == 2 && two) mma_16816(o[NT - 1][sl][j], a0, a1, a2, a3, pb[u][NT - 1][0], pb[u][NT - 1][1]);
+        }
       }
-    }
     __syncwarp();  // the stage's readers are done before its next copies
   }
   cp_async_wait_group<0>();
