@@ -542,8 +542,11 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 const F2 e = fma2(F2(__uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1])), mul2v, neg2);
-                // a quarter of the exponentials runs on the fp32 units, beside the exponential unit's
-                const F2 w2 = (i & 3) == 3 ? ex2_poly(e) : F2(ex2_approx(e.lo()), ex2_approx(e.hi()));
+                // At D > 64 an eighth of the exponentials runs on the fp32 units, beside the exponential unit's:
+                // [4, 32, 2048 x 4096, 128] takes 412 us so, 423 us with none and with a quarter.  At D <= 64 issue
+                // slots are what is short: [8, 16, 448 x 1500, 64] takes 50.6 us with none, 51.2 and 52.6 us with
+                // an eighth and a quarter.
+                const F2 w2 = NS == 2 && i % 8 == 7 ? ex2_poly(e) : F2(ex2_approx(e.lo()), ex2_approx(e.hi()));
                 sum[i & 1] = add2(sum[i & 1], w2);
                 pw[i] = pack_f16x2(w2.lo(), w2.hi());
               }
