@@ -868,7 +868,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
         if (std::max<int64_t>(n0 + n1, most_keys(r.tp, r.tk, 1)) * largest > 0xffffffffll) return 5;
       }
       r.by_hkv = SmallDiv::of(r.HKV);
-      r.late_wait = !together;
+      r.late_wait = !together && step == 1;
       e = launch_attention_rows(r, pass == AF_PASS_ROWS8 ? 1 : 2, variant, (int)op.ip[AF_WARPS], (unsigned)(n0 + n1), ctx.stream);
     } else {
       TileParams p{};

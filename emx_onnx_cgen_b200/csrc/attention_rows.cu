@@ -192,6 +192,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   // ---------------- boolean mask: bits of the item's keys, counted through its blocks; the blocks worth reading
   const bool one_row = p.mask_sh == 0 && p.mask_st == 0 && !past_item;  // every row of the tile has the same mask row
   int first = blk0;  // bits of block i start at bit (i - blk0) * AR_KB
+  int key_end = (blk1 - blk0) * AR_KB;  // end of the visible keys, counted the same way (the copies zero keys past `keys`)
   if (MASK == MASK_BITS) {
     if (threadIdx.x < 2) s_range[threadIdx.x] = threadIdx.x ? 0 : 0x7fffffff;
     __syncthreads();
@@ -234,6 +235,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
     // later copies stop at the last block with a visible key; the blocks before the first are passed over below
     blk1 = min(blk1, hi_blk);
     first = lo_blk;
+    key_end = s_range[1];
   }
 
   // additive mask entries of a step at this thread's scores, loaded a step ahead
@@ -358,16 +360,20 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
         v[u][sl][2] = lds128(at + 8 * ROW + (((8 * sl + g) ^ v_swz0) << 4));
         v[u][sl][3] = lds128(at + 9 * ROW + (((8 * sl + g) ^ v_swz1) << 4));
       }
-    if (U == 2) {  // a block without a visible key beside one with some takes no part, whatever its values hold
-      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-      if (MASK == MASK_BITS && blk < first) {
+    // keys behind the item's last visible one, and blocks before its first, take no part whatever their values hold
+    if ((blk + U - blk0) * AR_KB > key_end) {
 #pragma unroll
-        for (int i = 0; i < 4 * NS; ++i) v[0][i >> 2][i & 3] = zero;
-      }
-      if (blk + 1 >= blk1) {
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < 4 * NS; ++i) v[U - 1][i >> 2][i & 3] = zero;
-      }
+        for (int i = 0; i < 4; ++i)
+          if ((blk + u - blk0) * AR_KB + 2 * t + (i & 1) + 8 * (i >> 1) >= key_end) {
+#pragma unroll
+            for (int sl = 0; sl < NS; ++sl) v[u][sl][i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+    }
+    if (MASK == MASK_BITS && U == 2 && blk < first) {
+#pragma unroll
+      for (int i = 0; i < 4 * NS; ++i) v[0][i >> 2][i & 3] = make_uint4(0u, 0u, 0u, 0u);
     }
     // scores in log2 units; entries the row does not see are -inf
     if (see != ~0u) {

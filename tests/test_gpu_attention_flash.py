@@ -158,6 +158,102 @@ def test_padding_behind_a_boolean_mask(q_seq):
     check(run(wl, x), *want, str(kw))
 
 
+@pytest.mark.parametrize("q_seq,d", [(1, 64), (2, 128), (7, 64), (12, 64), (50, 64), (300, 64), (300, 128)])
+def test_padding_to_the_key_behind_a_boolean_mask(q_seq, d):
+    """What lies behind the last key that any row of a sequence sees reaches
+    nothing, from the very next key on, whichever pass runs."""
+    require_gpu()
+    kw = dict(batch=5, q_heads=2, kv_heads=2, q_seq=q_seq, kv_seq=300, mask="bool", head_dim=d)
+    wl = W.decoder_attention(**kw)
+    x = wl.make_inputs(21)
+    ends = [300, 77, 128, 1, 0]
+    x["mask"][:] = np.arange(300)[None, None, None, :] < np.array(ends)[:, None, None, None]
+    x["mask"][0, ..., :40] = False  # (keys before the first visible one stay finite)
+    want = decoder_attention(wl, x)
+    for b, n in enumerate(ends):
+        x["K"][b, :, n:] = np.nan
+        x["V"][b, :, n:] = np.nan
+    check(run(wl, x), *want, str(kw))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kw", [
+    dict(q_heads=6, kv_heads=2, q_seq=100, kv_seq=400, mask="bool", mask_shape="query"),      # three heads a group
+    dict(q_heads=6, kv_heads=2, q_seq=100, kv_seq=400, mask="bool", mask_shape="full", causal=True),
+    dict(q_heads=4, kv_heads=2, q_seq=200, kv_seq=130, mask="bool", mask_shape="seq", past=190),
+    dict(q_heads=4, kv_heads=2, q_seq=129, kv_seq=260, mask="bool", mask_shape="full", rank=3),
+    dict(q_heads=2, kv_heads=2, q_seq=300, kv_seq=700, count=True),
+    dict(q_heads=3, kv_heads=1, q_seq=43, kv_seq=257, count=True, rank=3),                     # 129 rows
+    dict(q_heads=2, kv_heads=1, q_seq=300, kv_seq=1, causal=True),
+    dict(q_heads=2, kv_heads=2, q_seq=257, kv_seq=385, scale=-0.3),
+])
+def test_two_row_tiles_an_item(kw, d):
+    """The 256-row pass: masks of every shape, counts with NaN behind them, groups that do not divide a tile."""
+    require_gpu()
+    b, t = 3, kw.get("past", 0) + kw["kv_seq"]
+    ms = {"seq": (b, 1, 1, t), "query": (b, 1, kw["q_seq"], t), "full": (b, kw["q_heads"], kw["q_seq"], t)}
+    kw = dict(kw, batch=b, head_dim=d)
+    if "mask_shape" in kw:
+        kw["mask_shape"] = ms[kw["mask_shape"]]
+    wl = W.decoder_attention(**kw)
+    x = wl.make_inputs(22)
+    if "mask" in kw:
+        x["mask"][1, :, -1] = False  # a row (or a sequence) without a key
+        x["mask"][2, ..., 140:] = False
+    if "count" in x:
+        x["count"][:] = [kw["kv_seq"], 0, 129]
+    want = decoder_attention(wl, x)
+    if "count" in x:
+        for i, n in enumerate(x["count"]):
+            if kw.get("rank") == 3:
+                x["K"][i, n:] = x["V"][i, n:] = np.nan
+            else:
+                x["K"][i, :, n:] = x["V"][i, :, n:] = np.nan
+    check(run(wl, x), *want, str(kw))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(batch=40, q_heads=4, kv_heads=1, q_seq=1, kv_seq=20, past=500, head_dim=128),                  # 160 rows
+    dict(batch=33, q_heads=8, kv_heads=2, q_seq=3, kv_seq=20, past=500, head_dim=64),                   # 12 a sequence
+    dict(batch=50, q_heads=3, kv_heads=1, q_seq=3, kv_seq=20, past=300, head_dim=128, rank=3),          # 9 a sequence
+    dict(batch=33, q_heads=4, kv_heads=1, q_seq=2, kv_seq=20, past=260, head_dim=64, mask="bool", mask_shape=(33, 4, 2, 280)),
+])
+def test_shared_past_in_the_256_row_pass(kw):
+    """The batch's rows packed in two row tiles against the one copy, own keys beside it."""
+    require_gpu()
+    wl = W.decoder_attention(**kw)
+    op = plan_for(wl, attention_mode="flash").ops[0]
+    assert op.ip[K.AF_PASS_PAST] == K.AF_PASS_WIDE
+    verify(kw)
+
+
+@pytest.mark.parametrize("q_seq,d", [(1, 64), (3, 128), (40, 64), (200, 64), (200, 128)])
+def test_infinite_and_nan_scores(q_seq, d):
+    """A visible NaN or infinite score makes its row NaN, as exp does, and no other row."""
+    require_gpu()
+    kw = dict(batch=2, q_heads=2, kv_heads=2, q_seq=q_seq, kv_seq=200, head_dim=d)
+    wl = W.decoder_attention(**kw)
+    x = wl.make_inputs(23)
+    want = decoder_attention(wl, x)
+    x["Q"][0, 1, q_seq // 2, 3] = np.nan
+    x["Q"][1, 0, 0] = 0  # only its first element meets the infinite key below
+    x["Q"][1, 0, 0, 0] = 1
+    x["K"][1, 0, 150, 0] = np.inf
+    got = run(wl, x)
+    assert np.isnan(got[0, 1, q_seq // 2]).all() and np.isnan(got[1, 0, 0]).all()
+    fine = np.ones(got.shape, bool)
+    fine[0, 1, q_seq // 2] = False
+    fine[1, 0] = False  # (every row of that head meets the infinity)
+    y, tol = want
+    check(got[fine], y[fine], tol[fine], str(kw))
+
+
+def test_boolean_mask_longer_than_an_item_holds():
+    """More keys than one few-row item keeps mask bits for: split, whatever the batch."""
+    require_gpu()
+    verify(dict(batch=160, q_heads=1, kv_heads=1, q_seq=1, kv_seq=4200, head_dim=8, mask="bool", mask_shape=(160, 1, 1, 4200)))
+
+
 def test_scores_of_hidden_keys_do_not_matter():
     """Infinite and NaN scores of keys that a row does not see leave it alone."""
     require_gpu()

@@ -35,6 +35,12 @@ pytestmark = pytest.mark.gpu
     dict(positions="rows", seq=21), dict(positions="rows", seq=5, head_dim=24, rotary_dim=8, dtype="f32"),
     dict(batch=7, seq=300, q_heads=32, kv_heads=8, head_dim=128),     # four rows per lane group
     dict(batch=5, seq=511, q_heads=12, kv_heads=5, head_dim=128, interleaved=True, dtype="f32"),
+    # lane groups that go around (norm_rope.cu): head counts off the four rows of a group, token counts off the grid
+    dict(batch=3, seq=1401, q_heads=30, kv_heads=7, head_dim=128),
+    dict(batch=3, seq=1401, q_heads=30, kv_heads=7, head_dim=128, rotary_dim=96, interleaved=True),
+    dict(batch=1, seq=3001, q_heads=21, kv_heads=5, head_dim=128, rotary_dim=64, interleaved=True, dtype="f32"),
+    dict(batch=2, seq=2003, q_heads=33, kv_heads=1, head_dim=72, rotary_dim=48, positions="rows", layout="heads"),
+    dict(batch=1, seq=5003, q_heads=31, kv_heads=30, head_dim=64, norm=False, dtype="f32", layout="flat"),
 ])
 def test_definition(kw):
     require_gpu()
@@ -95,6 +101,29 @@ def test_position_out_of_the_tables_is_reported():
                 sess.run(y)
         again = sess.run(x)  # the session stays usable
         assert all(np.array_equal(good[n], again[n]) for n in good)
+
+
+def test_position_out_of_the_tables_among_many_tokens():
+    """The rows of a bad position are NaN, every other row is as without it."""
+    require_gpu()
+    import torch
+    wl = W.norm_rope(batch=3, seq=1401, q_heads=30, kv_heads=7, head_dim=128)
+    x = wl.make_inputs(2)
+    plan = plan_for(wl)
+    sess = Session(plan)
+    want = sess.run(x)
+    x["pos"][2, 1400] = -5
+    x["pos"][0, 0] = wl.graph.initializers["cos"].shape[0]
+    dev = [torch.from_numpy(x[n]).cuda() for n in plan.input_names]
+    outs = [torch.zeros(s, dtype=torch.float16, device="cuda") for s in plan.output_shapes]
+    sess.run_ptrs([t.data_ptr() for t in dev], [o.data_ptr() for o in outs], stream=1)
+    with pytest.raises(EmxError, match="out of range"):
+        sess.sync()
+    for n, o in zip(plan.output_names, outs):
+        got, ref = o.cpu().numpy(), want[n].copy()
+        assert np.isnan(got[2, :, 1400]).all() and np.isnan(got[0, :, 0]).all()
+        got[2, :, 1400], got[0, :, 0] = ref[2, :, 1400], ref[0, :, 0]
+        assert np.array_equal(got, ref)
 
 
 def test_batch_slices():
