@@ -384,6 +384,34 @@ def test_two_sessions_on_two_streams():
         check(y.cpu().numpy(), *want, "")
 
 
+def test_captured_into_a_callers_graph():
+    """With its own graph replay off, a session's run can be part of a caller's
+    graph: replayed on other inputs, beside an eager run of another session."""
+    require_gpu()
+    import torch
+    for kw in (dict(batch=3, q_heads=8, kv_heads=2, q_seq=1, kv_seq=2000, past=3000, head_dim=128),
+               dict(batch=40, q_heads=8, kv_heads=2, q_seq=1, kv_seq=70, past=900, head_dim=128, mask="bool"),
+               dict(batch=2, q_heads=4, kv_heads=2, q_seq=100, kv_seq=77, mask="f16", mask_shape=(2, 1, 100, 77))):
+        wl = W.decoder_attention(**kw)
+        plan = plan_for(wl, attention_mode="flash")
+        sess, other = Session(plan), Session(plan)
+        sess.set_graphs(False)
+        x = [wl.make_inputs(s) for s in (1, 2)]
+        dev = [torch.from_numpy(x[0][n]).cuda() for n in plan.input_names]
+        y = torch.zeros(plan.output_shapes[0], dtype=torch.float16, device="cuda")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            sess.run_ptrs([t.data_ptr() for t in dev], [y.data_ptr()], stream=torch.cuda.current_stream().cuda_stream)
+        for v in (1, 0):
+            for t, n in zip(dev, plan.input_names):
+                t.copy_(torch.from_numpy(x[v][n]))
+            graph.replay()
+            check(other.run(x[1 - v])["Y"], *decoder_attention(wl, x[1 - v]), "beside the replay")
+            torch.cuda.synchronize()
+            check(y.cpu().numpy(), *decoder_attention(wl, x[v]), str(kw))
+
+
 def test_misaligned_buffers_are_refused():
     require_gpu()
     import torch
