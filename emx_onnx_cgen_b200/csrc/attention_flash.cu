@@ -62,33 +62,25 @@ constexpr uint32_t AFK_KSLAB = AFK_N * 128u;  // 64 fp16 columns of a K or V til
 constexpr uint32_t AFK_TMEM_COLS = 256;       // scores at columns 0 and 64, output at 128
 constexpr uint32_t AFK_O_COL = 128;
 
-// Eight entries of an additive mask; `see`: which of them may be read (the others are 0).
-__device__ __forceinline__ void additive8(const TileParams& p, int64_t at, uint32_t see, float (&mk)[8]) {
-  if (p.add_vec && (p.add_padded || see == 0xffu)) {
-    if (p.add_f32) {
-      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.add) + at);
-      const float4 a = __ldg(src), b = __ldg(src + 1);
-      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// Eight entries of an additive mask from 16 bytes of fp16, or 32 of fp32.
+__device__ __forceinline__ void mask_entries(const uint4& v, float (&mk)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mk[e] = additive_bounded(v[e]);
-    } else {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.add) + at));
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-        mk[2 * e] = f.x;
-        mk[2 * e + 1] = f.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mk[e] = (see >> e) & 1u ? additive_entry(p.add, p.add_f32, at + e) : 0.0f;
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+    mk[2 * e] = f.x;
+    mk[2 * e + 1] = f.y;
   }
+}
+__device__ __forceinline__ void mask_entries(const uint4& a, const uint4& b, float (&mk)[8]) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) mk[e] = __uint_as_float(w[e]);
 }
 
 template <int NS, int MASK>
 __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const __grid_constant__ TileParams p) {
+  constexpr bool ADD = MASK == MASK_ADD || MASK == MASK_ADD32;
   constexpr uint32_t QTILE = NS * AFK_QSLAB, KTILE = NS * AFK_KSLAB;
   constexpr int ST = NS == 1 ? 4 : 2;  // K and V stages: 64 KB of loads in flight per CTA at either head size
   extern __shared__ __align__(1024) uint8_t afk_raw[];
@@ -328,6 +320,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
     const bool pos = sc > 0.0f;
     const unsigned long long* words = MASK == MASK_BITS ? p.bits + mrow * p.words + (cl.past ? 0 : p.words_past) + j0 : nullptr;
     unsigned long long word = MASK == MASK_BITS && J > 0 ? words[0] : 0ull;  // the next tile's, loaded a tile ahead
+    const uint4* entries = p.add;  // this row's piece 0 of the tile
+    if (ADD) entries += mrow + (int64_t)((cl.past ? 0 : p.words_past) + j0) * (MASK == MASK_ADD ? 8 : 16) * p.mask_rows;
     bool ok = true;
     for (int j = 0; j < J && ok; ++j) {
       const int sb = j & 1, jj = j0 + j;
@@ -341,11 +335,16 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         vis &= word;
         if (j + 1 < J) word = words[j + 1];
       }
-      const int mask_at = (in_past ? 0 : p.tp) + key0;  // the tile's first key in a mask row
-      if (MASK == MASK_ADD && !p.add_padded) {  // keys past a short mask are not seen (padded: -inf)
-        const int left = p.mask_len - mask_at;
-        if (left < AFK_N) vis &= left > 0 ? (1ull << left) - 1 : 0ull;
+      // the tile's mask entries: fp16, held from here on; fp32, loaded where they are used (twice the registers)
+      uint4 raw[MASK == MASK_ADD ? 8 : 1];
+      if (MASK == MASK_ADD) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = __ldg(entries + i * p.mask_rows);
       }
+      auto load_entries = [&](int i, float (&mk)[8]) {  // of keys 8i .. 8i + 7
+        if (MASK == MASK_ADD) mask_entries(raw[i], mk);
+        else mask_entries(__ldg(entries + 2 * i * p.mask_rows), __ldg(entries + (2 * i + 1) * p.mask_rows), mk);
+      };
       ok = mbar_wait(&s_full[sb], (uint32_t)(j >> 1) & 1u, err, DEV_TIMEOUT_EPILOGUE);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -377,17 +376,15 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         }
       }
       float mx;
-      if (MASK == MASK_ADD) {
+      if (ADD) {
         // pass 1: -inf mask entries hide their key; the maximum of the masked scores (any value near it will do)
-        const int64_t at = mrow * p.add_pitch + (p.add_padded ? ((cl.past ? 0 : p.words_past) + jj) * AFK_N : mask_at);
         mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float mk[8];
-            additive8(p, at + 32 * c + i, (half >> i) & 0xffu, mk);
+            load_entries(4 * c + i / 8, mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               if (mk[e] == -INFINITY) sv[c][i + e] = 0xff800000u;
@@ -413,20 +410,18 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
       uint32_t pw[2][16];
       float lp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (MASK == MASK_ADD) {
-        const int64_t at = mrow * p.add_pitch + (p.add_padded ? ((cl.past ? 0 : p.words_past) + jj) * AFK_N : mask_at);
+      if (ADD) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float mk[8];
-            additive8(p, at + 32 * c + i, (half >> i) & 0xffu, mk);
+            load_entries(4 * c + i / 8, mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              // a hidden key's score is -inf; its mask entry must not turn that into NaN
-              const float mm = mk[e] == -INFINITY ? neg_m : fmaf(mk[e], AFK_LOG2E, neg_m);
-              sv[c][i + e] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(sv[c][i + e]), mul, mm)));
+              // (a hidden key's score is -inf, and so is the sum whatever finite or -inf entry it has)
+              sv[c][i + e] = __float_as_uint(
+                  ex2_approx(fmaf(__uint_as_float(sv[c][i + e]), mul, fmaf(mk[e], AFK_LOG2E, neg_m))));
             }
 #pragma unroll
             for (int e = 0; e < 8; e += 2)
@@ -479,6 +474,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         *reinterpret_cast<uint4*>(s_p + r * 128 + ((g ^ (r & 7)) << 4)) =
             make_uint4(pw[c][i], pw[c][i + 1], pw[c][i + 2], pw[c][i + 3]);
       }
+      if (ADD) entries += (MASK == MASK_ADD ? 8 : 16) * p.mask_rows;
       fence_async_shared();  // the generic writes of P become visible to the tensor cores
       tc_fence_before();
       __syncwarp();
@@ -652,19 +648,39 @@ __global__ void __launch_bounds__(256) mask_pack_kernel(const uint8_t* __restric
 }
 
 // ------------------------------------------------------------------ whole tiles of additive masks
-// y[row][tile][64]: the past's tiles, then the current keys', -inf past the mask's length and each part's keys.
+// y[tile][16-byte piece][row]: the past's tiles, then the current keys', -inf past the mask's length and each part's
+// keys, finite fp32 entries within their bound.  A row's thread reads its row of a tile 16 bytes at a time: straight
+// from the mask, 32 rows' pieces are 32 sectors of 32 rows ([57, 16, 45 x 2952, 96] with a mask row per query took
+// 810 us so); from here they are 512 bytes in line.  A CTA copies 32 rows of a tile through shared memory.
 template <typename T>
-__global__ void __launch_bounds__(256) mask_pad_kernel(const T* __restrict__ mask, int len, int past, int keys, int words1,
-                                                       int words, T* __restrict__ y) {
+__global__ void __launch_bounds__(256) mask_tiles_kernel(const T* __restrict__ mask, int len, int past, int keys, int words1,
+                                                         int words, int64_t rows, uint4* __restrict__ y) {
+  constexpr int E = 16 / sizeof(T), PIECES = 64 / E;
+  __shared__ uint4 s_tile[32][PIECES + 1];  // (the padding spreads a piece's rows over the banks)
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t row = blockIdx.x;
-  const T* src = mask + row * len;
-  T* dst = y + row * words * 64;
-  const T low = (T)-INFINITY;
-  for (int i = threadIdx.x; i < words * 64; i += 256) {
-    const int seg = i < words1 * 64 ? 1 : 0, k = seg ? i : i - words1 * 64, at = seg ? k : past + k;
-    dst[i] = k < (seg ? past : keys) && at < len ? src[at] : low;
+  const int64_t row0 = (int64_t)blockIdx.x * 32;
+  const int here = (int)min((int64_t)32, rows - row0);
+  for (int w = blockIdx.y; w < words; w += gridDim.y) {
+    const bool in_past = w < words1;
+    const int k0 = (in_past ? w : w - words1) * 64, at = (in_past ? 0 : past) + k0;
+    const int n = min((in_past ? past : keys) - k0, len - at);  // entries of the tile that exist
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int x = threadIdx.x + 256 * i, r = x >> 6, k = x & 63;
+      T v = (T)-INFINITY;
+      if (r < here && k < n) {
+        v = mask[(row0 + r) * len + at + k];
+        if (sizeof(T) == 4) v = (T)additive_bounded((float)v);
+      }
+      reinterpret_cast<T*>(s_tile[r])[k] = v;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < 32 * PIECES; x += 256) {
+      const int r = x & 31, piece = x >> 5;
+      if (r < here) y[((int64_t)w * PIECES + piece) * rows + row0 + r] = s_tile[r][piece];
+    }
+    __syncthreads();
   }
 }
 
@@ -677,9 +693,11 @@ static size_t flash_smem(int ns) {
 typedef void (*FlashKernel)(const TileParams);
 
 static FlashKernel flash_kernel(int ns, int mask) {
-  static const FlashKernel table[2][3] = {
-      {attention_flash_kernel<1, MASK_NONE>, attention_flash_kernel<1, MASK_BITS>, attention_flash_kernel<1, MASK_ADD>},
-      {attention_flash_kernel<2, MASK_NONE>, attention_flash_kernel<2, MASK_BITS>, attention_flash_kernel<2, MASK_ADD>}};
+  static const FlashKernel table[2][4] = {
+      {attention_flash_kernel<1, MASK_NONE>, attention_flash_kernel<1, MASK_BITS>, attention_flash_kernel<1, MASK_ADD>,
+       attention_flash_kernel<1, MASK_ADD32>},
+      {attention_flash_kernel<2, MASK_NONE>, attention_flash_kernel<2, MASK_BITS>, attention_flash_kernel<2, MASK_ADD>,
+       attention_flash_kernel<2, MASK_ADD32>}};
   return table[ns - 1][mask];
 }
 
@@ -699,7 +717,7 @@ int prepare_attention_flash(const PlanOp& op, void* const*, OpState*, int, char*
   for (int s = AF_Q_SB; s <= AF_O_ST; ++s)
     if (op.ip[s] % 8) return fail(msg, n, 5, "Attention: strides must be 16-byte multiples");
   for (int ns = 1; ns <= 2; ++ns)
-    for (int m = 0; m < 3; ++m) {
+    for (int m = 0; m < 4; ++m) {
       cudaError_t e =
           cudaFuncSetAttribute(flash_kernel(ns, m), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)flash_smem(ns));
       if (e != cudaSuccess) return fail(msg, n, 4, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
@@ -749,10 +767,7 @@ static int tile_params(TileParams& p, const RowsParams& r, const ItemClass* cls,
   p.causal = r.causal, p.tk = r.tk, p.tp = r.tp, p.past_shared = r.past_shared;
   p.counts = r.counts;
   p.mask_sb = r.mask_sb, p.mask_sh = r.mask_sh, p.mask_st = r.mask_st;
-  p.add = r.mask_add, p.add_f32 = r.add_f32, p.mask_len = r.mask_len;
-  p.add_pitch = p.mask_len;
-  const int entries = p.add_f32 ? 4 : 8;  // of 16 bytes: every row and both parts of the keys start on 16 bytes
-  p.add_vec = p.add && p.mask_len % entries == 0 && p.tp % entries == 0 && ((uintptr_t)p.add & 15u) == 0;
+  p.mask_len = r.mask_len;
   p.scale_log2 = r.scale_log2;
   p.err = r.err;
   const int64_t tq = r.TQ.d;
@@ -887,22 +902,22 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
                        (int)(p.mask_len % 16 == 0 && p.tp % 16 == 0 && ((uintptr_t)r.mask_bool & 15u) == 0),
                        (unsigned long long*)p.bits, (int4*)p.spans);
         ++*launches;
-      } else if (variant == MASK_ADD && op.ip[AF_MASK_PADDED]) {
-        if (p.add_f32)
-          e = launch_pdl(mask_pad_kernel<float>, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, (const float*)p.add,
-                         p.mask_len, p.tp, p.tk, p.words_past, p.words, (float*)ptr(9));
+      } else if (variant == MASK_ADD) {
+        p.add = (const uint4*)ptr(9);
+        p.mask_rows = mrows;
+        const dim3 grid((unsigned)((mrows + 31) / 32), (unsigned)std::min(p.words, 65535));
+        if (r.add_f32)
+          e = launch_pdl(mask_tiles_kernel<float>, grid, dim3(256), 0, ctx.stream, (const float*)r.mask_add, p.mask_len, p.tp,
+                         p.tk, p.words_past, p.words, mrows, (uint4*)ptr(9));
         else
-          e = launch_pdl(mask_pad_kernel<__half>, dim3((unsigned)mrows), dim3(256), 0, ctx.stream, (const __half*)p.add,
-                         p.mask_len, p.tp, p.tk, p.words_past, p.words, (__half*)ptr(9));
+          e = launch_pdl(mask_tiles_kernel<__half>, grid, dim3(256), 0, ctx.stream, (const __half*)r.mask_add, p.mask_len,
+                         p.tp, p.tk, p.words_past, p.words, mrows, (uint4*)ptr(9));
         ++*launches;
-        p.add = ptr(9);
-        p.add_pitch = (int64_t)p.words * 64;
-        p.add_vec = p.add_padded = 1;
       }
       if (e != cudaSuccess) return 4;
       const int ns = flash_slabs(op);
       e = pass == AF_PASS_WIDE ? launch_attention_wide(p, ns, variant, ctx.num_sms, ctx.stream)
-                               : launch_pdl(flash_kernel(ns, variant), dim3((unsigned)(n0 + n1)), dim3(AFK_THREADS),
+                               : launch_pdl(flash_kernel(ns, r.add_f32 ? MASK_ADD32 : variant), dim3((unsigned)(n0 + n1)), dim3(AFK_THREADS),
                                             flash_smem(ns), ctx.stream, p);
     }
     ++*launches;

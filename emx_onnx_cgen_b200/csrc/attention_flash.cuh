@@ -11,7 +11,7 @@ namespace emx {
 constexpr float AFK_RESCALE = 8.0f;  // the output is rescaled when a row's maximum grows by more (log2 units)
 constexpr float AFK_LOG2E = 1.4426950408889634f;
 
-enum { MASK_NONE = 0, MASK_BITS = 1, MASK_ADD = 2 };  // kernel variants
+enum { MASK_NONE = 0, MASK_BITS = 1, MASK_ADD = 2, MASK_ADD32 = 3 /*fp32 entries; attention_flash.cu only*/ };  // kernel variants
 
 struct RowId {
   int b, h, t;
@@ -86,11 +86,11 @@ struct TileParams {
   int64_t mask_sb, mask_sh, mask_st;  // mask row of (b, h, t): b * sb + h * sh + t * st
   const unsigned long long* bits;     // packed boolean mask [row][words], the past's words first
   const int4* spans;                  // per mask row: first and end visible current key, first and end visible past key
-  // additive mask [row][add_pitch]: as given, or, padded, every 64-key tile of the past and of the current keys whole
-  // (-inf past the mask) and in the tiles' order; add_vec: groups of 8 entries start on 16 bytes
-  const void* add;
-  int64_t add_pitch;
-  int words, words_past, mask_len, add_f32, add_vec, add_padded;
+  // additive mask in whole 64-key tiles, the past's first, -inf past the mask's length and past each part's keys:
+  // [tile][16-byte piece of its keys][mask row], so that neighbouring rows' loads of a piece are neighbours
+  const uint4* add;
+  int64_t mask_rows;
+  int words, words_past, mask_len;
   float scale_log2;
   int* err;
 };

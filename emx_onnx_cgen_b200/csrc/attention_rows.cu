@@ -190,13 +190,22 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   }
 
   // ---------------- boolean mask: bits of the item's keys, counted through its blocks; the blocks worth reading
-  const bool one_row = p.mask_sh == 0 && p.mask_st == 0 && !past_item;  // every row of the tile has the same mask row
+  // Rows with one mask row share its bits: all rows of a sequence's item where neither heads nor tokens have their
+  // own, a token's group of heads where heads have not, else none.
+  const bool one_row = p.mask_sh == 0 && p.mask_st == 0 && !past_item;
+  const int token0 = p.group.div(row0);
+  auto bits_of = [&](int r) { return one_row ? 0 : p.mask_sh == 0 ? p.group.div(row0 + r) - token0 : r; };
+  const uint32_t* bit_row[NT][2];  // this thread's rows
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) bit_row[n][e] = s_bits + bits_of(min(8 * n + 2 * t + e, rows - 1)) * (AF_ROWS_MASK_KEYS / 32);
   int first = blk0;  // bits of block i start at bit (i - blk0) * AR_KB
   int key_end = (blk1 - blk0) * AR_KB;  // end of the visible keys, counted the same way (the copies zero keys past `keys`)
   if (MASK == MASK_BITS) {
     if (threadIdx.x < 2) s_range[threadIdx.x] = threadIdx.x ? 0 : 0x7fffffff;
     __syncthreads();
-    const int words = ((blk1 - blk0) * AR_KB + 31) / 32, mask_rows = one_row ? 1 : rows;
+    const int words = ((blk1 - blk0) * AR_KB + 31) / 32, mask_rows = bits_of(rows - 1) + 1;
     int lo = 0x7fffffff, hi = 0;
     // a warp takes 256 keys of a row at a time, eight loads in flight
     constexpr int LOADS = 8;
@@ -204,7 +213,9 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
 #pragma unroll 1
     for (int i = warp; i < groups * mask_rows; i += warps) {
       const int r = i / groups, w4 = (i - r * groups) * LOADS;
-      const RowId w = row_of(row0 + r, p.group, p.TQ, kvh, b, past_item);
+      // (a row with these bits: the first of the token's, if the tile has it)
+      const int row = one_row || p.mask_sh != 0 ? row0 + r : max(row0, (token0 + r) * (int)p.group.d);
+      const RowId w = row_of(row, p.group, p.TQ, kvh, b, past_item);
       const uint8_t* src = p.mask_bool + (w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st) * (int64_t)p.mask_len;
       uint8_t v[LOADS];
 #pragma unroll
@@ -308,7 +319,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
         for (int e = 0; e < 2; ++e) {
           uint32_t bits = 0xffffu;
           if (MASK == MASK_BITS && blk + u < blk1)
-            bits = s_bits[(one_row ? 0 : min(8 * n2 + 2 * t + e, rows - 1)) * (AF_ROWS_MASK_KEYS / 32) + (bit >> 5)] >> (bit & 31);
+            bits = bit_row[n2][e][bit >> 5] >> (bit & 31);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int pos = pos0 + 8 * h + g, i = (h * NT + n2) * 2 + e;

@@ -14,7 +14,10 @@
 // spread over LPR lanes, each holding the two 16-byte pieces that pair up, so
 // a rotation needs no exchange and the row sum log2(LPR) shuffles; a lane
 // group takes HPG head rows of its token and loads the token's table entries
-// once for them.
+// once for them.  8 x 4096 tokens of 32 + 8 fp16 heads of 128 (671 MB moved)
+// take 134 us, 5.0 TB/s; back to back 125 us, and as long with the arithmetic
+// taken out.  4 x 2048 tokens: 37 us.  One token of 32 sequences: 8.6 us, of
+// which 7 are the host's call.
 //
 // K_RMS_NORM: rows of any length, a warp per row up to 1024 elements, else a
 // CTA per row; the second pass over the row hits L1 / L2.
@@ -254,9 +257,9 @@ __global__ void __launch_bounds__(256, RING ? 2 : 3) norm_rope_kernel(const __gr
         ff[e / 2] = mul2(wf, c2), fs[e / 2] = mul2(ws, m2), sf[e / 2] = mul2(wf, s2), ss[e / 2] = mul2(ws, c2);
       }
     }
-    if (RING) {
-      cp_async_wait_group<RING ? RING - 2 : 0>();  // own copies of this group
-      fetch(gi + (RING - 1) * stride, (slot + RING - 1) % (RING ? RING : 1));
+    if constexpr (RING > 0) {
+      cp_async_wait_group<RING - 2>();  // own copies of this group
+      fetch(gi + (RING - 1) * stride, (slot + RING - 1) % RING);
     }
     T* y = static_cast<T*>(it.y) + w.b * it.y_sb + w.t * it.y_st + w.j * it.y_sh;
     const int64_t hop = step * it.y_sh;
@@ -376,9 +379,11 @@ static cudaError_t launch_vec_rows(RopeParams p, int num_sms, cudaStream_t strea
 
 template <typename T, int LPR>
 static cudaError_t launch_vec(const RopeParams& p, const LaunchCtx& ctx) {
-  // Four rows per lane group, in lane groups that stay, once there is work for each to go around more than once;
-  // before that, one row each at once.
-  return p.tokens * p.heads * LPR >= (int64_t)ctx.num_sms * 2048 * 4
+  // One row per lane group at once, or, for more, four rows per group in lane groups that stay: 1024 / 3000 / 8192
+  // tokens of 40 fp16 heads of 128 take 13.4 / 21.4 / 41.0 us so and 14.3 / 28.6 / 63.5 us with a row each, 512 tokens
+  // 10.2 us both, 256 tokens 10.2 and 8.2 us.  An fp32 lane has half the pairs, whose matrices are what the four rows
+  // share: 2048 / 4096 / 8192 tokens of 16 fp32 heads of 80 take 16.4 / 22.5 / 32.8 us and 15.2 / 22.5 / 38.9 us.
+  return p.tokens * p.heads * LPR > (int64_t)ctx.num_sms * (sizeof(T) == 2 ? 1536 : 6144)
              ? launch_vec_rows<T, LPR, 4, NR_RING>(p, ctx.num_sms, ctx.stream)
              : launch_vec_rows<T, LPR, 1, 0>(p, ctx.num_sms, ctx.stream);
 }

@@ -304,6 +304,8 @@ def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, 
     # key ranges that the few-row pass needs at least: it keeps a range's boolean mask on chip
     at_least = lambda n: tiles(n * 16, K.AF_ROWS_MASK_KEYS) if mask == "bool" else 1
     sms = K.LP_PLAN_SMS
+    # the few-row pass holds 16 rows at most; up to there it is as fast as the tile pass or faster (8 sequences x 4
+    # heads x 16 rows, 1500 keys: 14.3 against 16.4 us at D = 64, 12 rows 18.4 us both at D = 128)
     few = rows <= 16
 
     def tile_pass(parts, share=1.0):
@@ -321,25 +323,33 @@ def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, 
     keys = tk if apart else tp + tk
     if few:
         packed = b * rows
-        # A work item of eight warps fills an SM; with an item for every SM, two of four warps share one instead.
+        # A work item of eight warps fills an SM; with an item for every SM, two of four warps share one instead
+        # (160 items of 1500 keys, D = 64: 18.4 against 20.5 us; 144 items: 18.4 against 16.4 us).
         warps = lambda items: 4 if items >= sms else 8
         own = K.AF_PASS_ROWS8 if rows <= 8 else K.AF_PASS_ROWS16
         if not apart:
             so = max(flash_splits([(b * hkv, tiles(keys, 64))], sms, 8)[0], at_least(blocks(tp, tk)))
             return FlashSchedule(own, K.AF_PASS_NONE, so, 0, warps(b * hkv * so))
-        if packed <= (64 if head <= 64 else 32):
-            # Up to four row tiles read the past's keys from L2 once each, which costs less than a tile pass takes to
-            # set up (7 sequences x 9 rows, 1001 keys, D = 64: 14.4 against 16.4 us; 16 x 4, 2048 keys, D = 128: 18.5
-            # against 16.4 us).
+        if packed <= (96 if head <= 64 else 64) and packed * tp * (1 if head <= 64 else 2) <= 1 << 19:
+            # A few row tiles read the past's keys from L2 once each, which costs less than a tile pass takes to set up:
+            # 7 sequences x 9 rows, 1001 keys, D = 64: 12.3 against 15.3 us; 20 x 4, 4096 keys, D = 64: 16.4 against
+            # 18.5; 16 x 4, 2048 keys, D = 128: 18.4 against 20.5; but 8192 keys: 30.7 against 26.6, and 32 x 4 rows,
+            # 2048 keys: 28.7 against 22.6.
             own = K.AF_PASS_ROWS8 if packed <= 8 else K.AF_PASS_ROWS16
             items = hkv * tiles(packed, 8 if packed <= 8 else 16)
-            sp = max(flash_splits([(items, tiles(tp, 64))], sms, 4)[0], at_least(blocks(tp)))
-            return FlashSchedule(own, own, max(1, at_least(blocks(tk))), sp, 8)
+            # items of four warps, two an SM, once there are some to begin with; of eight, one an SM, before (16 items:
+            # 8 x 4 rows, 8192 keys, D = 128: 22.5 us with 8 ranges of eight warps, 24.5 us with 8 of four)
+            w, places, least = (4, 2 * sms, 4) if items >= 24 else (8, sms, 5)
+            # ranges of `least` key tiles, and never more items than places (32 items, 8192 keys: 30.7 us
+            # with 9 ranges, 42.0 us with 10)
+            sp = max(1, min(tiles(tiles(tp, 64), least), places // items), at_least(blocks(tp)))
+            return FlashSchedule(own, own, max(1, at_least(blocks(tk))), sp, w)
         so = max(flash_splits([(b * hkv, tiles(keys, 64))], 2 * sms, 8)[0], at_least(blocks(tk)))
         # the sequences' own keys run beside the past on the SMs it leaves: 3/5 of them give the shortest whole
-        # (128 sequences, 8192 + 256 keys: 68 us with 5 key ranges, 83 us with 9)
+        # (128 sequences, 8192 + 256 keys: 57 us with 5 key ranges, 64 us with 7, 70 us with 9)
         past, sp = tile_pass([(packed, hkv, tp)], 0.6)
-        return FlashSchedule(own, past, so, sp[0], 4)
+        # (64 rows, 8192 keys: 26.6 us with 16 ranges, 31.7 us with 32: the merge reads them all)
+        return FlashSchedule(own, past, so, min(sp[0], 16), 4)
     own, splits = tile_pass([(rows, b * hkv, keys)] + ([(b * rows, hkv, tp)] if apart else []))
     return FlashSchedule(own, own if apart else K.AF_PASS_NONE, splits[0], splits[1] if apart else 0)
 
@@ -1602,9 +1612,7 @@ class B200PlanEmitter:
             if kind == K.AF_MASK_BOOL:
                 words = 2 * (-(-tp // (2 * FLASH_KEYS)) + -(-tk // (2 * FLASH_KEYS)))
                 t_bits = self._b.arena_tensor(T_TEMP, "u8", (mb * mh * mt, 16 + 8 * words), name="attention:mask-bits")
-            elif ms[-1] % 8 or tp % 8:
-                # rows or the two parts of the keys start off 16 bytes: a copy in whole tiles, read 16 bytes at a time
-                ip[K.AF_MASK_PADDED] = 1
+            else:
                 words = -(-tp // FLASH_KEYS) + -(-tk // FLASH_KEYS)
                 t_bits = self._b.arena_tensor(T_TEMP, self._dtype(op.input_attn_mask), (mb * mh * mt, 64 * words),
                                               name="attention:mask-tiles")

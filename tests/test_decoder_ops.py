@@ -219,7 +219,10 @@ def test_schedules():
     assert pick(4, 2, 4, 10, 500, False) == (rows8, none)       # a past of its own is part of the row's keys
     assert pick(8, 8, 4, 33, 2048, True) == (rows16, rows16)    # 32 packed rows
     assert pick(16, 8, 4, 33, 2048, True, "", 64) == (rows16, rows16)
-    assert pick(16, 8, 4, 33, 2048, True) == (rows8, tiles)
+    assert pick(16, 8, 4, 33, 2048, True) == (rows16, rows16)
+    assert pick(17, 8, 4, 33, 2048, True) == (rows8, tiles)
+    assert pick(16, 8, 4, 33, 4097, True) == (rows8, tiles)
+    assert pick(25, 8, 4, 33, 2048, True, "", 64) == (rows8, tiles)
     assert pick(2, 8, 4, 33, 2048, True) == (rows8, rows8)
     assert pick(33, 8, 4, 33, 2048, True) == (rows8, wide)
     assert pick(33, 8, 4, 33, 2048, True, "f16") == (rows8, tiles)  # additive masks: no wide form
