@@ -6,7 +6,13 @@
 // 4 flops a byte and row at most.  Each warp copies its 16-key blocks of K and V
 // into a ring of its own in shared memory (cp.async, 24 KB a warp), two to five
 // blocks ahead of the one it works on: with the blocks in registers, one ahead,
-// a block cost a memory latency (1.2 us).  The products are mma.sync.m16n8k16:
+// a block cost a memory latency (1.2 us).  At D <= 64 and up to 8 rows a step
+// takes two blocks: the chain of a step (scores, maximum, exponentials,
+// transposes, output) is 1500 clocks long and two warps a scheduler do not cover
+// it (16 sequences x 16 heads, up to 1500 keys, D = 64: 16.5 us, 4.5 TB/s of
+// valid keys; 20.5 us with one block).  128 sequences x 8 heads of 4 rows, 150
+// keys on average, D = 128: 29 us alone, 3.5 TB/s, a third of the stalls at the
+// CTA's barriers.  The products are mma.sync.m16n8k16:
 // a tcgen05 form needs a 128-row tile, tensor maps, barriers and TMEM set up per
 // work item, and at these sizes a work item is over before that has paid off.
 // Both products run transposed,
@@ -27,8 +33,9 @@
 // shared by the batch, two kinds of items: rows of several sequences against
 // the past, each sequence's rows against its own keys.  The item's part of a
 // boolean mask is first turned into bits in shared memory, beside the first
-// blocks' copies; blocks before its first and after its last visible key are
-// not read.
+// blocks' copies, once for the rows that share a mask row; blocks after its last
+// visible key are not read (but for the first copies, which are on their way by
+// then), and values behind that key take no part.
 #include <cuda_fp16.h>
 
 #include "attention_flash.cuh"

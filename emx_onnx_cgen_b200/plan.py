@@ -340,9 +340,12 @@ def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, 
             # items of four warps, two an SM, once there are some to begin with; of eight, one an SM, before (16 items:
             # 8 x 4 rows, 8192 keys, D = 128: 22.5 us with 8 ranges of eight warps, 24.5 us with 8 of four)
             w, places, least = (4, 2 * sms, 4) if items >= 24 else (8, sms, 5)
-            # ranges of `least` key tiles, and never more items than places (32 items, 8192 keys: 30.7 us
-            # with 9 ranges, 42.0 us with 10)
-            sp = max(1, min(tiles(tiles(tp, 64), least), places // items), at_least(blocks(tp)))
+            # ranges of `least` key tiles, but no more items than places (32 items, 8192 keys: 30.7 us with 9 ranges,
+            # 42.0 us with 10), where a sequence's own item takes a place for its share of a range's time, either
+            # counted with four tiles of set-up (16 x 4 rows, 2048 + 33 keys: 18.4 us with 6 ranges, 20.5 with 8)
+            t, mine = tiles(tp, 64), b * hkv * (tiles(tk, 64) + 4)
+            sp = next((n for n in range(tiles(t, least), 1, -1) if items * n + mine / (t / n + 4) <= places), 1)
+            sp = max(sp, at_least(blocks(tp)))
             return FlashSchedule(own, own, max(1, at_least(blocks(tk))), sp, w)
         so = max(flash_splits([(b * hkv, tiles(keys, 64))], 2 * sms, 8)[0], at_least(blocks(tk)))
         # the sequences' own keys run beside the past on the SMs it leaves: 3/5 of them give the shortest whole

@@ -91,7 +91,8 @@ int emx_b200_run(emx_plan_t *plan, const void *const *inputs, void *const *outpu
                  int64_t batch_begin, int64_t batch_count, void *stream);
 
 /* Wait for the plan's last run; reports device-side timeouts
- * (EMX_ERR_DEVICE_TIMEOUT) and asynchronous CUDA errors. */
+ * (EMX_ERR_DEVICE_TIMEOUT), position ids or valid key counts out of range
+ * (EMX_ERR_INVALID_ARGUMENT) and asynchronous CUDA errors. */
 int emx_b200_sync(emx_plan_t *plan);
 
 /* Release device memory and the handle (NULL is accepted). */

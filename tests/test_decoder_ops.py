@@ -326,3 +326,20 @@ def test_reference_rotation_against_angles():
                 z = (x[0, t, 0, a] + 1j * x[0, t, 0, b]) * np.exp(1j * ang[0, t, i])
                 assert np.allclose([y[0, t, 0, a], y[0, t, 0, b]], [z.real, z.imag])
         assert np.array_equal(y[..., 4:], x[..., 4:])
+
+
+def test_one_expand_for_two_attentions():
+    """Both read the one copy in place; with another reader as well, the Expand runs and both still read the one copy."""
+    wl = W.decoder_attention(batch=3, past=40, kv_seq=9, q_seq=2)
+    g = wl.graph
+    first = next(n for n in g.nodes if n.op_type == "Attention")
+    g.nodes.append(NodeSpec("Attention", "again", ("Y", *first.inputs[1:]), ("Z",), first.attrs))
+    g.outputs.append(TensorSpec("Z", "f16", g.tensor("Y").shape))
+    plan = plan_of(wl)
+    assert [o.kernel for o in plan.ops] == [K.K_ATTENTION_FLASH] * 2
+    assert all(o.ip[K.AF_PAST_SHARED] == 1 for o in plan.ops)
+    assert plan.ops[0].tensors[5:7] == plan.ops[1].tensors[5:7]
+    g.outputs.append(TensorSpec("PKx", "f16", g.tensor("PKx").shape))
+    plan = plan_of(wl)
+    assert sorted(o.kernel for o in plan.ops) == sorted([K.K_TRANSPOSE] + [K.K_ATTENTION_FLASH] * 2)
+    assert all(o.ip[K.AF_PAST_SHARED] == 1 for o in plan.ops if o.kernel == K.K_ATTENTION_FLASH)

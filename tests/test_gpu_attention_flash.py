@@ -346,6 +346,29 @@ def test_batch_slices():
         assert np.array_equal(part[1:3], whole[1:3]) and not part[0].any() and not part[3].any()
 
 
+@pytest.mark.parametrize("overlap", [False, True])
+def test_page_locked_host_buffers(overlap):
+    """Runs on page-locked host memory, sliced along the batch or overlapping one another, give the device run's bits."""
+    require_gpu()
+    import torch
+    wl = W.decoder_attention(batch=6, q_heads=8, kv_heads=4, q_seq=40, kv_seq=700, mask="bool", mask_shape=(6, 1, 40, 700),
+                             head_dim=64)
+    plan = plan_for(wl, attention_mode="flash")
+    sess = Session(plan)
+    sess.set_host_io_overlap(overlap)
+    jobs = []
+    for seed in (1, 2, 3):
+        x = wl.make_inputs(seed)
+        host = [torch.from_numpy(x[n]).pin_memory() for n in plan.input_names]
+        jobs.append((x, host, torch.zeros(plan.output_shapes[0], dtype=torch.float16).pin_memory()))
+    for _, host, y in jobs:
+        sess.run_ptrs([t.data_ptr() for t in host], [y.data_ptr()])
+    sess.sync()
+    for x, _, y in jobs:
+        check(y.numpy(), *decoder_attention(wl, x), "page-locked")
+        assert np.array_equal(y.numpy().view(np.uint16), Session(plan).run(x)["Y"].view(np.uint16))
+
+
 def test_repeated_and_uncaptured_runs_identical():
     """Merging split key ranges has a fixed order; a replayed graph and direct launches agree."""
     require_gpu()
