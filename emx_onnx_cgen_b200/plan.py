@@ -308,14 +308,20 @@ def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, 
     # heads x 16 rows, 1500 keys: 14.3 against 16.4 us at D = 64, 12 rows 18.4 us both at D = 128)
     few = rows <= 16
 
-    def tile_pass(parts, share=1.0):
+    def tile_pass(parts, share=1.0, merged=False):
         """Pass and splits for [(rows, heads, keys)]: two row tiles a work item
         where all rows fill more than one (attention_wide.cu has no additive
-        masks), one item per SM then, else one tile and two items."""
+        masks), one item per SM then, else one tile and two items.  ``merged``:
+        results are merged whatever the splits."""
         wide = not additive and all(n > FLASH_ROWS for n, _, _ in parts)
-        m, per_sm, least = (2 * FLASH_ROWS, share, 8) if wide else (FLASH_ROWS, 2, 1 if additive else 4)
-        return (K.AF_PASS_WIDE if wide else K.AF_PASS_TILES,
-                flash_splits([(h * tiles(n, m), tiles(t, FLASH_KEYS)) for n, h, t in parts], int(per_sm * sms), least))
+        m, per_sm, least = (2 * FLASH_ROWS, share, 4) if wide else (FLASH_ROWS, 2, 1 if additive else 4)
+        n = flash_splits([(h * tiles(n, m), tiles(t, FLASH_KEYS)) for n, h, t in parts], int(per_sm * sms), least)
+        if wide and not merged:
+            # the merge costs what eight key tiles do (8 heads x 300 rows, D = 128: 512 keys 18.4 us whole, 20.5 us in
+            # two; 768 keys 22.5 us whole, 20.5 us in three)
+            t = tiles(parts[0][2], FLASH_KEYS)
+            n = [n[0] if t - tiles(t, n[0]) >= 8 else 1]
+        return K.AF_PASS_WIDE if wide else K.AF_PASS_TILES, n
 
     # A sequence with at least a tile of rows reads a shared past for itself: packing other sequences' rows beside
     # them would save no read of it, and cost the merge.
@@ -350,10 +356,10 @@ def flash_schedule(b: int, hkv: int, rows: int, tk: int, tp: int, shared: bool, 
         so = max(flash_splits([(b * hkv, tiles(keys, 64))], 2 * sms, 8)[0], at_least(blocks(tk)))
         # the sequences' own keys run beside the past on the SMs it leaves: 3/5 of them give the shortest whole
         # (128 sequences, 8192 + 256 keys: 57 us with 5 key ranges, 64 us with 7, 70 us with 9)
-        past, sp = tile_pass([(packed, hkv, tp)], 0.6)
+        past, sp = tile_pass([(packed, hkv, tp)], 0.6, True)
         # (64 rows, 8192 keys: 26.6 us with 16 ranges, 31.7 us with 32: the merge reads them all)
         return FlashSchedule(own, past, so, min(sp[0], 16), 4)
-    own, splits = tile_pass([(rows, b * hkv, keys)] + ([(b * rows, hkv, tp)] if apart else []))
+    own, splits = tile_pass([(rows, b * hkv, keys)] + ([(b * rows, hkv, tp)] if apart else []), merged=apart)
     return FlashSchedule(own, own if apart else K.AF_PASS_NONE, splits[0], splits[1] if apart else 0)
 
 
