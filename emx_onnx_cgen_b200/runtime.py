@@ -114,13 +114,20 @@ class Session:
             _check(self.lib.emx_b200_plan_load_mem(self._blob, len(plan.plan_bytes), wbuf,
                                                    len(plan.weight_bytes), device, ctypes.byref(handle)))
         self.handle = handle
+        self._ins = (ctypes.c_void_p * len(plan.input_names))()
+        self._outs = (ctypes.c_void_p * len(plan.output_names))()
+        self._run = self.lib.emx_b200_run
 
     # -- raw pointer interface (host or device pointers)
     def run_ptrs(self, in_ptrs, out_ptrs, batch_begin: int = 0, batch_count: int = -1, stream: int = 0) -> None:
-        ins = (ctypes.c_void_p * max(1, len(in_ptrs)))(*in_ptrs)
-        outs = (ctypes.c_void_p * max(1, len(out_ptrs)))(*out_ptrs)
-        _check(self.lib.emx_b200_run(self.handle, ins, outs, batch_begin, batch_count,
-                                     ctypes.c_void_p(stream) if stream else None))
+        # the session's own arrays, written whole each call (making new ones took a microsecond of it)
+        ins, outs = self._ins, self._outs
+        if len(in_ptrs) < len(ins) or len(out_ptrs) < len(outs):
+            raise ValueError(f"{len(in_ptrs)} input and {len(out_ptrs)} output pointers, plan has {len(ins)} and {len(outs)}")
+        ins[:], outs[:] = in_ptrs[:len(ins)], out_ptrs[:len(outs)]
+        status = self._run(self.handle, ins, outs, batch_begin, batch_count, stream or None)
+        if status != EMX_OK:
+            _check(status)
 
     def sync(self) -> None:
         _check(self.lib.emx_b200_sync(self.handle))

@@ -162,3 +162,25 @@ def test_misaligned_device_buffers():
         o = o.cpu().numpy()
         assert o[0] == 7 and o[-1] == 7
         check(o[1:-1].reshape(s), *want[n], n)
+
+
+def test_pointers_are_taken_anew_each_call():
+    """Too few are refused, whatever the call before passed; extra ones are ignored."""
+    require_gpu()
+    import torch
+    wl = W.norm_rope(batch=2, seq=5)
+    plan = plan_for(wl)
+    sess = Session(plan)
+    x = [wl.make_inputs(s) for s in (1, 2)]
+    dev = [[torch.from_numpy(v[n]).cuda() for n in plan.input_names] for v in x]
+    outs = [[torch.zeros(s, dtype=torch.float16, device="cuda") for s in plan.output_shapes] for _ in x]
+    ptrs = lambda ts: [t.data_ptr() for t in ts]
+    for d, o in zip(dev, outs):
+        sess.run_ptrs(ptrs(d), ptrs(o) + [1], stream=1)
+        for i, j in ((1, 0), (0, 1)):
+            with pytest.raises(ValueError, match="pointers"):
+                sess.run_ptrs(ptrs(d)[i:], tuple(ptrs(o))[j:])
+    sess.sync()
+    for v, o in zip(x, outs):
+        for n, (y, tol) in norm_rope(wl, v).items():
+            check(o[plan.output_names.index(n)].cpu().numpy(), y, tol, n)
