@@ -394,6 +394,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
             load_entries(4 * c + i / 8, mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+              if (MASK == MASK_ADD32 && fabsf(mk[e]) >= AFK_ALONE && sv[c][i + e] != 0xff800000u)
+                sv[c][i + e] = 0u;  // (fp16 entries are not as large; a hidden key's score stays -inf)
               if (mk[e] == -INFINITY) sv[c][i + e] = 0xff800000u;
               else mx = fmaxf(mx, fmaf(__uint_as_float(sv[c][i + e]), mul, mk[e] * AFK_LOG2E));
             }

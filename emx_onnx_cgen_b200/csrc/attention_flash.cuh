@@ -41,9 +41,12 @@ __device__ __forceinline__ RowId row_of(int r, const SmallDiv& group, const Smal
 }
 
 // Finite fp32 entries beyond 2^24 count as 2^24: no score reaches across that, and the differences formed from
-// them stay finite.  -inf (and NaN) stay.
+// them stay finite.  From 2^56 on they count as 2^25 and stand alone: beside them a sum, in 64 bits too, has none of
+// its score's digits left, so keys at the type's lowest value weigh the same among themselves.  Infinities and NaN stay.
+constexpr float AFK_ALONE = 0x1p25f;
 __device__ __forceinline__ float additive_bounded(float v) {
-  return v > 0x1p24f ? 0x1p24f : (v < -0x1p24f && v > -INFINITY ? -0x1p24f : v);
+  const float a = fabsf(v);
+  return a > 0x1p24f && a < INFINITY ? copysignf(a >= 0x1p56f ? AFK_ALONE : 0x1p24f, v) : v;
 }
 
 __device__ __forceinline__ float additive_entry(const void* mask, int f32, int64_t at) {

@@ -364,7 +364,10 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
           mma_16816(s2, k[u][0][c].z, k[u][1][c].z, k[u][0][c].w, k[u][1][c].w, q[n2][c].z, q[n2][c].w);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[u][n2][e] = (s[u][n2][e] + s2[e]) * sc;
+        for (int e = 0; e < 4; ++e) {
+          s[u][n2][e] = (s[u][n2][e] + s2[e]) * sc;
+          if (MASK == MASK_ADD && fabsf(mk[u][((e >> 1) * NT + n2) * 2 + (e & 1)]) >= AFK_ALONE) s[u][n2][e] = 0.0f;
+        }
       }
     // V in K's registers, on its way during the softmax
     uint4 v[U][NS][4];

@@ -94,8 +94,9 @@ def test_rows_that_see_nothing(mask, kv_seq, q_seq):
 @pytest.mark.parametrize("heads", [2, 40])
 @pytest.mark.parametrize("mask", ["f16", "f32"])
 def test_lowest_value_masks(mask, heads):
-    """Padding at the type's lowest value; a row of nothing else is a softmax of
-    its scores, with all their digits."""
+    """Padding at the type's lowest value.  A row of nothing else is a softmax of
+    its scores, with all their digits, at fp16's lowest value; at fp32's the sum
+    has none of them left, in 64 bits too, and its keys weigh the same."""
     require_gpu()
     # 20 queries of two heads to a key/value head, or eight of one
     kw = dict(batch=2, q_heads=heads, kv_heads=heads // 2 if heads == 2 else heads, q_seq=20 if heads == 2 else 8, kv_seq=200,
@@ -111,9 +112,15 @@ def test_lowest_value_masks(mask, heads):
     if mask == "f32":  # the fp32 type's own lowest value
         x["mask"][:, :, :, 120:] = np.finfo(np.float32).min
         x["mask"][1, 0, 4, 130:] = 0
-        want = decoder_attention(wl, dict(x, mask=np.where(np.arange(kw["q_seq"])[:, None] == 7, 0, x["mask"]).astype(np.float32)))
-        x["mask"][:, 0, 7, :] = np.finfo(np.float32).min  # one constant over a whole row changes nothing
-        check(run(wl, x), *want, str(kw))
+        x["mask"][:, 0, 7, :] = np.finfo(np.float32).min
+        x["mask"][0, 0, 6, :] = -1e9  # beside this the scores keep enough digits
+        x["mask"][0, 0, 5, :] = -1e9
+        x["mask"][0, 0, 5, 9:] = np.finfo(np.float32).min
+        x["mask"][1, 0, 6, :] = np.finfo(np.float32).max
+        x["mask"][1, 0, 5, :] = -3e38
+        got, (want, tol) = run(wl, x), decoder_attention(wl, x)
+        check(got, want, tol, str(kw))
+        assert np.abs(want[0, 0, 7] - x["V"][0, 0].astype(np.float64).mean(0)).max() < 1e-12
 
 
 @pytest.mark.parametrize("q_seq,d", [(9, 64), (1, 128), (5, 64)])
