@@ -39,7 +39,7 @@
 // What bounds it: at two CTAs an SM the softmax warps' issue slots (64 scores a
 // row and tile in registers, an exponential each), then, for short keys, the
 // set-up of a work item (TMEM, barriers, Q: some 5 us).  [57, 16, 45 x 2952, 96]
-// with an additive mask: 217 us, 215 TFLOP/s; [3, 12, 77 x 333, 80]: 18.4 us,
+// with an additive mask: 217 us, 215 TFLOP/s; [3, 12, 77 x 333, 80]: 18 us,
 // three launches.
 //
 // Boolean masks are first packed by mask_pack_kernel to one 64-bit word per
