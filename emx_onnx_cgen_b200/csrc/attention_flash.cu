@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
     if (p.causal) keys = min(keys, p.group.div(row0 + rows - 1) + 1);
     if (p.counts) {
       const long long n = p.counts[b];
-      if (n < 0 || n > p.tk) record_error(err, DEV_BAD_INDEX);
+      if (n < 0 || n > p.tk) record_bad_index(err);
       keys = min(keys, (int)max(0ll, min(n, (long long)p.tk)));
     }
   }

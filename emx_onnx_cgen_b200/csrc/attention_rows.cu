@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
     if (p.causal) keys = min(keys, p.group.div(row0 + rows - 1) + 1);
     if (p.counts) {
       const long long n = p.counts[b];
-      if ((n < 0 || n > p.tk) && threadIdx.x == 0) record_error(p.err, DEV_BAD_INDEX);
+      if ((n < 0 || n > p.tk) && threadIdx.x == 0) record_bad_index(p.err);
       keys = min(keys, (int)max(0ll, min(n, (long long)p.tk)));
     }
   }

@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
         if (p.causal) keys = min(keys, p.group.div(w.row0 + w.rows - 1) + 1);
         if (p.counts) {
           const long long c = p.counts[w.b];
-          if (c < 0 || c > p.tk) record_error(err, DEV_BAD_INDEX);
+          if (c < 0 || c > p.tk) record_bad_index(err);
           keys = min(keys, (int)max(0ll, min(c, (long long)p.tk)));
         }
       }

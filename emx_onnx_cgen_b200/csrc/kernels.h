@@ -228,9 +228,6 @@ inline int64_t eff_batch(const LaunchCtx& c, const PlanOp& op, int64_t compiled)
   return (c.batch > 0 && op.ip[IP_BATCHED]) ? c.batch : compiled;
 }
 
-// tc100.cuh's DEV_BAD_INDEX, for the host: reported as EMX_ERR_INVALID_ARGUMENT.
-constexpr int DEV_BAD_INDEX_CODE = 6;
-
 // Launch with programmatic stream serialisation allowed (see pdl_wait() in
 // tc100.cuh): every kernel of the library goes through this helper and waits
 // on its predecessor inside the kernel.

@@ -98,7 +98,7 @@ __device__ __forceinline__ int64_t table_row(const RopeParams& p, int64_t token)
   if (!p.positions) return token;
   const long long at = p.pos[token];
   if (at >= 0 && at < p.positions) return at;
-  record_error(p.err, DEV_BAD_INDEX);
+  record_bad_index(p.err);
   return -1;
 }
 

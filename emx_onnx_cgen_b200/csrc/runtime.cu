@@ -768,14 +768,15 @@ int emx_b200_sync(emx_plan_t* p) {
     ++p->profiled_runs;
     p->events_pending = false;
   }
-  int err = 0;
-  CUDA_TRY(cudaMemcpy(&err, p->d_error, sizeof(int), cudaMemcpyDeviceToHost), "error word read");
-  if (err) {
-    cudaMemset(p->d_error, 0, sizeof(int));
-    if (err == emx::DEV_BAD_INDEX_CODE)
-      return set_error(EMX_ERR_INVALID_ARGUMENT, "an input of position ids or valid key counts holds a value out of range");
-    return set_error(EMX_ERR_DEVICE_TIMEOUT, "device-side wait gave up (code %d)", err);
-  }
+  // the error word, and 16 bytes after it the word of record_bad_index (tc100.cuh)
+  int words[5] = {0, 0, 0, 0, 0};
+  CUDA_TRY(cudaMemcpy(words, p->d_error, sizeof(words), cudaMemcpyDeviceToHost), "error word read");
+  const int err = words[0], bad_index = words[4];
+  if (err) cudaMemset(p->d_error, 0, sizeof(int));
+  if (bad_index) cudaMemset(p->d_error + 4, 0, sizeof(int));
+  if (err) return set_error(EMX_ERR_DEVICE_TIMEOUT, "device-side wait gave up (code %d)", err);
+  if (bad_index)
+    return set_error(EMX_ERR_INVALID_ARGUMENT, "an input of position ids or valid key counts holds a value out of range");
   return EMX_OK;
 }
 

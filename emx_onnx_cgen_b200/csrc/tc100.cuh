@@ -18,7 +18,6 @@ enum DeviceError : int {
   DEV_TIMEOUT_EPILOGUE = 3,
   DEV_TIMEOUT_GRID = 4,
   DEV_BAD_CONFIG = 5,
-  DEV_BAD_INDEX = 6,  // an input tensor of positions or counts holds a value out of range
 };
 
 // Bounded waits: give up after this many nanoseconds of %globaltimer.  The
@@ -46,6 +45,12 @@ __device__ __forceinline__ void record_error(int* err, int code) {
 
 __device__ __forceinline__ bool error_raised(const int* err) {
   return err && *reinterpret_cast<const volatile int*>(err) != 0;
+}
+
+// An input of positions or counts holds a value out of range.  The kernel carries on (with a clamped count, or NaN
+// rows), so this is a word of its own, 16 bytes after the error word: waits give up when that one is raised.
+__device__ __forceinline__ void record_bad_index(int* err) {
+  if (err) *reinterpret_cast<volatile int*>(err + 4) = 1;
 }
 
 // Wait budget of the plan owning `err` (read when a wait starts spinning, not
