@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         const int in_past = jj < np ? 1 : 0, key0 = (in_past ? jj : jj - np) * AFK_N;
         const int kb = in_past && p.past_shared ? 0 : b;
         const uint32_t ph = (uint32_t)(j / ST - 1) & 1u;
-        if (j >= ST && !mbar_wait(&k_empty[s], ph, err, DEV_TIMEOUT_PRODUCER)) ok = false;
+        if (p.drop_keys && j > 0) ok = false;
+        if (ok && j >= ST && !mbar_wait(&k_empty[s], ph, err, DEV_TIMEOUT_PRODUCER)) ok = false;
         if (!ok) break;
         mbar_arrive_expect_tx(&k_full[s], KTILE);
 #pragma unroll
@@ -899,6 +900,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
       const int tile_keys = pass == AF_PASS_WIDE ? 128 : AFK_N;
       if (pass == AF_PASS_WIDE && variant == MASK_ADD) return 5;  // (never planned)
       int rc = tile_params(p, r, cls, (int)n1, (int)(n0 + n1), tile_keys);
+      p.drop_keys = (ctx.fault & FAULT_DROP_KEY_TILES) != 0;
       if (rc) return rc;
       const int64_t mrows = p.mask_sb ? p.mask_sb * p.B : op.ip[AF_MASK_ROWS];
       p.words_past = (p.tp + tile_keys - 1) / tile_keys * (tile_keys / 64);

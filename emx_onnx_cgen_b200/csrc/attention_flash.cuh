@@ -95,6 +95,7 @@ struct TileParams {
   int64_t mask_rows;
   int words, words_past, mask_len;
   float scale_log2;
+  int drop_keys;  // failure-detection test hook (FAULT_DROP_KEY_TILES)
   int* err;
 };
 

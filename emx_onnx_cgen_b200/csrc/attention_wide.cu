@@ -231,6 +231,11 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
     return true;
   };
 
+  // On the way out of a loader of query rows: its last copies (those before them have been read) have landed.
+  auto q_landed = [&](int x, int loads) {
+    if (loads > 0) (void)mbar_wait(&q_full[x], (uint32_t)(loads - 1) & 1u, nullptr, 0);
+  };
+
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AW_REGS_OTHER));
   if (warp == 11) {
@@ -281,8 +286,12 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
         mbar_arrive(&info_full[n & 1]);
       }
       __syncwarp();
-      if (k.J > 0 && w.rows > AW_M && !load_q(w, 1, nq++)) break;
+      if (k.J > 0 && w.rows > AW_M) {
+        if (!load_q(w, 1, nq)) break;
+        ++nq;
+      }
     }
+    q_landed(1, nq);
   } else if (warp == 8) {
     // ---------------- producer (lane 0 issues)
     int nkv = 0, issued = 0;  // key tiles so far; copies so far (K and V of a tile count one each)
@@ -301,7 +310,8 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
           const int in_past = jj < np ? 1 : 0, key0 = (in_past ? jj : jj - np) * AW_N;
           const int kb = in_past && p.past_shared ? 0 : w.b;
           const uint32_t ph = (uint32_t)(nkv / ST - 1) & 1u;
-          if (nkv >= ST && !mbar_wait(&k_empty[s], ph, err, DEV_TIMEOUT_PRODUCER)) ok = false;
+          if (p.drop_keys && nkv > 0) ok = false;
+          if (ok && nkv >= ST && !mbar_wait(&k_empty[s], ph, err, DEV_TIMEOUT_PRODUCER)) ok = false;
           if (!ok) break;
           mbar_arrive_expect_tx(&k_full[s], TILE);
 #pragma unroll
@@ -415,7 +425,10 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
     for (int n = 0, id = blockIdx.x; id < p.items; ++n, id += gridDim.x) {
       WideKeys k;
       if (!item_keys(n, k)) break;
-      if (k.J > 0 && !load_q(wide_item(p, id), 0, nq++)) break;
+      if (k.J > 0) {
+        if (!load_q(wide_item(p, id), 0, nq)) break;
+        ++nq;
+      }
       nkv += k.J;
       if (k.J == 0 || k.last >= AW_N) continue;
       const int s = (nkv - 1) % ST;
@@ -431,6 +444,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
       if (lane == 0) mbar_arrive(v_clean);
       ++nclean;
     }
+    q_landed(0, nq);
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AW_REGS_SOFTMAX));

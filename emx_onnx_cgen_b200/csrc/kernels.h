@@ -214,6 +214,7 @@ struct LaunchCtx {
 // device wait run out; none faults, traps or hangs the GPU.
 enum FaultHook : int {
   FAULT_DROP_CHAIN_PROGRESS = 1,  // chained convolutions never publish their progress words
+  FAULT_DROP_KEY_TILES = 2,       // attention_flash.cu, attention_wide.cu: a CTA's producer stops after its first key tile
 };
 
 // Last integer slot of every op: 1 when the op's leading (batch) extent

@@ -817,7 +817,7 @@ int emx_b200_set_wait_budget(emx_plan_t* p, uint64_t ns) {
 
 int emx_b200_set_fault(emx_plan_t* p, int hooks) {
   if (!p) return set_error(EMX_ERR_INVALID_ARGUMENT, "plan is NULL");
-  if (hooks & ~emx::FAULT_DROP_CHAIN_PROGRESS) return set_error(EMX_ERR_INVALID_ARGUMENT, "unknown hook bits %d", hooks);
+  if (hooks & ~(emx::FAULT_DROP_CHAIN_PROGRESS | emx::FAULT_DROP_KEY_TILES)) return set_error(EMX_ERR_INVALID_ARGUMENT, "unknown hook bits %d", hooks);
   if (hooks == p->fault) return EMX_OK;
   CUDA_TRY(cudaSetDevice(p->device), "cudaSetDevice");
   CUDA_TRY(cudaDeviceSynchronize(), "device synchronize");

@@ -29,6 +29,7 @@ EXPORTED = ("emx_b200_version", "emx_b200_last_error", "emx_b200_plan_load", "em
             "emx_b200_set_wait_budget", "emx_b200_set_fault")
 
 FAULT_DROP_CHAIN_PROGRESS = 1
+FAULT_DROP_KEY_TILES = 2
 
 
 class EmxError(RuntimeError):

@@ -164,10 +164,13 @@ int emx_b200_set_wait_budget(emx_plan_t *plan, uint64_t ns);
  * EMX_FAULT_DROP_CHAIN_PROGRESS: chained convolutions never publish their
  * per-tile progress words, so the next layer's bounded waits run out and the
  * run ends with EMX_ERR_DEVICE_TIMEOUT -- a flag that nothing sets; nothing
- * faults, traps or hangs.  Changing the hooks drops the plan's captured
+ * faults, traps or hangs.  EMX_FAULT_DROP_KEY_TILES: the tile passes of
+ * flash-mode Attention load one tile of keys a thread block and no more, with
+ * the same effect on the waits for the others.  Changing the hooks drops the plan's captured
  * graphs.  No counterpart in the reference (its failure paths are host-side:
  * a NULL malloc, c_emitter.py:2785-2788). */
 #define EMX_FAULT_DROP_CHAIN_PROGRESS 1
+#define EMX_FAULT_DROP_KEY_TILES 2
 int emx_b200_set_fault(emx_plan_t *plan, int hooks);
 
 /* Allocation-free standalone QLinearConv, 3x3 kernel, stride 1, pads 1,
