@@ -102,10 +102,24 @@ __device__ __forceinline__ int64_t table_row(const RopeParams& p, int64_t token)
   return -1;
 }
 
-// 1 / sqrt(v) to fp32 accuracy: the hardware estimate and one Newton step.
+// 1 / sqrt(v), 0 of an infinite v: rsqrtf (2 steps of fp32 at most) for fp16 results, one Newton step more for fp32's.
+template <typename T>
 __device__ __forceinline__ float inv_sqrt(float v) {
   const float y = rsqrtf(v);
-  return fmaf(y * 0.5f, fmaf(-v * y, y, 1.0f), y);
+  return sizeof(T) == 2 || v == INFINITY ? y : fmaf(y * 0.5f, fmaf(-v * y, y, 1.0f), y);
+}
+
+// A row's norm factor 1 / sqrt(mean(x^2) + eps) is taken in two parts, x * pre * inv, where the squares leave fp32's
+// range: above it, v = mean + eps is infinite (or NaN); below it, squares under 2^-126 lose their digits, which counts
+// where v < 2^-90.  The row's squares are then summed again with pre = 2^-96 or 2^96, a power of two:
+//   inv = 1 / sqrt(mean((pre x)^2) + pre^2 eps),
+// all of it in range, and what underflows now is below the sum's last digit.  An infinite element keeps inv at 0, so
+// the row's finite elements are 0 and it is NaN, as in x / sqrt(inf).  (fp16 rows: 2^-48 / N <= mean < 2^33, or infinite
+// with an infinite element: nothing to sum again.)
+__device__ __forceinline__ bool squares_in_range(float v) { return v >= 0x1p-90f && v < INFINITY; }
+__device__ __forceinline__ float norm_pre(float v) { return v < 1.0f ? 0x1p96f : 0x1p-96f; }
+__device__ __forceinline__ float norm_inv_pre(float mean, float eps, float pre) {
+  return inv_sqrt<float>(mean + eps * pre * pre);  // (pre^2 alone is beyond fp32)
 }
 
 // Vector form: D and the rotated halves are whole 16-byte pieces, every row starts on 16 bytes.
@@ -290,7 +304,21 @@ __global__ void __launch_bounds__(256, RING ? 2 : 3) norm_rope_kernel(const __gr
         float sum = (q0.lo() + q0.hi()) + (q1.lo() + q1.hi());
 #pragma unroll
         for (int d = LPR / 2; d; d >>= 1) sum += __shfl_xor_sync(group_mask, sum, d, LPR);
-        inv = inv_sqrt(fmaf(sum, p.inv_d, it.eps));
+        const float v = fmaf(sum, p.inv_d, it.eps);
+        inv = inv_sqrt<T>(v);
+        if (sizeof(T) == 4 && !squares_in_range(v)) {  // (the group's lanes share v)
+          const float pre = norm_pre(v);
+          const F2 pre2(pre, pre);
+#pragma unroll
+          for (int e = 0; e < V / 2; ++e) f[e] = mul2(f[e], pre2), s[e] = mul2(s[e], pre2);
+          q0 = mul2(f[0], f[0]), q1 = mul2(s[0], s[0]);
+#pragma unroll
+          for (int e = 1; e < V / 2; ++e) q0 = fma2(f[e], f[e], q0), q1 = fma2(s[e], s[e], q1);
+          sum = (q0.lo() + q0.hi()) + (q1.lo() + q1.hi());
+#pragma unroll
+          for (int d = LPR / 2; d; d >>= 1) sum += __shfl_xor_sync(group_mask, sum, d, LPR);
+          inv = norm_inv_pre(sum * p.inv_d, it.eps, pre);
+        }
       }
       const F2 inv2(inv, inv);
 #pragma unroll
@@ -331,16 +359,24 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const __grid_constan
   const T* x = static_cast<const T*>(it.x) + b * it.x_sb + t * it.x_st + h * it.x_sh;
   T* y = static_cast<T*>(it.y) + b * it.y_sb + t * it.y_st + h * it.y_sh;
   const T* sc = static_cast<const T*>(it.scale);
-  float inv = 1.0f;
+  float inv = 1.0f, pre = 1.0f;
   if (sc) {
-    float ss = 0.0f;
-    for (int e = lane; e < p.D; e += 32) {
-      const float v = to_f32(x[e]);
-      ss = fmaf(v, v, ss);
-    }
+    auto sum = [&]() {
+      float ss = 0.0f;
+      for (int e = lane; e < p.D; e += 32) {
+        const float v = to_f32(x[e]) * pre;
+        ss = fmaf(v, v, ss);
+      }
 #pragma unroll
-    for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    inv = inv_sqrt(fmaf(ss, p.inv_d, it.eps));
+      for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+      return ss;
+    };
+    const float v = fmaf(sum(), p.inv_d, it.eps);
+    inv = inv_sqrt<T>(v);
+    if (sizeof(T) == 4 && !squares_in_range(v)) {
+      pre = norm_pre(v);
+      inv = norm_inv_pre(sum() * p.inv_d, it.eps, pre);
+    }
   }
   const int64_t at = table_row(p, token);
   const int half = p.rot / 2;
@@ -350,12 +386,12 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const __grid_constan
     const int ea = p.interleaved ? 2 * i : i, eb = p.interleaved ? 2 * i + 1 : i + half;
     const float c = at >= 0 ? to_f32(ct[i]) : __int_as_float(0x7fc00000);
     const float s = at >= 0 ? to_f32(st[i]) : __int_as_float(0x7fc00000);
-    const float va = to_f32(x[ea]) * inv * (sc ? to_f32(sc[ea]) : 1.0f);
-    const float vb = to_f32(x[eb]) * inv * (sc ? to_f32(sc[eb]) : 1.0f);
+    const float va = to_f32(x[ea]) * pre * inv * (sc ? to_f32(sc[ea]) : 1.0f);
+    const float vb = to_f32(x[eb]) * pre * inv * (sc ? to_f32(sc[eb]) : 1.0f);
     from_f32(va * c - vb * s, y[ea]);
     from_f32(va * s + vb * c, y[eb]);
   }
-  for (int e = p.rot + lane; e < p.D; e += 32) from_f32(to_f32(x[e]) * inv * (sc ? to_f32(sc[e]) : 1.0f), y[e]);
+  for (int e = p.rot + lane; e < p.D; e += 32) from_f32(to_f32(x[e]) * pre * inv * (sc ? to_f32(sc[e]) : 1.0f), y[e]);
 }
 
 constexpr int NR_RING = 3;  // groups of four rows a lane holds at once in shared memory: 96 KB a CTA, two CTAs an SM
@@ -463,38 +499,48 @@ __global__ void __launch_bounds__(256) rms_norm_kernel(const T* __restrict__ x, 
   if (WARPS == 1 && row >= rows) return;  // a CTA per row has no rows past the end
   const T* xr = x + row * n;
   T* yr = y + row * n;
-  float ss = 0.0f;
-  for (int64_t e = (int64_t)tid * V; e < n; e += 32 * WARPS * V) {
-    if (VEC) {
-      float f[Chunk<T>::N];
-      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(xr + e), f);
+  float pre = 1.0f;
+  auto sum = [&]() {
+    float ss = 0.0f;
+    for (int64_t e = (int64_t)tid * V; e < n; e += 32 * WARPS * V) {
+      if (VEC) {
+        float f[Chunk<T>::N];
+        Chunk<T>::unpack(*reinterpret_cast<const uint4*>(xr + e), f);
 #pragma unroll
-      for (int i = 0; i < Chunk<T>::N; ++i) ss = fmaf(f[i], f[i], ss);
-    } else {
-      const float f = to_f32(xr[e]);
-      ss = fmaf(f, f, ss);
+        for (int i = 0; i < Chunk<T>::N; ++i) ss = fmaf(f[i] * pre, f[i] * pre, ss);
+      } else {
+        const float f = to_f32(xr[e]) * pre;
+        ss = fmaf(f, f, ss);
+      }
     }
-  }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-  if (WARPS > 1) {
-    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = ss;
-    __syncthreads();
-    ss = 0.0f;
+    for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    if (WARPS > 1) {
+      if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = ss;
+      __syncthreads();
+      ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) ss += s_sum[i];
+      for (int i = 0; i < WARPS; ++i) ss += s_sum[i];
+    }
+    return ss;
+  };
+  const float v = sum() / (float)n + eps;
+  float inv = inv_sqrt<T>(v);
+  if (sizeof(T) == 4 && !squares_in_range(v)) {  // (all of a row's threads)
+    pre = norm_pre(v);
+    if (WARPS > 1) __syncthreads();  // the first sum's parts have been read
+    inv = norm_inv_pre(sum() / (float)n, eps, pre);
   }
-  const float inv = inv_sqrt(ss / (float)n + eps);
   for (int64_t e = (int64_t)tid * V; e < n; e += 32 * WARPS * V) {
     if (VEC) {
       float f[Chunk<T>::N], w[Chunk<T>::N];
       Chunk<T>::unpack(*reinterpret_cast<const uint4*>(xr + e), f);
       Chunk<T>::unpack(*reinterpret_cast<const uint4*>(scale + e), w);
 #pragma unroll
-      for (int i = 0; i < Chunk<T>::N; ++i) f[i] = f[i] * inv * w[i];
+      for (int i = 0; i < Chunk<T>::N; ++i) f[i] = f[i] * pre * inv * w[i];
       *reinterpret_cast<uint4*>(yr + e) = Chunk<T>::pack(f);
     } else {
-      from_f32(to_f32(xr[e]) * inv * to_f32(scale[e]), yr[e]);
+      from_f32(to_f32(xr[e]) * pre * inv * to_f32(scale[e]), yr[e]);
     }
   }
 }
