@@ -85,6 +85,17 @@ __device__ __forceinline__ void mask_entries(const uint4& a, const uint4& b, flo
   for (int e = 0; e < 8; ++e) mk[e] = __uint_as_float(w[e]);
 }
 
+// Eight fp16 entries with -inf for keys whose bit is not set.
+__device__ __forceinline__ uint4 hide_entries(uint4 v, uint32_t see) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (!(see & (1u << (2 * e)))) w[e] = (w[e] & 0xffff0000u) | 0xfc00u;
+    if (!(see & (2u << (2 * e)))) w[e] = (w[e] & 0xffffu) | 0xfc000000u;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <int NS, int MASK>
 __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const __grid_constant__ TileParams p) {
   constexpr bool ADD = MASK == MASK_ADD || MASK == MASK_ADD32;
@@ -349,6 +360,13 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i] = __ldg(entries + i * p.mask_rows);
       }
+      // tiles every row of the warp sees whole skip the test of its keys
+      const bool cut = !__all_sync(0xffffffffu, vis == ~0ull);
+      // whatever a mask holds for a key that the row does not see takes no part: -inf in its place (fp32: see below)
+      if (MASK == MASK_ADD && cut) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = hide_entries(raw[i], (uint32_t)(vis >> (8 * i)));
+      }
       auto load_entries = [&](int i, float (&mk)[8]) {  // of keys 8i .. 8i + 7
         if (MASK == MASK_ADD) mask_entries(raw[i], mk);
         else mask_entries(__ldg(entries + 2 * i * p.mask_rows), __ldg(entries + (2 * i + 1) * p.mask_rows), mk);
@@ -373,8 +391,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
           for (int i = 0; i < 32; ++i) sv[c][i] = __float_as_uint(__uint_as_float(sv[c][i]) * sc);
       }
       const float mul = pos ? sc : 1.0f;
-      // keys the row does not see become -inf; tiles every row of the warp sees whole skip the test
-      if (!__all_sync(0xffffffffu, vis == ~0ull)) {
+      // keys the row does not see become -inf
+      if (cut) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
@@ -429,9 +447,9 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
             load_entries(4 * c + i / 8, mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              // (a hidden key's score is -inf, and so is the sum whatever finite or -inf entry it has)
-              sv[c][i + e] = __float_as_uint(
-                  ex2_approx(fmaf(__uint_as_float(sv[c][i + e]), mul, fmaf(mk[e], AFK_LOG2E, neg_m))));
+              // (a hidden key's score is -inf, and its fp16 entry; an fp32 entry may be anything)
+              const float x = ex2_approx(fmaf(__uint_as_float(sv[c][i + e]), mul, fmaf(mk[e], AFK_LOG2E, neg_m)));
+              sv[c][i + e] = MASK == MASK_ADD32 && sv[c][i + e] == 0xff800000u ? 0u : __float_as_uint(x);
             }
 #pragma unroll
             for (int e = 0; e < 8; e += 2)
