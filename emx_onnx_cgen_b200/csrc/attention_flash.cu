@@ -50,6 +50,7 @@
 // work item's last visible key inside its last tile have their V rows zeroed
 // in shared memory: what padding holds, NaN included, reaches no result.
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include "attention_flash.cuh"
 #include <algorithm>
@@ -98,7 +99,7 @@ __device__ __forceinline__ uint4 hide_entries(uint4 v, uint32_t see) {
 
 template <int NS, int MASK>
 __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const __grid_constant__ TileParams p) {
-  constexpr bool ADD = MASK == MASK_ADD || MASK == MASK_ADD32;
+  constexpr bool ADD32 = MASK == MASK_ADD32;
   constexpr uint32_t QTILE = NS * AFK_QSLAB, KTILE = NS * AFK_KSLAB;
   constexpr int ST = NS == 1 ? 4 : 2;  // K and V stages: 64 KB of loads in flight per CTA at either head size
   extern __shared__ __align__(1024) uint8_t afk_raw[];
@@ -340,7 +341,9 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
     const unsigned long long* words = MASK == MASK_BITS ? p.bits + mrow * p.words + (cl.past ? 0 : p.words_past) + j0 : nullptr;
     unsigned long long word = MASK == MASK_BITS && J > 0 ? words[0] : 0ull;  // the next tile's, loaded a tile ahead
     const uint4* entries = p.add;  // this row's piece 0 of the tile
-    if (ADD) entries += mrow + (int64_t)((cl.past ? 0 : p.words_past) + j0) * (MASK == MASK_ADD ? 8 : 16) * p.mask_rows;
+    if (MASK == MASK_ADD || ADD32)
+      entries += mrow + (int64_t)((cl.past ? 0 : p.words_past) + j0) * (ADD32 ? 16 : 8) * p.mask_rows;
+    float ref = 0.0f;  // mask reference (fp32 entries)
     bool ok = true;
     for (int j = 0; j < J && ok; ++j) {
       const int sb = j & 1, jj = j0 + j;
@@ -367,9 +370,9 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i] = hide_entries(raw[i], (uint32_t)(vis >> (8 * i)));
       }
-      auto load_entries = [&](int i, float (&mk)[8]) {  // of keys 8i .. 8i + 7
-        if (MASK == MASK_ADD) mask_entries(raw[i], mk);
-        else mask_entries(__ldg(entries + 2 * i * p.mask_rows), __ldg(entries + (2 * i + 1) * p.mask_rows), mk);
+      // fp32 entries of keys 8i .. 8i + 7
+      auto load_entries = [&](int i, float (&mk)[8]) {
+        mask_entries(__ldg(entries + 2 * i * p.mask_rows), __ldg(entries + (2 * i + 1) * p.mask_rows), mk);
       };
       ok = mbar_wait(&s_full[sb], (uint32_t)(j >> 1) & 1u, err, DEV_TIMEOUT_EPILOGUE);
       if (!__all_sync(0xffffffffu, ok)) {
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
 #pragma unroll
           for (int i = 0; i < 32; ++i) sv[c][i] = __float_as_uint(__uint_as_float(sv[c][i]) * sc);
       }
-      const float mul = pos ? sc : 1.0f;
+      float mul = pos ? sc : 1.0f;
       // keys the row does not see become -inf
       if (cut) {
 #pragma unroll
@@ -401,8 +404,41 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
             if (!(half & (1u << i))) sv[c][i] = 0xff800000u;
         }
       }
+      if (ADD32) {
+        // the largest entry of a key that the row sees; does it move the reference?
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float mk[8];
+            load_entries(4 * c + i / 8, mk);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (sv[c][i + e] != 0xff800000u) top = fmaxf(top, mk[e]);
+          }
+        if (top > -INFINITY && (m_used == -INFINITY || top - ref > AFK_REFERENCE)) {
+          // (a difference beyond fp32 leaves the keys before no weight, but -inf stands for none seen)
+          if (m_used != -INFINITY) m_used = fmaxf(fmaf(ref - top, AFK_LOG2E, m_used), -FLT_MAX);
+          ref = top;
+        }
+        // scores with their entries; from here on as without a mask
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float mk[8];
+            load_entries(4 * c + i / 8, mk);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float s = fabsf(mk[e]) >= AFK_ALONE ? 0.0f : __uint_as_float(sv[c][i + e]) * mul;
+              if (sv[c][i + e] != 0xff800000u) sv[c][i + e] = __float_as_uint(fmaf(mk[e] - ref, AFK_LOG2E, s));
+            }
+          }
+        mul = 1.0f;
+      }
       float mx;
-      if (ADD) {
+      if (MASK == MASK_ADD) {
         // pass 1: -inf mask entries hide their key; the maximum of the masked scores (any value near it will do)
         mx = -INFINITY;
 #pragma unroll
@@ -410,11 +446,9 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float mk[8];
-            load_entries(4 * c + i / 8, mk);
+            mask_entries(raw[4 * c + i / 8], mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              if (MASK == MASK_ADD32 && fabsf(mk[e]) >= AFK_ALONE && sv[c][i + e] != 0xff800000u)
-                sv[c][i + e] = 0u;  // (fp16 entries are not as large; a hidden key's score stays -inf)
               if (mk[e] == -INFINITY) sv[c][i + e] = 0xff800000u;
               else mx = fmaxf(mx, fmaf(__uint_as_float(sv[c][i + e]), mul, mk[e] * AFK_LOG2E));
             }
@@ -438,18 +472,18 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
       uint32_t pw[2][16];
       float lp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (ADD) {
+      if (MASK == MASK_ADD) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float mk[8];
-            load_entries(4 * c + i / 8, mk);
+            mask_entries(raw[4 * c + i / 8], mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              // (a hidden key's score is -inf, and its fp16 entry; an fp32 entry may be anything)
-              const float x = ex2_approx(fmaf(__uint_as_float(sv[c][i + e]), mul, fmaf(mk[e], AFK_LOG2E, neg_m)));
-              sv[c][i + e] = MASK == MASK_ADD32 && sv[c][i + e] == 0xff800000u ? 0u : __float_as_uint(x);
+              // (a hidden key's score is -inf, and its entry)
+              sv[c][i + e] = __float_as_uint(
+                  ex2_approx(fmaf(__uint_as_float(sv[c][i + e]), mul, fmaf(mk[e], AFK_LOG2E, neg_m))));
             }
 #pragma unroll
             for (int e = 0; e < 8; e += 2)
@@ -502,7 +536,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         *reinterpret_cast<uint4*>(s_p + r * 128 + ((g ^ (r & 7)) << 4)) =
             make_uint4(pw[c][i], pw[c][i + 1], pw[c][i + 2], pw[c][i + 3]);
       }
-      if (ADD) entries += (MASK == MASK_ADD ? 8 : 16) * p.mask_rows;
+      if (MASK == MASK_ADD || ADD32) entries += (ADD32 ? 16 : 8) * p.mask_rows;
       fence_async_shared();  // the generic writes of P become visible to the tensor cores
       tc_fence_before();
       __syncwarp();
@@ -522,6 +556,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       uint16_t* orow = p.o + (int64_t)w.b * p.o_sb + (int64_t)w.h * p.o_sh + (int64_t)w.t * p.o_st;
       float* prow = part ? p.part_o + slot_row * p.DV : nullptr;
       if (part && live) p.part_ml[slot_row] = make_float2(m_used, l);
+      if (ADD32 && part && live) p.part_ref[slot_row] = ref;
       if (!(part && J == 0)) {  // the merge does not read the output of an item with l = 0
 #pragma unroll
         for (int c = 0; c < 2 * NS; ++c) {
@@ -565,8 +600,11 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
 
 // ------------------------------------------------------------------ merging split key ranges
 // One warp per query row, DV / 4 lanes with four columns each; slots in order.
+// REF: maxima are relative to mask references (fp32 additive masks); they are taken to the slots' largest one first.
+template <bool REF>
 __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __restrict__ part_o,
-                                                                const float2* __restrict__ part_ml, int slots,
+                                                                const float2* __restrict__ part_ml,
+                                                                const float* __restrict__ part_ref, int slots,
                                                                 int64_t rows, int TQ, int HQ, int DV,
                                                                 uint16_t* __restrict__ o, int64_t o_sb, int64_t o_sh,
                                                                 int64_t o_st) {
@@ -577,11 +615,23 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __r
   if (row >= rows) return;
   // lane s: slot s0 + s; the first 32 slots' (m, l) are loaded once
   const float2 none = make_float2(-INFINITY, 0.0f);
-  float2 ml = lane < slots ? part_ml[(int64_t)lane * rows + row] : none;
+  float ref = -INFINITY;
+  if (REF) {
+    for (int s = lane; s < slots; s += 32)
+      if (part_ml[(int64_t)s * rows + row].y != 0.0f) ref = fmaxf(ref, part_ref[(int64_t)s * rows + row]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, d));
+  }
+  auto slot_ml = [&](int s) {
+    float2 ml = part_ml[(int64_t)s * rows + row];
+    if (REF && ml.y != 0.0f) ml.x = fmaf(part_ref[(int64_t)s * rows + row] - ref, AFK_LOG2E, ml.x);
+    return ml;
+  };
+  float2 ml = lane < slots ? slot_ml(lane) : none;
   const float2 first = ml;
   float m = ml.y != 0.0f ? ml.x : -INFINITY;
   for (int s = lane + 32; s < slots; s += 32) {
-    ml = part_ml[(int64_t)s * rows + row];
+    ml = slot_ml(s);
     if (ml.y != 0.0f) m = fmaxf(m, ml.x);
   }
 #pragma unroll
@@ -589,7 +639,7 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __r
   float l = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < slots; s0 += 32) {
-    ml = s0 == 0 ? first : s0 + lane < slots ? part_ml[(int64_t)(s0 + lane) * rows + row] : none;
+    ml = s0 == 0 ? first : s0 + lane < slots ? slot_ml(s0 + lane) : none;
     const float wgt = ml.y != 0.0f ? ex2_approx(ml.x - m) : 0.0f;
     const uint32_t seen = __ballot_sync(0xffffffffu, ml.y != 0.0f);  // the others saw no key: their output is not written
     float part_l = ml.y != 0.0f ? wgt * ml.y : 0.0f;
@@ -677,7 +727,7 @@ __global__ void __launch_bounds__(256) mask_pack_kernel(const uint8_t* __restric
 
 // ------------------------------------------------------------------ whole tiles of additive masks
 // y[tile][16-byte piece][row]: the past's tiles, then the current keys', -inf past the mask's length and each part's
-// keys, finite fp32 entries within their bound.  A row's thread reads its row of a tile 16 bytes at a time: straight
+// keys.  A row's thread reads its row of a tile 16 bytes at a time: straight
 // from the mask, 32 rows' pieces are 32 sectors of 32 rows ([57, 16, 45 x 2952, 96] with a mask row per query took
 // 810 us so); from here they are 512 bytes in line.  A CTA copies 32 rows of a tile through shared memory.
 template <typename T>
@@ -697,10 +747,7 @@ __global__ void __launch_bounds__(256) mask_tiles_kernel(const T* __restrict__ m
     for (int i = 0; i < 8; ++i) {
       const int x = threadIdx.x + 256 * i, r = x >> 6, k = x & 63;
       T v = (T)-INFINITY;
-      if (r < here && k < n) {
-        v = mask[(row0 + r) * len + at + k];
-        if (sizeof(T) == 4) v = (T)additive_bounded((float)v);
-      }
+      if (r < here && k < n) v = mask[(row0 + r) * len + at + k];
       reinterpret_cast<T*>(s_tile[r])[k] = v;
     }
     __syncthreads();
@@ -789,7 +836,7 @@ static int make_tmap_q(CUtensorMap* map, const RowsParams& r, int64_t tokens, in
 static int tile_params(TileParams& p, const RowsParams& r, const ItemClass* cls, int first1, int items,
                        int tile_keys) {
   p.cls[0] = cls[0], p.cls[1] = cls[1], p.first1 = first1, p.items = items;
-  p.q = r.q, p.o = r.o, p.part_o = r.part_o, p.part_ml = r.part_ml;
+  p.q = r.q, p.o = r.o, p.part_o = r.part_o, p.part_ml = r.part_ml, p.part_ref = r.part_ref;
   p.q_sb = r.q_sb, p.q_sh = r.q_sh, p.q_st = r.q_st, p.o_sb = r.o_sb, p.o_sh = r.o_sh, p.o_st = r.o_st;
   p.B = r.B, p.HQ = r.HQ, p.HKV = r.HKV, p.group = r.group, p.TQ = r.TQ, p.D = r.D, p.DV = r.DV;
   p.causal = r.causal, p.tk = r.tk, p.tp = r.tp, p.past_shared = r.past_shared;
@@ -845,13 +892,13 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
     if ((uintptr_t)ptr(i) & 15u) return 5;
   if ((uintptr_t)r.counts & 7u) return 5;
   const int kind = (int)op.ip[AF_MASK_KIND];
-  const int variant = kind == AF_MASK_NONE ? MASK_NONE : kind == AF_MASK_BOOL ? MASK_BITS : MASK_ADD;
+  const int variant = kind == AF_MASK_NONE ? MASK_NONE : kind == AF_MASK_BOOL ? MASK_BITS : kind == AF_MASK_F16 ? MASK_ADD : MASK_ADD32;
+  const bool additive = variant == MASK_ADD || variant == MASK_ADD32;
   r.mask_sb = op.ip[AF_MASK_SB], r.mask_sh = op.ip[AF_MASK_SH], r.mask_st = op.ip[AF_MASK_ST];
   r.mask_len = (int)op.ip[AF_MASK_LEN];
   r.mask_bool = variant == MASK_BITS ? (const uint8_t*)ptr(4) : nullptr;
-  r.mask_add = variant == MASK_ADD ? ptr(4) : nullptr;
-  r.add_f32 = kind == AF_MASK_F32;
-  if (variant == MASK_ADD && ((uintptr_t)r.mask_add & (r.add_f32 ? 3u : 1u))) return 5;
+  r.mask_add = additive ? ptr(4) : nullptr;
+  if (additive && ((uintptr_t)r.mask_add & (variant == MASK_ADD32 ? 3u : 1u))) return 5;
 
   // ---------------- work items of the two classes
   const int64_t rows = (int64_t)r.B * tq * r.HQ;
@@ -880,9 +927,10 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
       (apart && r.B * tq * tq > 0xffffffffll))
     return 5;
   if (slots > 1) {
-    // (m, l) pairs behind the outputs, both sized for the compiled batch
+    // (m, l) pairs behind the outputs, mask references behind them, all sized for the compiled batch
     r.part_o = (float*)ptr(8);
     r.part_ml = (float2*)(r.part_o + (int64_t)slots * rows * r.DV);
+    if (variant == MASK_ADD32) r.part_ref = (float*)(r.part_ml + (int64_t)slots * rows);
   }
 
   // ---------------- passes: one kernel for both classes, or the past's first and the own keys' beside it
@@ -916,7 +964,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
     } else {
       TileParams p{};
       const int tile_keys = pass == AF_PASS_WIDE ? 128 : AFK_N;
-      if (pass == AF_PASS_WIDE && variant == MASK_ADD) return 5;  // (never planned)
+      if (pass == AF_PASS_WIDE && additive) return 5;  // (never planned)
       int rc = tile_params(p, r, cls, (int)n1, (int)(n0 + n1), tile_keys);
       p.drop_keys = (ctx.fault & FAULT_DROP_KEY_TILES) != 0;
       if (rc) return rc;
@@ -931,11 +979,11 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
                        (int)(p.mask_len % 16 == 0 && p.tp % 16 == 0 && ((uintptr_t)r.mask_bool & 15u) == 0),
                        (unsigned long long*)p.bits, (int4*)p.spans);
         ++*launches;
-      } else if (variant == MASK_ADD) {
+      } else if (additive) {
         p.add = (const uint4*)ptr(9);
         p.mask_rows = mrows;
         const dim3 grid((unsigned)((mrows + 31) / 32), (unsigned)std::min(p.words, 65535));
-        if (r.add_f32)
+        if (variant == MASK_ADD32)
           e = launch_pdl(mask_tiles_kernel<float>, grid, dim3(256), 0, ctx.stream, (const float*)r.mask_add, p.mask_len, p.tp,
                          p.tk, p.words_past, p.words, mrows, (uint4*)ptr(9));
         else
@@ -946,14 +994,15 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
       if (e != cudaSuccess) return 4;
       const int ns = flash_slabs(op);
       e = pass == AF_PASS_WIDE ? launch_attention_wide(p, ns, variant, ctx.num_sms, ctx.stream)
-                               : launch_pdl(flash_kernel(ns, r.add_f32 ? MASK_ADD32 : variant), dim3((unsigned)(n0 + n1)), dim3(AFK_THREADS),
+                               : launch_pdl(flash_kernel(ns, variant), dim3((unsigned)(n0 + n1)), dim3(AFK_THREADS),
                                             flash_smem(ns), ctx.stream, p);
     }
     ++*launches;
   }
   if (e == cudaSuccess && slots > 1) {
-    e = launch_pdl(attention_combine_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx.stream,
-                   (const float*)r.part_o, (const float2*)r.part_ml, slots, rows, (int)tq, r.HQ, r.DV, r.o, r.o_sb, r.o_sh,
+    e = launch_pdl(r.part_ref ? attention_combine_kernel<true> : attention_combine_kernel<false>,
+                   dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx.stream, (const float*)r.part_o,
+                   (const float2*)r.part_ml, (const float*)r.part_ref, slots, rows, (int)tq, r.HQ, r.DV, r.o, r.o_sb, r.o_sh,
                    r.o_st);
     ++*launches;
   }

@@ -11,7 +11,7 @@ namespace emx {
 constexpr float AFK_RESCALE = 8.0f;  // the output is rescaled when a row's maximum grows by more (log2 units)
 constexpr float AFK_LOG2E = 1.4426950408889634f;
 
-enum { MASK_NONE = 0, MASK_BITS = 1, MASK_ADD = 2, MASK_ADD32 = 3 /*fp32 entries; attention_flash.cu only*/ };  // kernel variants
+enum { MASK_NONE = 0, MASK_BITS = 1, MASK_ADD = 2 /*fp16 entries*/, MASK_ADD32 = 3 };  // kernel variants
 
 struct RowId {
   int b, h, t;
@@ -40,19 +40,14 @@ __device__ __forceinline__ RowId row_of(int r, const SmallDiv& group, const Smal
   return id;
 }
 
-// Finite fp32 entries beyond 2^24 count as 2^24: no score reaches across that, and the differences formed from
-// them stay finite.  From 2^56 on they count as 2^25 and stand alone: beside them a sum, in 64 bits too, has none of
-// its score's digits left, so keys at the type's lowest value weigh the same among themselves.  Infinities and NaN stay.
-constexpr float AFK_ALONE = 0x1p25f;
-__device__ __forceinline__ float additive_bounded(float v) {
-  const float a = fabsf(v);
-  return a > 0x1p24f && a < INFINITY ? copysignf(a >= 0x1p56f ? AFK_ALONE : 0x1p24f, v) : v;
-}
-
-__device__ __forceinline__ float additive_entry(const void* mask, int f32, int64_t at) {
-  if (f32) return additive_bounded(__ldg(static_cast<const float*>(mask) + at));
-  return __half2float(__ldg(static_cast<const __half*>(mask) + at));
-}
+// fp32 entries may be so large that a score added to them loses its digits, and so far apart that their difference
+// decides alone.  The passes therefore hold a row's running maximum as a pair (mask reference R, maximum m of
+// score + (entry - R)): R is the largest visible entry of some key tile, and moves when a later one is more than
+// AFK_REFERENCE above it, so keys that matter have small differences to it, formed before the score is added.  Partial
+// results carry R beside (m, l).  Entries from 2^56 on leave no digit of a score in 64 bits either: their keys count
+// without it (those at the type's lowest value weigh the same among themselves).
+constexpr float AFK_ALONE = 0x1p56f;
+constexpr float AFK_REFERENCE = 16.0f;
 
 // The work items of a pass come in two classes: 0, the rows of one sequence
 // against its own keys (behind its past where `past` is set: one list of key
@@ -82,6 +77,7 @@ struct TileParams {
   uint16_t* o;
   float* part_o;    // [slot][row][DV], null: one item per row, written to o
   float2* part_ml;  // [slot][row] (m, l)
+  float* part_ref;  // [slot][row] mask references, fp32 additive masks only
   int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
   int B, HQ, HKV, D, DV, causal, tk, tp, past_shared;
   SmallDiv group, TQ;
@@ -107,6 +103,7 @@ struct RowsParams {
   uint16_t* o;
   float* part_o;
   float2* part_ml;
+  float* part_ref;
   int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, o_sb, o_sh, o_st;
   int B, HQ, HKV, D, DV, causal, tp, tk, past_shared;
   SmallDiv group, TQ;
@@ -114,7 +111,7 @@ struct RowsParams {
   int64_t mask_sb, mask_sh, mask_st;
   const uint8_t* mask_bool;
   const void* mask_add;
-  int mask_len, add_f32;
+  int mask_len;
   float scale_log2;
   int late_wait;  // launched behind a pass whose results it does not read
   int* err;

@@ -37,6 +37,7 @@
 // visible key are not read (but for the first copies, which are on their way by
 // then), and values behind that key take no part.
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include "attention_flash.cuh"
 #include "host_util.h"
@@ -79,6 +80,11 @@ __device__ __forceinline__ int rows_place(int r, int c) { return c ^ (r & 6) ^ (
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+template <bool F32>
+__device__ __forceinline__ float additive_entry(const void* mask, int64_t at) {
+  return F32 ? __ldg(static_cast<const float*>(mask) + at) : __half2float(__ldg(static_cast<const __half*>(mask) + at));
+}
+
 // NS: 64-wide slabs of the head size; NT: tiles of 8 query rows; MASK: MASK_*
 template <int NS, int NT, int MASK>
 __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const __grid_constant__ RowsParams p) {
@@ -89,14 +95,16 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   constexpr int STAGE = U * BLOCK;
   constexpr int ST = AR_RING / STAGE;             // 3 steps, or 6 at NS = 1, NT = 2
   constexpr int OW = 64 * NS + 4;                 // padded row of the merge buffer
+  constexpr bool ADD = MASK == MASK_ADD || MASK == MASK_ADD32, ADD32 = MASK == MASK_ADD32;
   extern __shared__ __align__(128) uint8_t s_all[];  // rows_smem() bytes
   __shared__ uint32_t s_bits[MASK == MASK_BITS ? 8 * NT * AF_ROWS_MASK_KEYS / 32 : 1];  // [row][32 keys]
   __shared__ int s_range[2];
   __shared__ float2 s_row[8 * NT];
+  __shared__ float s_ref[ADD32 ? 8 * NT : 1];
   const int warps = blockDim.x >> 5;
   float(*s_o)[8 * NT][OW] = reinterpret_cast<float(*)[8 * NT][OW]>(s_all);  // once the ring is done with
   float(*s_m)[8 * NT] = reinterpret_cast<float(*)[8 * NT]>(s_all + (size_t)warps * 8 * NT * OW * 4);
-  float(*s_l)[8 * NT] = s_m + warps;
+  float(*s_l)[8 * NT] = s_m + warps, (*s_r)[8 * NT] = s_l + warps;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (!p.late_wait) pdl_wait();
   pdl_launch_dependents();
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
     for (int e = 0; e < 2; ++e) {
       const int r = 8 * n + 2 * t + e;
       const RowId w = row_of(row0 + min(r, rows - 1), p.group, p.TQ, kvh, b, past_item);
-      mrow[n][e] = MASK != MASK_ADD ? 0 : (w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st) * (int64_t)p.mask_len;
+      mrow[n][e] = !ADD ? 0 : (w.b * p.mask_sb + w.h * p.mask_sh + w.t * p.mask_st) * (int64_t)p.mask_len;
       lim[n][e] = r >= rows || past_item ? 0x7fffffff : p.tp + (p.causal ? min(keys, w.t + 1) : keys);
       lim_all = min(lim_all, lim[n][e]);
     }
@@ -257,10 +265,10 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   }
 
   // additive mask entries of a step at this thread's scores, loaded a step ahead
-  float mk[U][MASK == MASK_ADD ? 4 * NT : 1], mk_next[U][MASK == MASK_ADD ? 4 * NT : 1];
+  float mk[U][ADD ? 4 * NT : 1], mk_next[U][ADD ? 4 * NT : 1];
   auto load_add = [&](int blk) {
 #pragma unroll
-    for (int u = 0; u < (MASK == MASK_ADD ? U : 0); ++u, ++blk) {
+    for (int u = 0; u < (ADD ? U : 0); ++u, ++blk) {
       const bool is_past = blk < pblocks;
       const int k0 = (is_past ? blk : blk - pblocks) * AR_KB, pos0 = (is_past ? 0 : p.tp) + k0;
 #pragma unroll
@@ -272,17 +280,17 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             mk_next[u][(h * NT + n) * 2 + e] =
-                in && pos < p.mask_len ? additive_entry(p.mask_add, p.add_f32, mrow[n][e] + pos) : -INFINITY;
+                in && pos < p.mask_len ? additive_entry<ADD32>(p.mask_add, mrow[n][e] + pos) : -INFINITY;
       }
     }
   };
 
   float o[NT][NS][4][4];  // O^T: [row tile][slab][d pair][(d, row), (d, row + 1), (d + 1, row), (d + 1, row + 1)]
-  float m_ref[NT][2], l[NT][2];
+  float m_ref[NT][2], l[NT][2], ref[NT][2];  // ref: mask references (fp32 entries)
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) m_ref[n][e] = -INFINITY, l[n][e] = 0.0f;
+    for (int e = 0; e < 2; ++e) m_ref[n][e] = -INFINITY, l[n][e] = 0.0f, ref[n][e] = 0.0f;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -301,7 +309,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
     cp_async_wait_group<ST - 2>();  // this step's copies (one group a step) are done, for every lane
     __syncwarp();
     issue(blk + (ST - 1) * U * warps, (n + ST - 1) % ST);  // into the stage of the step before this one
-    if (MASK == MASK_ADD) {
+    if (ADD) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -331,9 +339,9 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
           for (int h = 0; h < 2; ++h) {
             const int pos = pos0 + 8 * h + g, i = (h * NT + n2) * 2 + e;
             bool ok = pos < min(lim[n2][e], seg_end) && ((bits >> (8 * h + g)) & 1u);
-            if (MASK == MASK_ADD) {
+            if (ADD) {
               ok = ok && mk[u][i] != -INFINITY;
-              if (!ok) mk[u][i] = 0.0f;
+              if (!ok) mk[u][i] = ADD32 ? -INFINITY : 0.0f;
             }
             if (!ok) see &= ~(1u << (4 * NT * u + i));
           }
@@ -366,7 +374,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[u][n2][e] = (s[u][n2][e] + s2[e]) * sc;
-          if (MASK == MASK_ADD && fabsf(mk[u][((e >> 1) * NT + n2) * 2 + (e & 1)]) >= AFK_ALONE) s[u][n2][e] = 0.0f;
+          if (ADD32 && fabsf(mk[u][((e >> 1) * NT + n2) * 2 + (e & 1)]) >= AFK_ALONE) s[u][n2][e] = 0.0f;
         }
       }
     // V in K's registers, on its way during the softmax
@@ -405,6 +413,44 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (!((see >> (4 * NT * u + ((e >> 1) * NT + n2) * 2 + (e & 1))) & 1u)) s[u][n2][e] = -INFINITY;
+    }
+    // fp32 entries: the largest of a row's visible keys may move its reference; then they join the scores
+    if (ADD32) {
+      float most[NT][2];
+      bool move = false;
+#pragma unroll
+      for (int n2 = 0; n2 < NT; ++n2)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          most[n2][e] = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) most[n2][e] = fmaxf(most[n2][e], mk[u][(h * NT + n2) * 2 + e]);
+          move = move || (most[n2][e] > -INFINITY && (m_ref[n2][e] == -INFINITY || most[n2][e] - ref[n2][e] > AFK_REFERENCE));
+        }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int n2 = 0; n2 < NT; ++n2)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = most[n2][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            if (x > -INFINITY && (m_ref[n2][e] == -INFINITY || x - ref[n2][e] > AFK_REFERENCE)) {
+              // (a difference beyond fp32 leaves the keys before no weight, but -inf stands for none seen)
+              if (m_ref[n2][e] != -INFINITY) m_ref[n2][e] = fmaxf(fmaf(ref[n2][e] - x, AFK_LOG2E, m_ref[n2][e]), -FLT_MAX);
+              ref[n2][e] = x;
+            }
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n2 = 0; n2 < NT; ++n2)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[u][n2][e] = fmaf(mk[u][((e >> 1) * NT + n2) * 2 + (e & 1)] - ref[n2][e & 1], AFK_LOG2E, s[u][n2][e]);
     }
     bool grow = false;
     float top[NT][2];
@@ -503,6 +549,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
       if (g == 0) {
         s_m[warp][r] = m_ref[n][e];
         s_l[warp][r] = l[n][e];
+        if (ADD32) s_r[warp][r] = ref[n][e];
       }
       if (!any_block) continue;  // l = 0: nothing reads this warp's output
 #pragma unroll
@@ -520,7 +567,16 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
     if (r < 8 * NT) {  // whole groups of eight lanes; CTAs of fewer threads than rows x 8 go around below
       for (int rr = r; rr < 8 * NT; rr += blockDim.x >> 3) {
         const bool in = w < warps && rr < rows;
-        const float lw = in ? s_l[w][rr] : 0.0f, mw = in && lw != 0.0f ? s_m[w][rr] : -INFINITY;
+        const float lw = in ? s_l[w][rr] : 0.0f;
+        float mw = in && lw != 0.0f ? s_m[w][rr] : -INFINITY;
+        if (ADD32) {  // maxima relative to the warps' largest reference
+          const float rw = in && lw != 0.0f ? s_r[w][rr] : -INFINITY;
+          float most = rw;
+#pragma unroll
+          for (int d = 4; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d, 8));
+          if (in && lw != 0.0f) mw = fmaf(rw - most, AFK_LOG2E, mw);
+          if (w == 0 && rr < rows) s_ref[rr] = most;
+        }
         float m = mw, sum;
 #pragma unroll
         for (int d = 4; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d, 8));
@@ -551,6 +607,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
     if (p.part_o) {
       const int64_t at = (int64_t)(cl.part0 + split) * ((int64_t)p.B * (int)p.TQ.d * p.HQ) + ((int64_t)w.b * (int)p.TQ.d + w.t) * p.HQ + w.h;
       if (d == 0) p.part_ml[at] = ms;
+      if (ADD32 && d == 0) p.part_ref[at] = s_ref[r];
       *reinterpret_cast<float4*>(p.part_o + at * p.DV + d) = acc;
     } else {
       const float inv = ms.y == 0.0f ? 0.0f : 1.0f / ms.y;
@@ -566,7 +623,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
 
 // ------------------------------------------------------------------ host side
 static size_t rows_smem(int ns, int nt, int warps) {
-  const size_t merge = (size_t)warps * 8 * nt * (64 * ns + 4 + 2) * sizeof(float), ring = (size_t)warps * AR_RING;
+  const size_t merge = (size_t)warps * 8 * nt * (64 * ns + 4 + 3) * sizeof(float), ring = (size_t)warps * AR_RING;
   return merge > ring ? merge : ring;
 }
 
@@ -574,7 +631,8 @@ template <int NS, int NT>
 static const void* rows_kernel(int mask) {
   return mask == MASK_NONE ? (const void*)attention_rows_kernel<NS, NT, MASK_NONE>
          : mask == MASK_BITS ? (const void*)attention_rows_kernel<NS, NT, MASK_BITS>
-                             : (const void*)attention_rows_kernel<NS, NT, MASK_ADD>;
+         : mask == MASK_ADD  ? (const void*)attention_rows_kernel<NS, NT, MASK_ADD>
+                             : (const void*)attention_rows_kernel<NS, NT, MASK_ADD32>;
 }
 
 static const void* rows_kernel(bool wide, int row_tiles, int mask) {
@@ -583,7 +641,7 @@ static const void* rows_kernel(bool wide, int row_tiles, int mask) {
 }
 
 cudaError_t prepare_attention_rows() {
-  for (int i = 0; i < 12; ++i) {
+  for (int i = 0; i < 16; ++i) {
     cudaError_t e = cudaFuncSetAttribute(rows_kernel(i & 1, 1 + ((i >> 1) & 1), i >> 2),
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, AR_WARPS * AR_RING);
     if (e != cudaSuccess) return e;

@@ -64,3 +64,39 @@ def test_visible_infinite_and_nan_entries(q_seq, mask):
     assert np.isnan(got[0, :, 1]).all() and np.isnan(got[1, :, 2]).all()
     got[0, :, 1], got[1, :, 2] = want[0, :, 1], want[1, :, 2]
     check(got, want, tol, str(kw))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(batch=3, q_heads=2, kv_heads=2, q_seq=2, kv_seq=200),                         # few-row pass
+    dict(batch=2, q_heads=6, kv_heads=2, q_seq=5, kv_seq=333, head_dim=128),           # its 16-row form
+    dict(batch=1, q_heads=2, kv_heads=2, q_seq=3, kv_seq=4000),                        # split key ranges
+    dict(batch=3, q_heads=2, kv_heads=2, q_seq=40, kv_seq=200),                        # 128-row pass
+    dict(batch=1, q_heads=2, kv_heads=2, q_seq=20, kv_seq=3000, head_dim=128),         # split
+    dict(batch=2, q_heads=2, kv_heads=1, q_seq=150, kv_seq=190, causal=True),
+    dict(batch=3, q_heads=4, kv_heads=2, q_seq=2, kv_seq=70, past=321),                # a shared past: merged
+    dict(batch=40, q_heads=8, kv_heads=2, q_seq=1, kv_seq=70, past=700, head_dim=128),
+    dict(batch=3, q_heads=4, kv_heads=2, q_seq=30, kv_seq=30, past=321, shared_past=False, causal=True),
+])
+def test_large_additive_entries_keep_their_order(kw):
+    """fp32 entries beyond 2^24 of different sizes in one row: only the largest of them count, and among equal ones the
+    scores decide (from 2^56 on a sum has none of its score's digits in 64 bits either)."""
+    require_gpu()
+    b, tq, t = kw["batch"], kw["q_seq"], kw["kv_seq"] + kw.get("past", 0)
+    kw = dict(kw, mask="f32", mask_shape=(b, 1, tq, t))
+    wl = W.decoder_attention(**kw)
+    x = wl.make_inputs(31)
+    r = np.random.default_rng(7)
+    levels = [(-1e9, -2e9), (-1e30, np.finfo(np.float32).min), (-2e9, -1e9, -3e7), (0.0, -1e9, -2e9), (1e9, 2e9, -1e9),
+              (-1e30, -1e9), (1e30, 3e38), (-3e7, -4e7), (-1e9, -1e9 - 64, -1e9 - 128), (0.0, -1e9, np.finfo(np.float32).min),
+              (np.finfo(np.float32).min, np.finfo(np.float32).max), (-16777216.0, -16777218.0, -16777220.0)]
+    m = x["mask"]
+    for i in range(b):
+        for q in range(tq):
+            lv = np.array(levels[(i * tq + q) % len(levels)], np.float32)
+            row = lv[r.integers(0, len(lv), t)]
+            if q % 3 == 1:  # the larger ones late, or early, in the row
+                row = np.sort(row)
+            elif q % 3 == 2:
+                row = np.sort(row)[::-1]
+            m[i, 0, q] = row
+    check(run(wl, x), *decoder_attention(wl, x), str(kw))
