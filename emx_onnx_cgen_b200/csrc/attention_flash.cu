@@ -365,11 +365,6 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       }
       // tiles every row of the warp sees whole skip the test of its keys
       const bool cut = !__all_sync(0xffffffffu, vis == ~0ull);
-      // whatever a mask holds for a key that the row does not see takes no part: -inf in its place (fp32: see below)
-      if (MASK == MASK_ADD && cut) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) raw[i] = hide_entries(raw[i], (uint32_t)(vis >> (8 * i)));
-      }
       // fp32 entries of keys 8i .. 8i + 7
       auto load_entries = [&](int i, float (&mk)[8]) {
         mask_entries(__ldg(entries + 2 * i * p.mask_rows), __ldg(entries + (2 * i + 1) * p.mask_rows), mk);
@@ -394,8 +389,12 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
           for (int i = 0; i < 32; ++i) sv[c][i] = __float_as_uint(__uint_as_float(sv[c][i]) * sc);
       }
       float mul = pos ? sc : 1.0f;
-      // keys the row does not see become -inf
+      // keys the row does not see become -inf, and so do their fp16 entries, whatever they are (fp32: see below)
       if (cut) {
+        if (MASK == MASK_ADD) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) raw[i] = hide_entries(raw[i], (uint32_t)(vis >> (8 * i)));
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
