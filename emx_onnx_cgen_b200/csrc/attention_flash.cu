@@ -11,9 +11,9 @@
 // accumulator are fp32 (TMEM for the latter); the weights are rounded to fp16
 // for the second matrix product (half an fp16 step each, 2^-11 relative: the
 // output type's own step) and the sum adds those same rounded weights.  A row
-// that sees no key gives 0.  An additive mask enters the exponent as
-// (mask log2 e - m) before the score is added, so scores keep their digits
-// beside masks as large as the type's lowest value.
+// that sees no key gives 0.  Additive entries are taken relative to a mask
+// reference of the row (attention_flash.cuh) before the score is added, so
+// scores keep their digits beside masks as large as the type's lowest value.
 //
 // Rows: the query rows that read the same keys are packed into tiles of 128
 // whatever (token, head, sequence) they come from -- the group of query heads
@@ -39,8 +39,8 @@
 // What bounds it: at two CTAs an SM the softmax warps' issue slots (64 scores a
 // row and tile in registers, an exponential each), then, for short keys, the
 // set-up of a work item (TMEM, barriers, Q: some 5 us).  [57, 16, 45 x 2952, 96]
-// with an additive mask: 217 us, 215 TFLOP/s; [3, 12, 77 x 333, 80]: 18 us,
-// three launches.
+// with an fp16 additive mask: 211 us, 221 TFLOP/s; [3, 12, 77 x 333, 80]: 16.4
+// us, three launches.
 //
 // Boolean masks are first packed by mask_pack_kernel to one 64-bit word per
 // (mask row, 64 keys) plus each row's first and last visible key, so a row's
@@ -50,7 +50,6 @@
 // work item's last visible key inside its last tile have their V rows zeroed
 // in shared memory: what padding holds, NaN included, reaches no result.
 #include <cuda_fp16.h>
-#include <float.h>
 
 #include "attention_flash.cuh"
 #include <algorithm>
@@ -97,9 +96,27 @@ __device__ __forceinline__ uint4 hide_entries(uint4 v, uint32_t see) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The largest of a tile's fp16 entries (NaN left out).
+template <int N>
+__device__ __forceinline__ float largest_entry(const uint4 (&raw)[N]) {
+  __half2 m[4];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const __half2 v = *reinterpret_cast<const __half2*>(&w[e]);
+      m[e] = i == 0 ? v : __hmax2(m[e], v);
+    }
+  }
+  const float2 f = __half22float2(__hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3])));
+  return fmaxf(f.x, f.y);
+}
+
 template <int NS, int MASK>
 __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const __grid_constant__ TileParams p) {
-  constexpr bool ADD32 = MASK == MASK_ADD32;
+  constexpr bool ADD32 = MASK == MASK_ADD32, ADD = MASK == MASK_ADD || ADD32;
+  using Ref = MaskReference<ADD32>;
   constexpr uint32_t QTILE = NS * AFK_QSLAB, KTILE = NS * AFK_KSLAB;
   constexpr int ST = NS == 1 ? 4 : 2;  // K and V stages: 64 KB of loads in flight per CTA at either head size
   extern __shared__ __align__(1024) uint8_t afk_raw[];
@@ -341,9 +358,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
     const unsigned long long* words = MASK == MASK_BITS ? p.bits + mrow * p.words + (cl.past ? 0 : p.words_past) + j0 : nullptr;
     unsigned long long word = MASK == MASK_BITS && J > 0 ? words[0] : 0ull;  // the next tile's, loaded a tile ahead
     const uint4* entries = p.add;  // this row's piece 0 of the tile
-    if (MASK == MASK_ADD || ADD32)
-      entries += mrow + (int64_t)((cl.past ? 0 : p.words_past) + j0) * (ADD32 ? 16 : 8) * p.mask_rows;
-    float ref = 0.0f;  // mask reference (fp32 entries)
+    if (ADD) entries += mrow + (int64_t)((cl.past ? 0 : p.words_past) + j0) * (ADD32 ? 16 : 8) * p.mask_rows;
+    float ref = 0.0f;  // mask reference
     bool ok = true;
     for (int j = 0; j < J && ok; ++j) {
       const int sb = j & 1, jj = j0 + j;
@@ -365,9 +381,9 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       }
       // tiles every row of the warp sees whole skip the test of its keys
       const bool cut = !__all_sync(0xffffffffu, vis == ~0ull);
-      // fp32 entries of keys 8i .. 8i + 7
-      auto load_entries = [&](int i, float (&mk)[8]) {
-        mask_entries(__ldg(entries + 2 * i * p.mask_rows), __ldg(entries + (2 * i + 1) * p.mask_rows), mk);
+      auto load_entries = [&](int i, float (&mk)[8]) {  // of keys 8i .. 8i + 7
+        if (MASK == MASK_ADD) mask_entries(raw[i], mk);
+        else mask_entries(__ldg(entries + 2 * i * p.mask_rows), __ldg(entries + (2 * i + 1) * p.mask_rows), mk);
       };
       ok = mbar_wait(&s_full[sb], (uint32_t)(j >> 1) & 1u, err, DEV_TIMEOUT_EPILOGUE);
       if (!__all_sync(0xffffffffu, ok)) {
@@ -389,12 +405,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
           for (int i = 0; i < 32; ++i) sv[c][i] = __float_as_uint(__uint_as_float(sv[c][i]) * sc);
       }
       float mul = pos ? sc : 1.0f;
-      // keys the row does not see become -inf, and so do their fp16 entries, whatever they are (fp32: see below)
-      if (cut) {
-        if (MASK == MASK_ADD) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) raw[i] = hide_entries(raw[i], (uint32_t)(vis >> (8 * i)));
-        }
+      // keys the row does not see become -inf, and so do their fp16 entries, whatever they are
+      auto hide = [&]() {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t half = c ? (uint32_t)(vis >> 32) : (uint32_t)vis;
@@ -402,10 +414,34 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
           for (int i = 0; i < 32; ++i)
             if (!(half & (1u << i))) sv[c][i] = 0xff800000u;
         }
+      };
+      if (cut && !ADD32) {
+        if (MASK == MASK_ADD) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) raw[i] = hide_entries(raw[i], (uint32_t)(vis >> (8 * i)));
+        }
+        hide();
       }
-      if (ADD32) {
+      if (ADD) {
         // the largest entry of a key that the row sees; does it move the reference?
         float top = -INFINITY;
+        if (MASK == MASK_ADD) {
+          top = largest_entry(raw);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float mk[8];
+            load_entries(i, mk);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (!cut || ((vis >> (8 * i + e)) & 1u)) top = fmaxf(top, mk[e]);
+          }
+        }
+        if (Ref::moves(top, ref, m_used)) {
+          m_used = Ref::moved(m_used, ref, Ref::of(top));
+          ref = Ref::of(top);
+        }
+        // scores with their entries (-inf hides the key); from here on as without a mask
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -414,97 +450,48 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
             load_entries(4 * c + i / 8, mk);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (sv[c][i + e] != 0xff800000u) top = fmaxf(top, mk[e]);
+              sv[c][i + e] = __float_as_uint(Ref::score(mk[e], ref, __uint_as_float(sv[c][i + e]) * mul));
           }
-        if (top > -INFINITY && (m_used == -INFINITY || top - ref > AFK_REFERENCE)) {
-          // (a difference beyond fp32 leaves the keys before no weight, but -inf stands for none seen)
-          if (m_used != -INFINITY) m_used = fmaxf(fmaf(ref - top, AFK_LOG2E, m_used), -FLT_MAX);
-          ref = top;
-        }
-        // scores with their entries; from here on as without a mask
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float mk[8];
-            load_entries(4 * c + i / 8, mk);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float s = fabsf(mk[e]) >= AFK_ALONE ? 0.0f : __uint_as_float(sv[c][i + e]) * mul;
-              if (sv[c][i + e] != 0xff800000u) sv[c][i + e] = __float_as_uint(fmaf(mk[e] - ref, AFK_LOG2E, s));
-            }
-          }
+        if (cut && ADD32) hide();
         mul = 1.0f;
       }
-      float mx;
-      if (MASK == MASK_ADD) {
-        // pass 1: -inf mask entries hide their key; the maximum of the masked scores (any value near it will do)
-        mx = -INFINITY;
+      float mxp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float mk[8];
-            mask_entries(raw[4 * c + i / 8], mk);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (mk[e] == -INFINITY) sv[c][i + e] = 0xff800000u;
-              else mx = fmaxf(mx, fmaf(__uint_as_float(sv[c][i + e]), mul, mk[e] * AFK_LOG2E));
-            }
-          }
-        }
-      } else {
-        float mxp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mxp[i & 3] = fmaxf(mxp[i & 3], __uint_as_float(sv[c][i]));
-        mx = fmaxf(fmaxf(mxp[0], mxp[1]), fmaxf(mxp[2], mxp[3])) * mul;
-      }
+        for (int i = 0; i < 32; ++i) mxp[i & 3] = fmaxf(mxp[i & 3], __uint_as_float(sv[c][i]));
+      const float mx = fmaxf(fmaxf(mxp[0], mxp[1]), fmaxf(mxp[2], mxp[3])) * mul;
       float m_new = m_used;
       bool rescale = false;
-      if (mx > m_used + AFK_RESCALE || m_used == -INFINITY) {
+      // (rows of large scores come through here every time)
+      bool stop = !(mx - m_used <= AFK_RESCALE) || large_scores(m_used);
+      if (!(mx - m_used <= AFK_RESCALE) && mx > -INFINITY) {  // (also where there was none before)
         m_new = mx;
         rescale = j > 0 && m_used != -INFINITY;
+      }
+      if (!ADD) stop = __any_sync(0xffffffffu, stop);
+      if (!ADD && stop && __any_sync(0xffffffffu, large_scores(m_new))) {
+        if (pos) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sv[c][i] = __float_as_uint(__uint_as_float(sv[c][i]) * sc);
+        }
+        mul = 1.0f;
       }
       const float alpha = rescale ? ex2_approx(m_used - m_new) : 1.0f;
       const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
       uint32_t pw[2][16];
       float lp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (MASK == MASK_ADD) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float mk[8];
-            mask_entries(raw[4 * c + i / 8], mk);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              // (a hidden key's score is -inf, and its entry)
-              sv[c][i + e] = __float_as_uint(
-                  ex2_approx(fmaf(__uint_as_float(sv[c][i + e]), mul, fmaf(mk[e], AFK_LOG2E, neg_m))));
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e += 2)
-              pw[c][(i + e) >> 1] = pack_f16x2(__uint_as_float(sv[c][i + e]), __uint_as_float(sv[c][i + e + 1]));
-          }
+        for (int i = 0; i < 16; ++i) {
+          const float e0 = ex2_approx(fmaf(__uint_as_float(sv[c][2 * i]), mul, neg_m));
+          const float e1 = ex2_approx(fmaf(__uint_as_float(sv[c][2 * i + 1]), mul, neg_m));
+          pw[c][i] = pack_f16x2(e0, e1);
+          lp[i & 3] = add_f16((uint16_t)(pw[c][i] >> 16), add_f16((uint16_t)pw[c][i], lp[i & 3]));
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            lp[i & 3] = add_f16((uint16_t)(pw[c][i] >> 16), add_f16((uint16_t)pw[c][i], lp[i & 3]));
-      } else {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e0 = ex2_approx(fmaf(__uint_as_float(sv[c][2 * i]), mul, neg_m));
-            const float e1 = ex2_approx(fmaf(__uint_as_float(sv[c][2 * i + 1]), mul, neg_m));
-            pw[c][i] = pack_f16x2(e0, e1);
-            lp[i & 3] = add_f16((uint16_t)(pw[c][i] >> 16), add_f16((uint16_t)pw[c][i], lp[i & 3]));
-          }
-      }
       l = l * alpha + ((lp[0] + lp[1]) + (lp[2] + lp[3]));
       m_used = m_new;
       // P_{j-1} V_{j-1} must be done before P is overwritten and O rescaled
@@ -535,7 +522,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
         *reinterpret_cast<uint4*>(s_p + r * 128 + ((g ^ (r & 7)) << 4)) =
             make_uint4(pw[c][i], pw[c][i + 1], pw[c][i + 2], pw[c][i + 3]);
       }
-      if (MASK == MASK_ADD || ADD32) entries += (ADD32 ? 16 : 8) * p.mask_rows;
+      if (ADD) entries += (ADD32 ? 16 : 8) * p.mask_rows;
       fence_async_shared();  // the generic writes of P become visible to the tensor cores
       tc_fence_before();
       __syncwarp();
@@ -555,7 +542,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
       uint16_t* orow = p.o + (int64_t)w.b * p.o_sb + (int64_t)w.h * p.o_sh + (int64_t)w.t * p.o_st;
       float* prow = part ? p.part_o + slot_row * p.DV : nullptr;
       if (part && live) p.part_ml[slot_row] = make_float2(m_used, l);
-      if (ADD32 && part && live) p.part_ref[slot_row] = ref;
+      if (ADD && part && live) p.part_ref[slot_row] = ref;
       if (!(part && J == 0)) {  // the merge does not read the output of an item with l = 0
 #pragma unroll
         for (int c = 0; c < 2 * NS; ++c) {
@@ -599,8 +586,8 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
 
 // ------------------------------------------------------------------ merging split key ranges
 // One warp per query row, DV / 4 lanes with four columns each; slots in order.
-// REF: maxima are relative to mask references (fp32 additive masks); they are taken to the slots' largest one first.
-template <bool REF>
+// MASK: of additive masks, maxima are relative to mask references; they are taken to the slots' largest one first.
+template <int MASK>
 __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __restrict__ part_o,
                                                                 const float2* __restrict__ part_ml,
                                                                 const float* __restrict__ part_ref, int slots,
@@ -614,6 +601,8 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __r
   if (row >= rows) return;
   // lane s: slot s0 + s; the first 32 slots' (m, l) are loaded once
   const float2 none = make_float2(-INFINITY, 0.0f);
+  constexpr bool REF = MASK == MASK_ADD || MASK == MASK_ADD32;
+  using Ref = MaskReference<MASK == MASK_ADD32>;
   float ref = -INFINITY;
   if (REF) {
     for (int s = lane; s < slots; s += 32)
@@ -623,7 +612,7 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __r
   }
   auto slot_ml = [&](int s) {
     float2 ml = part_ml[(int64_t)s * rows + row];
-    if (REF && ml.y != 0.0f) ml.x = fmaf(part_ref[(int64_t)s * rows + row] - ref, AFK_LOG2E, ml.x);
+    if (REF && ml.y != 0.0f) ml.x += Ref::from(ref, part_ref[(int64_t)s * rows + row]);
     return ml;
   };
   float2 ml = lane < slots ? slot_ml(lane) : none;
@@ -929,7 +918,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
     // (m, l) pairs behind the outputs, mask references behind them, all sized for the compiled batch
     r.part_o = (float*)ptr(8);
     r.part_ml = (float2*)(r.part_o + (int64_t)slots * rows * r.DV);
-    if (variant == MASK_ADD32) r.part_ref = (float*)(r.part_ml + (int64_t)slots * rows);
+    if (additive) r.part_ref = (float*)(r.part_ml + (int64_t)slots * rows);
   }
 
   // ---------------- passes: one kernel for both classes, or the past's first and the own keys' beside it
@@ -999,7 +988,9 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
     ++*launches;
   }
   if (e == cudaSuccess && slots > 1) {
-    e = launch_pdl(r.part_ref ? attention_combine_kernel<true> : attention_combine_kernel<false>,
+    e = launch_pdl(variant == MASK_ADD     ? attention_combine_kernel<MASK_ADD>
+                   : variant == MASK_ADD32 ? attention_combine_kernel<MASK_ADD32>
+                                           : attention_combine_kernel<MASK_NONE>,
                    dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx.stream, (const float*)r.part_o,
                    (const float2*)r.part_ml, (const float*)r.part_ref, slots, rows, (int)tq, r.HQ, r.DV, r.o, r.o_sb, r.o_sh,
                    r.o_st);

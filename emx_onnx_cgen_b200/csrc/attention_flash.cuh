@@ -4,12 +4,19 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 namespace emx {
 
 constexpr float AFK_RESCALE = 8.0f;  // the output is rescaled when a row's maximum grows by more (log2 units)
 constexpr float AFK_LOG2E = 1.4426950408889634f;
+
+// Exponents are score * scale - m in one fused step, m the rounded product of the largest score, so they are off by half
+// a step of m at most, by the same in numerator and sum.  From 2^24 on (a step of 2) a row's scores are scaled, and
+// rounded like m, first: from 2^27 on its largest weight could leave fp16's range either way.
+constexpr float AFK_LARGE = 0x1p24f;
+__device__ __forceinline__ bool large_scores(float m) { return fabsf(m) >= AFK_LARGE && m > -INFINITY; }
 
 enum { MASK_NONE = 0, MASK_BITS = 1, MASK_ADD = 2 /*fp16 entries*/, MASK_ADD32 = 3 };  // kernel variants
 
@@ -40,14 +47,36 @@ __device__ __forceinline__ RowId row_of(int r, const SmallDiv& group, const Smal
   return id;
 }
 
-// fp32 entries may be so large that a score added to them loses its digits, and so far apart that their difference
-// decides alone.  The passes therefore hold a row's running maximum as a pair (mask reference R, maximum m of
-// score + (entry - R)): R is the largest visible entry of some key tile, and moves when a later one is more than
-// AFK_REFERENCE above it, so keys that matter have small differences to it, formed before the score is added.  Partial
-// results carry R beside (m, l).  Entries from 2^56 on leave no digit of a score in 64 bits either: their keys count
-// without it (those at the type's lowest value weigh the same among themselves).
+// An entry of an additive mask may be so large that a score added to it loses its digits, and entries so far apart that
+// their difference decides alone.  The passes therefore hold a row's running maximum as a pair (mask reference R,
+// maximum m of score + (entry - R)): R is the largest visible entry of some key tile, and moves when a later one is
+// more than AFK_REFERENCE above it, so keys that matter have small differences to it, formed before the score is added.
+// Partial results carry R beside (m, l).  fp32 entries from 2^56 on leave no digit of a score in 64 bits either: their
+// keys count without it (those at the type's lowest value weigh the same among themselves).
 constexpr float AFK_ALONE = 0x1p56f;
 constexpr float AFK_REFERENCE = 16.0f;
+
+// R is held in log2 units for fp16 entries, as the entry itself for fp32 ones (whose product may leave the range).
+template <bool F32>
+struct MaskReference {
+  static __device__ __forceinline__ float of(float entry) { return F32 ? entry : entry * AFK_LOG2E; }
+  // log2 units from reference r to reference (or entry) to
+  static __device__ __forceinline__ float from(float r, float to) { return F32 ? (to - r) * AFK_LOG2E : to - r; }
+  // score (log2 units) with its key's entry; -inf hides the key whatever its score is
+  static __device__ __forceinline__ float score(float entry, float r, float s) {
+    if (F32) return fmaf(entry - r, AFK_LOG2E, fabsf(entry) >= AFK_ALONE ? 0.0f : s);
+    return entry == -INFINITY ? -INFINITY : s + fmaf(entry, AFK_LOG2E, -r);
+  }
+  // whether a largest visible entry moves the reference of a row with maximum m (-inf: it has none yet)
+  static __device__ __forceinline__ bool moves(float entry, float r, float m) {
+    return entry > -INFINITY && (m == -INFINITY || from(r, of(entry)) > AFK_REFERENCE);
+  }
+  // the maximum m under the new reference (a difference beyond fp32 leaves the keys before no weight, but -inf stands
+  // for none seen)
+  static __device__ __forceinline__ float moved(float m, float r, float to) {
+    return m == -INFINITY ? m : fmaxf(m - from(r, to), -FLT_MAX);
+  }
+};
 
 // The work items of a pass come in two classes: 0, the rows of one sequence
 // against its own keys (behind its past where `past` is set: one list of key
@@ -77,7 +106,7 @@ struct TileParams {
   uint16_t* o;
   float* part_o;    // [slot][row][DV], null: one item per row, written to o
   float2* part_ml;  // [slot][row] (m, l)
-  float* part_ref;  // [slot][row] mask references, fp32 additive masks only
+  float* part_ref;  // [slot][row] mask references, additive masks only
   int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
   int B, HQ, HKV, D, DV, causal, tk, tp, past_shared;
   SmallDiv group, TQ;

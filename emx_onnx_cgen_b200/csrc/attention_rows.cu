@@ -37,7 +37,6 @@
 // visible key are not read (but for the first copies, which are on their way by
 // then), and values behind that key take no part.
 #include <cuda_fp16.h>
-#include <float.h>
 
 #include "attention_flash.cuh"
 #include "host_util.h"
@@ -96,11 +95,12 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   constexpr int ST = AR_RING / STAGE;             // 3 steps, or 6 at NS = 1, NT = 2
   constexpr int OW = 64 * NS + 4;                 // padded row of the merge buffer
   constexpr bool ADD = MASK == MASK_ADD || MASK == MASK_ADD32, ADD32 = MASK == MASK_ADD32;
+  using Ref = MaskReference<ADD32>;
   extern __shared__ __align__(128) uint8_t s_all[];  // rows_smem() bytes
   __shared__ uint32_t s_bits[MASK == MASK_BITS ? 8 * NT * AF_ROWS_MASK_KEYS / 32 : 1];  // [row][32 keys]
   __shared__ int s_range[2];
   __shared__ float2 s_row[8 * NT];
-  __shared__ float s_ref[ADD32 ? 8 * NT : 1];
+  __shared__ float s_ref[ADD ? 8 * NT : 1];
   const int warps = blockDim.x >> 5;
   float(*s_o)[8 * NT][OW] = reinterpret_cast<float(*)[8 * NT][OW]>(s_all);  // once the ring is done with
   float(*s_m)[8 * NT] = reinterpret_cast<float(*)[8 * NT]>(s_all + (size_t)warps * 8 * NT * OW * 4);
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   };
 
   float o[NT][NS][4][4];  // O^T: [row tile][slab][d pair][(d, row), (d, row + 1), (d + 1, row), (d + 1, row + 1)]
-  float m_ref[NT][2], l[NT][2], ref[NT][2];  // ref: mask references (fp32 entries)
+  float m_ref[NT][2], l[NT][2], ref[NT][2];  // ref: mask references
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
             bool ok = pos < min(lim[n2][e], seg_end) && ((bits >> (8 * h + g)) & 1u);
             if (ADD) {
               ok = ok && mk[u][i] != -INFINITY;
-              if (!ok) mk[u][i] = ADD32 ? -INFINITY : 0.0f;
+              if (!ok) mk[u][i] = -INFINITY;
             }
             if (!ok) see &= ~(1u << (4 * NT * u + i));
           }
@@ -372,10 +372,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
           mma_16816(s2, k[u][0][c].z, k[u][1][c].z, k[u][0][c].w, k[u][1][c].w, q[n2][c].z, q[n2][c].w);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[u][n2][e] = (s[u][n2][e] + s2[e]) * sc;
-          if (ADD32 && fabsf(mk[u][((e >> 1) * NT + n2) * 2 + (e & 1)]) >= AFK_ALONE) s[u][n2][e] = 0.0f;
-        }
+        for (int e = 0; e < 4; ++e) s[u][n2][e] = (s[u][n2][e] + s2[e]) * sc;
       }
     // V in K's registers, on its way during the softmax
     uint4 v[U][NS][4];
@@ -414,8 +411,8 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
           for (int e = 0; e < 4; ++e)
             if (!((see >> (4 * NT * u + ((e >> 1) * NT + n2) * 2 + (e & 1))) & 1u)) s[u][n2][e] = -INFINITY;
     }
-    // fp32 entries: the largest of a row's visible keys may move its reference; then they join the scores
-    if (ADD32) {
+    // the largest entry of a row's visible keys may move its mask reference; then the entries join the scores
+    if (ADD) {
       float most[NT][2];
       bool move = false;
 #pragma unroll
@@ -427,7 +424,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
           for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) most[n2][e] = fmaxf(most[n2][e], mk[u][(h * NT + n2) * 2 + e]);
-          move = move || (most[n2][e] > -INFINITY && (m_ref[n2][e] == -INFINITY || most[n2][e] - ref[n2][e] > AFK_REFERENCE));
+          move = move || Ref::moves(most[n2][e], ref[n2][e], m_ref[n2][e]);
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -437,10 +434,9 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
             float x = most[n2][e];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            if (x > -INFINITY && (m_ref[n2][e] == -INFINITY || x - ref[n2][e] > AFK_REFERENCE)) {
-              // (a difference beyond fp32 leaves the keys before no weight, but -inf stands for none seen)
-              if (m_ref[n2][e] != -INFINITY) m_ref[n2][e] = fmaxf(fmaf(ref[n2][e] - x, AFK_LOG2E, m_ref[n2][e]), -FLT_MAX);
-              ref[n2][e] = x;
+            if (Ref::moves(x, ref[n2][e], m_ref[n2][e])) {
+              m_ref[n2][e] = Ref::moved(m_ref[n2][e], ref[n2][e], Ref::of(x));
+              ref[n2][e] = Ref::of(x);
             }
           }
       }
@@ -450,7 +446,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
         for (int n2 = 0; n2 < NT; ++n2)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            s[u][n2][e] = fmaf(mk[u][((e >> 1) * NT + n2) * 2 + (e & 1)] - ref[n2][e & 1], AFK_LOG2E, s[u][n2][e]);
+            s[u][n2][e] = Ref::score(mk[u][((e >> 1) * NT + n2) * 2 + (e & 1)], ref[n2][e & 1], s[u][n2][e]);
     }
     bool grow = false;
     float top[NT][2];
@@ -461,16 +457,10 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
         if (n2 == 1 && !two) continue;
         float x = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float x0 = s[u][n2][e], x1 = s[u][n2][2 + e];
-          if (MASK == MASK_ADD) {
-            x0 = fmaf(mk[u][n2 * 2 + e], AFK_LOG2E, x0);
-            x1 = fmaf(mk[u][(NT + n2) * 2 + e], AFK_LOG2E, x1);
-          }
-          x = fmaxf(x, fmaxf(x0, x1));
-        }
+        for (int u = 0; u < U; ++u)
+          x = fmaxf(x, fmaxf(s[u][n2][e], s[u][n2][2 + e]));
         top[n2][e] = x;
-        grow = grow || x > m_ref[n2][e] + AFK_RESCALE || (m_ref[n2][e] == -INFINITY && x > -INFINITY);
+        grow = grow || x - m_ref[n2][e] > AFK_RESCALE;  // (or the first one: inf > 8)
       }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -482,7 +472,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
           const float old = m_ref[n2][e];
-          if (x > old + AFK_RESCALE || old == -INFINITY) {
+          if (x - old > AFK_RESCALE || old == -INFINITY) {
             m_ref[n2][e] = x;
             const float alpha = old == -INFINITY ? 0.0f : ex2_approx(old - x);
             l[n2][e] *= alpha;
@@ -508,9 +498,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
           const float neg = m_ref[n2][e] == -INFINITY ? 0.0f : -m_ref[n2][e];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float off = neg;
-            if (MASK == MASK_ADD) off = fmaf(mk[u][(h * NT + n2) * 2 + e], AFK_LOG2E, neg);
-            s[u][n2][2 * h + e] = ex2_approx(s[u][n2][2 * h + e] + off);
+            s[u][n2][2 * h + e] = ex2_approx(s[u][n2][2 * h + e] + neg);
             l[n2][e] += s[u][n2][2 * h + e];
           }
         }
@@ -549,7 +537,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
       if (g == 0) {
         s_m[warp][r] = m_ref[n][e];
         s_l[warp][r] = l[n][e];
-        if (ADD32) s_r[warp][r] = ref[n][e];
+        if (ADD) s_r[warp][r] = ref[n][e];
       }
       if (!any_block) continue;  // l = 0: nothing reads this warp's output
 #pragma unroll
@@ -569,12 +557,12 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
         const bool in = w < warps && rr < rows;
         const float lw = in ? s_l[w][rr] : 0.0f;
         float mw = in && lw != 0.0f ? s_m[w][rr] : -INFINITY;
-        if (ADD32) {  // maxima relative to the warps' largest reference
+        if (ADD) {  // maxima relative to the warps' largest reference
           const float rw = in && lw != 0.0f ? s_r[w][rr] : -INFINITY;
           float most = rw;
 #pragma unroll
           for (int d = 4; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d, 8));
-          if (in && lw != 0.0f) mw = fmaf(rw - most, AFK_LOG2E, mw);
+          if (in && lw != 0.0f) mw += Ref::from(most, rw);
           if (w == 0 && rr < rows) s_ref[rr] = most;
         }
         float m = mw, sum;
@@ -607,7 +595,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
     if (p.part_o) {
       const int64_t at = (int64_t)(cl.part0 + split) * ((int64_t)p.B * (int)p.TQ.d * p.HQ) + ((int64_t)w.b * (int)p.TQ.d + w.t) * p.HQ + w.h;
       if (d == 0) p.part_ml[at] = ms;
-      if (ADD32 && d == 0) p.part_ref[at] = s_ref[r];
+      if (ADD && d == 0) p.part_ref[at] = s_ref[r];
       *reinterpret_cast<float4*>(p.part_o + at * p.DV + d) = acc;
     } else {
       const float inv = ms.y == 0.0f ? 0.0f : 1.0f / ms.y;

@@ -456,7 +456,6 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
     const float sc = p.scale_log2;
     const bool pos = sc > 0.0f;
     const float mul = pos ? sc : 1.0f;
-    const F2 mul2v(mul, mul);
     int nt = 0, nitems = 0;  // key tiles, items of this row tile so far
     int id = blockIdx.x;
     WideItem w = {};
@@ -470,6 +469,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
       const RowId row = row_of(w.row0 + (live ? r : 0), p.group, p.TQ, w.kvh, w.b, w.shared);
       float m_used = -INFINITY;  // reference of the exponentials, log2 units
       float l = 0.0f;
+      F2 mul2v(mul, mul);
       const int J = mine ? k.J : 0;
       if (J > 0) {
         const int np = cl.past ? (p.tp + AW_N - 1) / AW_N : 0;
@@ -536,20 +536,32 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
                                    max_nan(max_nan(mxp[4], mxp[5]), max_nan(mxp[6], mxp[7]))) * mul;
           bool rescale = false;
           float alpha = 1.0f;
-          if (!(mx <= m_used + AFK_RESCALE) || m_used == -INFINITY) {
+          // (rows of large scores come through here every time)
+          const bool stop = !(mx - m_used <= AFK_RESCALE) || large_scores(m_used);
+          if (!(mx - m_used <= AFK_RESCALE)) {  // (also where there was none before)
             rescale = j > 0 && m_used != -INFINITY;
             if (rescale) alpha = ex2_approx(m_used - mx);
             m_used = mx == INFINITY ? NAN : mx;
           }
-          if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll 1
-            for (int q = 0; q < 4 * NS; ++q) {
-              uint32_t o[16];
-              tmem_ld16(o_col + 16u * q, o);
-              tmem_wait_ld();
+          if (__any_sync(0xffffffffu, stop)) {
+            const bool large = __any_sync(0xffffffffu, large_scores(m_used));
+            mul2v = large ? F2(1.0f, 1.0f) : F2(mul, mul);
+            if (large && pos) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st16(o_col + 16u * q, o);
+              for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sv[q][i] = __float_as_uint(__uint_as_float(sv[q][i]) * sc);
+            }
+            if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+              for (int q = 0; q < 4 * NS; ++q) {
+                uint32_t o[16];
+                tmem_ld16(o_col + 16u * q, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st16(o_col + 16u * q, o);
+              }
             }
           }
           const float neg_m = m_used == -INFINITY ? 0.0f : -m_used;

@@ -101,7 +101,7 @@ enum {
 enum { ATF_SCALE };
 
 // ---- K_ATTENTION_FLASH: t[0]=Q, t[1]=K, t[2]=V, t[3]=Y (fp16), t[4]=mask|-1, t[5]=past K|-1, t[6]=past V|-1,
-//      t[7]=valid key counts i64 [B]|-1, t[8]=partial results f32|-1 (slots x rows x (DV + 2, or 3 with an fp32 mask), slots = AF_SPLITS_K +
+//      t[7]=valid key counts i64 [B]|-1, t[8]=partial results f32|-1 (slots x rows x (DV + 2, or 3 with an additive mask), slots = AF_SPLITS_K +
 //      AF_SPLITS_P, rows = B*TQ*HQ), t[9]=boolean mask as bits (16 bytes per mask row, then 8 per 64 keys of the past
 //      and of the current keys, each rounded up to 128), or additive mask in tiles of 64 keys (past first)|-1: for the tile passes.  Element (b, h, t, d) of Q, K, V, Y sits at b*SB + h*SH + t*ST + d; the past is contiguous
 //      [B or 1][HKV][TP][D].  Mask row of query (b, h, t): b*SB + h*SH + t*ST, each of AF_MASK_LEN keys, past first.

@@ -1618,8 +1618,8 @@ class B200PlanEmitter:
         ip.update({K.AF_PASS_OWN: sch.own, K.AF_PASS_PAST: sch.past, K.AF_SPLITS_K: sch.splits_own,
                    K.AF_SPLITS_P: sch.splits_past, K.AF_WARPS: sch.warps})
         if sch.slots > 1:
-            # output, maximum and sum of a row, and with an fp32 mask its reference
-            t_part = self._b.arena_tensor(T_TEMP, "f32", (sch.slots, b * tq * hq, dv + 2 + (t_mask >= 0 and kind == K.AF_MASK_F32)),
+            # output, maximum and sum of a row, and with an additive mask its reference
+            t_part = self._b.arena_tensor(T_TEMP, "f32", (sch.slots, b * tq * hq, dv + 2 + (t_mask >= 0 and kind != K.AF_MASK_BOOL)),
                                           name="attention:partials")
         if t_mask >= 0 and not {K.AF_PASS_TILES, K.AF_PASS_WIDE}.isdisjoint((sch.own, sch.past)):
             if kind == K.AF_MASK_BOOL:

@@ -100,3 +100,61 @@ def test_large_additive_entries_keep_their_order(kw):
                 row = np.sort(row)[::-1]
             m[i, 0, q] = row
     check(run(wl, x), *decoder_attention(wl, x), str(kw))
+
+
+@pytest.mark.parametrize("mask", ["none", "bool", "f16", "f32"])
+@pytest.mark.parametrize("scale", [0.125, -0.125, 0.5])
+@pytest.mark.parametrize("kw", [
+    dict(q_seq=1, kv_seq=300), dict(q_seq=9, kv_seq=300, head_dim=128), dict(q_seq=40, kv_seq=300),
+    dict(q_seq=40, kv_seq=300, head_dim=128), dict(q_seq=300, kv_seq=300), dict(q_seq=300, kv_seq=300, head_dim=128),
+    dict(q_seq=1, kv_seq=3000), dict(q_seq=2, kv_seq=60, past=240),
+])
+def test_scores_far_apart_pick_one_key(kw, scale, mask):
+    """Scores of 2^17 to 2^33, further apart than any rounding of them: all the weight is on the largest, and its value
+    comes out, within half a step for the weight (a pass may round it for the product but not for the sum) and half a
+    step for the result."""
+    require_gpu()
+    past = kw.get("past", 0)
+    t = kw["kv_seq"] + past
+    kw = dict(batch=2, q_heads=2, kv_heads=2, scale=scale, **kw)
+    if mask != "none":
+        kw.update(mask=mask, mask_shape=(2, 1, kw["q_seq"], t))
+    wl = W.decoder_attention(**kw)
+    x = wl.make_inputs(35)
+    if mask == "bool":
+        x["mask"][:] = True
+    r = np.random.default_rng(8)
+    for size in (37.0, 8192.0, 60000.0):
+        x["Q"][:] = size
+        # D times whole numbers, each key its own: scores are at least size * D * |scale| apart
+        level = np.stack([r.permutation(2047)[:t] - 1023 if t < 2000 else r.permutation(t) - t // 2 for _ in range(4)]).reshape(2, 2, t).astype(np.float16)
+        if past:
+            level[1, :, :past] = level[0, :, :past]
+            x["PK"][:] = level[:1, :, :past, None]
+        x["K"][:] = level[:, :, past:, None]
+        top = np.sort(level if scale > 0 else -level, axis=2)
+        assert (top[..., -1] > top[..., -2]).all()
+        best = level.argmax(2) if scale > 0 else level.argmin(2)
+        got = run(wl, x)
+        for b in range(2):
+            for h in range(2):
+                k = best[b, h]
+                want = x["PV"][0, h, k] if k < past else x["V"][b, h, k - past]
+                want = np.broadcast_to(want, got[b, h].shape).astype(np.float64)
+                check(got[b, h], want, (2.0 ** -10 + 2.0 ** -20) * np.abs(want) + 2.0 ** -25, f"{size} {b} {h}")
+
+
+@pytest.mark.parametrize("mask", ["f16", "f32"])
+@pytest.mark.parametrize("q_seq", [1, 9, 40, 150])
+def test_scores_of_keys_hidden_by_an_entry(q_seq, mask):
+    """-inf hides its key whatever the key's score is, beside entries of any size."""
+    require_gpu()
+    kw = dict(batch=2, q_heads=2, kv_heads=2, q_seq=q_seq, kv_seq=260, mask=mask, mask_shape=(2, 1, q_seq, 260))
+    wl = W.decoder_attention(**kw)
+    x = wl.make_inputs(38)
+    hidden = [0, 3, 70, 128, 259]
+    x["mask"][1] -= 60000 if mask == "f16" else np.float32(1e9)
+    x["mask"][..., hidden] = -np.inf
+    want = decoder_attention(wl, x)
+    x["K"][:, :, hidden] = np.array([np.inf, np.nan, -np.inf, np.nan, np.inf], np.float16)[:, None]
+    check(run(wl, x), *want, str(kw))
