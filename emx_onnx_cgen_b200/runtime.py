@@ -123,9 +123,10 @@ class Session:
     def run_ptrs(self, in_ptrs, out_ptrs, batch_begin: int = 0, batch_count: int = -1, stream: int = 0) -> None:
         # the session's own arrays, written whole each call (making new ones took a microsecond of it)
         ins, outs = self._ins, self._outs
-        if len(in_ptrs) < len(ins) or len(out_ptrs) < len(outs):
+        # (a surplus input would shift those behind it onto other tensors; outputs past the plan's are left alone)
+        if len(in_ptrs) != len(ins) or len(out_ptrs) < len(outs):
             raise ValueError(f"{len(in_ptrs)} input and {len(out_ptrs)} output pointers, plan has {len(ins)} and {len(outs)}")
-        ins[:], outs[:] = in_ptrs[:len(ins)], out_ptrs[:len(outs)]
+        ins[:], outs[:] = in_ptrs, out_ptrs[:len(outs)]
         status = self._run(self.handle, ins, outs, batch_begin, batch_count, stream or None)
         if status != EMX_OK:
             _check(status)
