@@ -793,7 +793,7 @@ int prepare_attention_flash(const PlanOp& op, void* const*, OpState*, int, char*
 static int make_tmap_kv(CUtensorMap* map, const void* base, int64_t d, int64_t t, int64_t heads, int64_t batch,
                         int64_t st, int64_t sh, int64_t sb, int tile_keys) {
   EncodeTiledFn enc = encode_tiled_fn();
-  if (!enc || ((uintptr_t)base & 15u)) return 5;
+  if (!enc) return 4;
   cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)t, (cuuint64_t)heads, (cuuint64_t)batch};
   cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
   cuuint32_t box[4] = {64, (cuuint32_t)tile_keys, 1, 1};
@@ -877,8 +877,8 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
   r.err = ctx.d_error;
   if (r.B <= 0 || tq <= 0) return 0;
   for (int i : {0, 1, 2, 3, 5, 6})
-    if ((uintptr_t)ptr(i) & 15u) return 5;
-  if ((uintptr_t)r.counts & 7u) return 5;
+    if ((uintptr_t)ptr(i) & 15u) return REFUSED_ALIGNMENT;
+  if ((uintptr_t)r.counts & 7u) return REFUSED_ALIGNMENT;
   const int kind = (int)op.ip[AF_MASK_KIND];
   const int variant = kind == AF_MASK_NONE ? MASK_NONE : kind == AF_MASK_BOOL ? MASK_BITS : kind == AF_MASK_F16 ? MASK_ADD : MASK_ADD32;
   const bool additive = variant == MASK_ADD || variant == MASK_ADD32;
@@ -886,7 +886,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
   r.mask_len = (int)op.ip[AF_MASK_LEN];
   r.mask_bool = variant == MASK_BITS ? (const uint8_t*)ptr(4) : nullptr;
   r.mask_add = additive ? ptr(4) : nullptr;
-  if (additive && ((uintptr_t)r.mask_add & (variant == MASK_ADD32 ? 3u : 1u))) return 5;
+  if (additive && ((uintptr_t)r.mask_add & (variant == MASK_ADD32 ? 3u : 1u))) return REFUSED_ALIGNMENT;
 
   // ---------------- work items of the two classes
   const int64_t rows = (int64_t)r.B * tq * r.HQ;
@@ -913,7 +913,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
   // (SmallDiv: rows divided by the group, and, against a shared past, by the tokens)
   if (items[0] + items[1] > 0x7fffffff || (apart ? r.B : 1) * tq * group * group > 0xffffffffll ||
       (apart && r.B * tq * tq > 0xffffffffll))
-    return 5;
+    return REFUSED_SIZE;
   if (slots > 1) {
     // (m, l) pairs behind the outputs, mask references behind them, all sized for the compiled batch
     r.part_o = (float*)ptr(8);
@@ -944,7 +944,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
         // (an absent class divides by 1)
         r.by[c][0] = SmallDiv::of(cls[c].splits ? cls[c].splits : 1), r.by[c][1] = SmallDiv::of(cls[c].tiles ? cls[c].tiles : 1);
         const int64_t largest = std::max<int64_t>(std::max(cls[c].splits, cls[c].tiles), r.HKV);
-        if (std::max<int64_t>(n0 + n1, most_keys(r.tp, r.tk, 1)) * largest > 0xffffffffll) return 5;
+        if (std::max<int64_t>(n0 + n1, most_keys(r.tp, r.tk, 1)) * largest > 0xffffffffll) return REFUSED_SIZE;
       }
       r.by_hkv = SmallDiv::of(r.HKV);
       r.late_wait = !together && step == 1;

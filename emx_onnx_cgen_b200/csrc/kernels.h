@@ -217,6 +217,12 @@ enum FaultHook : int {
   FAULT_DROP_KEY_TILES = 2,       // attention_flash.cu, attention_wide.cu: a CTA's producer stops after its first key tile
 };
 
+// What a launch may return beside the C API's codes: both are reported as EMX_ERR_UNSUPPORTED, with their reason.
+enum LaunchRefusal : int {
+  REFUSED_ALIGNMENT = 101,  // a buffer of this run starts off the boundary the kernel needs
+  REFUSED_SIZE = 102,       // more work than one launch can index
+};
+
 // Last integer slot of every op: 1 when the op's leading (batch) extent
 // follows the run's batch slice.  The plan emitter sets it only on ops whose
 // leading extent is the plan batch, and marks a plan sliceable only if every

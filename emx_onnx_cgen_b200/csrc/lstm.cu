@@ -472,7 +472,7 @@ int launch_lstm_f32(const PlanOp& op, void* const* ptrs, const OpState*, const L
   float* y_h = op.t[8] >= 0 ? (float*)ptrs[op.t[8]] : nullptr;
   float* y_c = op.t[9] >= 0 ? (float*)ptrs[op.t[9]] : nullptr;
   if (((uintptr_t)x | (uintptr_t)wp | (uintptr_t)rp | (uintptr_t)bsum | (uintptr_t)gx | (uintptr_t)hbuf) & 15u)
-    return 5;  // 16-byte aligned rows (the plan places every tensor on 256 bytes; a caller's X must be too)
+    return REFUSED_ALIGNMENT;  // 16-byte aligned rows (the plan places every tensor on 256 bytes; a caller's X must be too)
   const int hp = (H + LS_TILE_UNITS - 1) / LS_TILE_UNITS * LS_TILE_UNITS;
   const int N = 4 * hp;
   const int64_t bh = (int64_t)B * H;

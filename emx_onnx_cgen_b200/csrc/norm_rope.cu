@@ -436,7 +436,7 @@ static int launch_rope_t(const RopeParams& p, int items, const LaunchCtx& ctx, i
     bases |= (uintptr_t)it.x | (uintptr_t)it.y | (uintptr_t)it.scale;
     vec = vec && (it.x_sb % V | it.x_st % V | it.x_sh % V | it.y_sb % V | it.y_st % V | it.y_sh % V) == 0;
   }
-  if ((bases & (sizeof(T) - 1)) != 0 || ((uintptr_t)p.pos & 7u) != 0) return 5;
+  if ((bases & (sizeof(T) - 1)) != 0 || ((uintptr_t)p.pos & 7u) != 0) return REFUSED_ALIGNMENT;
   vec = vec && (bases & 15u) == 0;
   cudaError_t e;
   if (vec) {
@@ -447,9 +447,10 @@ static int launch_rope_t(const RopeParams& p, int items, const LaunchCtx& ctx, i
     else e = launch_vec<T, 32>(p, ctx);
   } else {
     const int64_t blocks = (p.tokens * p.heads + 7) / 8;
-    if (blocks > 0x7fffffff) return 5;
+    if (blocks > 0x7fffffff) return REFUSED_SIZE;
     e = launch_pdl(norm_rope_any_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, ctx.stream, p);
   }
+  if (e == cudaErrorInvalidConfiguration) return REFUSED_SIZE;  // (launch_vec_rows)
   ++*launches;
   return e == cudaSuccess ? 0 : 4;
 }
@@ -548,11 +549,11 @@ __global__ void __launch_bounds__(256) rms_norm_kernel(const T* __restrict__ x, 
 template <typename T>
 static int launch_rms_t(const void* x, const void* scale, void* y, int64_t rows, int64_t n, float eps,
                         const LaunchCtx& ctx, int* launches) {
-  if (((uintptr_t)x | (uintptr_t)scale | (uintptr_t)y) & (sizeof(T) - 1)) return 5;
+  if (((uintptr_t)x | (uintptr_t)scale | (uintptr_t)y) & (sizeof(T) - 1)) return REFUSED_ALIGNMENT;
   const bool vec = n % Chunk<T>::N == 0 && (((uintptr_t)x | (uintptr_t)scale | (uintptr_t)y) & 15u) == 0;
   const bool wide = n > 1024;
   const int64_t blocks = wide ? rows : (rows + 7) / 8;
-  if (blocks > 0x7fffffff) return 5;
+  if (blocks > 0x7fffffff) return REFUSED_SIZE;
   auto kernel = wide ? (vec ? rms_norm_kernel<T, 8, true> : rms_norm_kernel<T, 8, false>)
                      : (vec ? rms_norm_kernel<T, 1, true> : rms_norm_kernel<T, 1, false>);
   cudaError_t e = launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), 0, ctx.stream, (const T*)x, (const T*)scale,

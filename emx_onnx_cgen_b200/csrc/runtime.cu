@@ -299,9 +299,14 @@ int launch_ops(emx_plan* p, int64_t run_batch, cudaStream_t stream, int* launche
     if (rc) {
       if (p->profiling) *(volatile int*)p->h_hold = seq;
       cudaError_t e = cudaGetLastError();
+      if (rc == emx::REFUSED_ALIGNMENT)
+        return set_error(EMX_ERR_UNSUPPORTED, "op %zu (%s): a buffer of this run does not start on the boundary the kernel "
+                         "needs (16 bytes; masks and norm or rotation operands their element, counts and positions 8)", i,
+                         p->entries[i]->name);
+      if (rc == emx::REFUSED_SIZE)
+        return set_error(EMX_ERR_UNSUPPORTED, "op %zu (%s): this run is too large for one launch", i, p->entries[i]->name);
       if (rc == EMX_ERR_UNSUPPORTED)
-        return set_error(rc, "op %zu (%s): a buffer of this run does not start on the boundary the kernel needs (16 bytes), "
-                         "or the run is too large for one launch", i, p->entries[i]->name);
+        return set_error(rc, "op %zu (%s): the kernel cannot run this batch range, size or device", i, p->entries[i]->name);
       return set_error(rc == EMX_ERR_CUDA ? EMX_ERR_CUDA : rc, "op %zu (%s) launch failed: %s", i,
                        p->entries[i]->name, cudaGetErrorString(e));
     }
