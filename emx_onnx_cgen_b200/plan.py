@@ -269,6 +269,7 @@ def lstm_persistent_fits(b: int, isz: int, h: int, sms: int) -> bool:
 
 
 FLASH_ROWS, FLASH_KEYS = 128, 64   # query rows and keys of a tile of attention_flash.cu
+INDEX_LIMIT = 2 ** 31 - 1024       # rows, keys and tokens that the decoder operators' kernels number in 32 bits
 
 
 def flash_splits(items_tiles, resident: int, least: int) -> list[int]:
@@ -1505,6 +1506,8 @@ class B200PlanEmitter:
         group = self._rotary[i]
         op = group[0]["op"]
         b, t, d, rot = group[0]["b"], group[0]["t"], group[0]["d"], int(op.rotary_dim)
+        if t > INDEX_LIMIT:
+            raise UnsupportedOpError(f"RotaryEmbedding of {t} tokens has no B200 kernel")
         if rot < 2 or rot % 2 or rot > d:
             raise UnsupportedOpError(f"RotaryEmbedding: {rot} rotated elements of a head size of {d}")
         tables = tuple(int(v) for v in self._shape(op.cos_cache))
@@ -1579,6 +1582,9 @@ class B200PlanEmitter:
             return "nonpad_kv_seqlen that is not int64"
         if op.input_attn_mask and self._dtype(op.input_attn_mask) not in ("bool", "f16", "f32"):
             return f"a {self._dtype(op.input_attn_mask)} mask"
+        b, tq, group = int(op.batch), int(op.q_seq), int(op.q_heads) // int(op.kv_heads)
+        if max(b * tq * group, int(op.total_seq)) > INDEX_LIMIT:  # row and key numbers of the kernels
+            return f"{b * tq * group} query rows of a key/value head, or {int(op.total_seq)} keys (up to {INDEX_LIMIT}),"
         return None
 
     def _emit_attention_flash(self, i, op):

@@ -343,3 +343,21 @@ def test_one_expand_for_two_attentions():
     plan = plan_of(wl)
     assert sorted(o.kernel for o in plan.ops) == sorted([K.K_TRANSPOSE] + [K.K_ATTENTION_FLASH] * 2)
     assert all(o.ip[K.AF_PAST_SHARED] == 1 for o in plan.ops if o.kernel == K.K_ATTENTION_FLASH)
+
+
+def test_more_rows_or_keys_than_the_kernels_number():
+    """Row, key and token numbers are 32-bit in the kernels: larger plans are refused, whatever the memory."""
+    big = 2 ** 31
+    for kw in (dict(batch=1, q_heads=1, kv_heads=1, q_seq=big, kv_seq=8, head_dim=8),
+               dict(batch=2, q_heads=2, kv_heads=1, q_seq=big // 4, kv_seq=8, head_dim=8),
+               dict(batch=1, q_heads=1, kv_heads=1, q_seq=1, kv_seq=big, head_dim=8),
+               dict(batch=1, q_heads=1, kv_heads=1, q_seq=1, kv_seq=big // 2, past=big // 2, head_dim=8)):
+        with pytest.raises(UnsupportedOpError, match="no B200 kernel"):
+            plan_of(W.decoder_attention(**kw))
+    x = TensorSpec("X", "f16", (1, 1, big, 8))
+    g = GraphSpec("r", [x, TensorSpec("pos", "i64", (1, big))], [TensorSpec("Y", "f16", x.shape)],
+                  [NodeSpec("RotaryEmbedding", "r", ("X", "cos", "sin", "pos"), ("Y",), {})],
+                  {n: np.zeros((4, 4), np.float16) for n in ("cos", "sin")})
+    with pytest.raises(UnsupportedOpError, match="tokens"):
+        plan_of(g)
+    assert plan_of(W.decoder_attention(batch=1, q_heads=1, kv_heads=1, q_seq=1, kv_seq=2 ** 20, head_dim=8)).ops
