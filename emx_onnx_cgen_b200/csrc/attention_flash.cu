@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(AFK_THREADS, 2) attention_flash_kernel(const _
     tmem_relinquish();
   }
   pdl_wait();  // Q, K, V, masks and counts may come from the preceding kernel
+  if (p.publish && blockIdx.x == 0 && threadIdx.x == 0) publish_waited(p.err, 1);
   pdl_launch_dependents();
 
   // ---------------- Q tile, zero past the head size and the rows
@@ -593,8 +594,9 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const float* __r
                                                                 const float* __restrict__ part_ref, int slots,
                                                                 int64_t rows, int TQ, int HQ, int DV,
                                                                 uint16_t* __restrict__ o, int64_t o_sb, int64_t o_sh,
-                                                                int64_t o_st) {
+                                                                int64_t o_st, int* published /*or null*/) {
   pdl_wait();
+  if (published && blockIdx.x == 0 && threadIdx.x == 0) publish_waited(published, 0);
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -954,6 +956,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
       const int tile_keys = pass == AF_PASS_WIDE ? 128 : AFK_N;
       if (pass == AF_PASS_WIDE && additive) return 5;  // (never planned)
       int rc = tile_params(p, r, cls, (int)n1, (int)(n0 + n1), tile_keys);
+      p.publish = !together;
       p.drop_keys = (ctx.fault & FAULT_DROP_KEY_TILES) != 0;
       if (rc) return rc;
       const int64_t mrows = p.mask_sb ? p.mask_sb * p.B : op.ip[AF_MASK_ROWS];
@@ -993,7 +996,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
                                            : attention_combine_kernel<MASK_NONE>,
                    dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx.stream, (const float*)r.part_o,
                    (const float2*)r.part_ml, (const float*)r.part_ref, slots, rows, (int)tq, r.HQ, r.DV, r.o, r.o_sb, r.o_sh,
-                   r.o_st);
+                   r.o_st, together ? nullptr : r.err);
     ++*launches;
   }
   return e == cudaSuccess ? 0 : 4;

@@ -120,6 +120,7 @@ struct TileParams {
   int64_t mask_rows;
   int words, words_past, mask_len;
   float scale_log2;
+  int publish;    // the own keys' few-row pass runs beside this one: tell it when this one has waited (publish_waited)
   int drop_keys;  // failure-detection test hook (FAULT_DROP_KEY_TILES)
   int* err;
 };
@@ -142,7 +143,7 @@ struct RowsParams {
   const void* mask_add;
   int mask_len;
   float scale_log2;
-  int late_wait;  // launched behind a pass whose results it does not read
+  int late_wait;  // launched beside a tile pass (publish) whose results it does not read
   int* err;
 };
 

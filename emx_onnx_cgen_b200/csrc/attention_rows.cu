@@ -106,7 +106,9 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
   float(*s_m)[8 * NT] = reinterpret_cast<float(*)[8 * NT]>(s_all + (size_t)warps * 8 * NT * OW * 4);
   float(*s_l)[8 * NT] = s_m + warps, (*s_r)[8 * NT] = s_l + warps;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if (!p.late_wait) pdl_wait();
+  // Launched beside a tile pass, this grid starts when that one's CTAs have all passed their wait, which the acquire
+  // confirms; whatever came before both is then visible here.  If it does not, this grid waits for the tile pass.
+  if (!p.late_wait || !others_waited(p.err)) pdl_wait();
   pdl_launch_dependents();
 
   // ---------------- work item
@@ -603,9 +605,8 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
           make_uint2(pack_f16x2(acc.x * inv, acc.y * inv), pack_f16x2(acc.z * inv, acc.w * inv));
     }
   }
-  // This grid may run beside the pass before it, which has passed its own wait (so all that came before both is
-  // complete) and whose results it neither reads nor writes.  One CTA ends after that pass, so this grid does,
-  // and the merge kernel's wait for this grid covers both.
+  // This grid neither reads nor writes the results of the tile pass beside it.  One CTA ends after that pass, so this
+  // grid does, and the merge kernel's wait for this grid covers both.
   if (p.late_wait && blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 

@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *holder, 0);
   pdl_wait();  // Q, K, V, masks and counts may come from the preceding kernel
+  if (p.publish && blockIdx.x == 0 && threadIdx.x == 0) publish_waited(p.err, 1);
   pdl_launch_dependents();
 
   // the item's key range, read by every role (whole warps)

@@ -53,6 +53,18 @@ __device__ __forceinline__ void record_bad_index(int* err) {
   if (err) *reinterpret_cast<volatile int*>(err + 4) = 1;
 }
 
+// The word 24 bytes after the error word, between a grid that has waited for its predecessors (pdl_wait) and one that
+// runs beside it without a wait of its own: the first publishes with release order, the second reads with acquire
+// order, and so sees all that the first one's wait made visible.  The grid behind both takes it back.
+__device__ __forceinline__ void publish_waited(int* err, int v) {
+  asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(err + 6), "r"(v) : "memory");
+}
+__device__ __forceinline__ bool others_waited(const int* err) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(err + 6) : "memory");
+  return v != 0;
+}
+
 // Wait budget of the plan owning `err` (read when a wait starts spinning, not
 // on the fast path): the word 8 bytes after the error word, 0 = the default.
 __device__ __forceinline__ uint64_t wait_budget_ns(const int* err) {

@@ -507,3 +507,44 @@ def test_decoder_layer(kw):
     heads = [v[n].reshape(b, -1, hq, d).transpose(0, 2, 1, 3) for n in ("X", "enc_k", "enc_v")]
     y, tol = attention(*heads, d ** -0.5, counts=x["count"])
     check(v["Y"], *(a.transpose(0, 2, 1, 3).reshape(b, t, hq * d) for a in (y, tol)), "cross")
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("kw", [dict(batch=80, tokens=1, q_heads=8, prefix=900), dict(batch=40, tokens=2, q_heads=4, prefix=4200),
+                                dict(batch=60, tokens=1, q_heads=8, prefix=700, head_dim=128)])
+def test_passes_side_by_side_read_what_came_before_both(kw, graphs):
+    """Own keys' few-row pass beside the shared past's tile pass, with Q and K from the same run's rotation: the bits of
+    a run of its own, on changing inputs in the same buffers."""
+    require_gpu()
+    import torch
+    wl = W.decoder_layer(**kw)
+    plan = plan_for(wl, attention_mode="flash")
+    op = next(o for o in plan.ops if o.kernel == K.K_ATTENTION_FLASH)
+    assert op.ip[K.AF_PASS_OWN] in (K.AF_PASS_ROWS8, K.AF_PASS_ROWS16) and op.ip[K.AF_PASS_PAST] in (K.AF_PASS_TILES, K.AF_PASS_WIDE)
+    g = infer_types(wl.graph)
+    stages = []
+    for names, ins, outs in (
+            (["Q_norm", "Q_heads", "Q_rope", "K_norm", "K_heads", "K_rope"], ["Q", "K", "pos"], ["Qr", "Kr"]),
+            (["share_k", "share_v", "self"], ["Qr", "Kr", "V", "prefix_k", "prefix_v"], ["S"]),
+            (["tokens", "join", "x_norm"], ["S"], ["X"]), (["cross"], ["X", "enc_k", "enc_v", "count"], ["Y"])):
+        st = B200PlanEmitter(attention_mode="flash").emit_plan(lowering.lower(_stage(g, names, ins, outs)))
+        stages.append((Session(st), ins))
+    xs = [wl.make_inputs(s) for s in range(50, 53)]
+    want = []
+    for x in xs:
+        v = dict(x)
+        for sess, ins in stages:
+            v.update(sess.run({n: v[n] for n in ins}))
+        want.append(v["Y"])
+    sess = Session(plan)
+    sess.set_graphs(graphs)
+    dev = [torch.from_numpy(xs[0][n]).cuda() for n in plan.input_names]
+    y = torch.zeros(plan.output_shapes[0], dtype=torch.float16, device="cuda")
+    for _ in range(4):
+        for x, w in zip(xs, want):
+            for t, n in zip(dev, plan.input_names):
+                t.copy_(torch.from_numpy(x[n]))
+            sess.run_ptrs([t.data_ptr() for t in dev], [y.data_ptr()], stream=torch.cuda.current_stream().cuda_stream or 1)
+            torch.cuda.synchronize()
+            assert np.array_equal(y.cpu().numpy().view(np.uint16), w.view(np.uint16))
+    sess.sync()
