@@ -182,8 +182,6 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *holder, 0);
   pdl_wait();  // Q, K, V, masks and counts may come from the preceding kernel
-  if (p.publish && blockIdx.x == 0 && threadIdx.x == 0) publish_waited(p.err, 1);
-  pdl_launch_dependents();
 
   // the item's key range, read by every role (whole warps)
   auto item_keys = [&](int n, WideKeys& k) -> bool {
@@ -241,6 +239,9 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AW_REGS_OTHER));
   if (warp == 11) {
     // ---------------- key ranges: tiles of the past first, positions count through the tiles (attention_flash.cu)
+    // (not beside the wait above, where it costs registers in the softmax)
+    if (p.publish && blockIdx.x == 0) publish_waited(err, 1);
+    pdl_launch_dependents();
     int nq = 0;  // items of tile B
     for (int n = 0, id = blockIdx.x; id < p.items; ++n, id += gridDim.x) {
       const WideItem w = wide_item(p, id);
