@@ -824,7 +824,8 @@ static int make_tmap_q(CUtensorMap* map, const RowsParams& r, int64_t tokens, in
 
 // Fills what the tile pass needs beside the rows' parameters.
 static int tile_params(TileParams& p, const RowsParams& r, const ItemClass* cls, int first1, int items,
-                       int tile_keys) {
+                       bool wide) {
+  const int tile_keys = wide ? 128 : AFK_N;
   p.cls[0] = cls[0], p.cls[1] = cls[1], p.first1 = first1, p.items = items;
   p.q = r.q, p.o = r.o, p.part_o = r.part_o, p.part_ml = r.part_ml, p.part_ref = r.part_ref;
   p.q_sb = r.q_sb, p.q_sh = r.q_sh, p.q_st = r.q_st, p.o_sb = r.o_sb, p.o_sh = r.o_sh, p.o_st = r.o_st;
@@ -836,9 +837,11 @@ static int tile_params(TileParams& p, const RowsParams& r, const ItemClass* cls,
   p.scale_log2 = r.scale_log2;
   p.err = r.err;
   const int64_t tq = r.TQ.d;
-  p.q_boxes[0] = make_tmap_q(&p.map_q[0], r, tq, r.q_st, r.B, r.q_sb);
-  if (tq == 1 || r.q_sb == tq * r.q_st)
-    p.q_boxes[1] = make_tmap_q(&p.map_q[1], r, r.B * tq, tq == 1 ? r.q_sb : r.q_st, 1, (int64_t)r.B * r.q_sb);
+  if (wide) {  // (the 128-row pass copies its query rows)
+    p.q_boxes[0] = make_tmap_q(&p.map_q[0], r, tq, r.q_st, r.B, r.q_sb);
+    if (tq == 1 || r.q_sb == tq * r.q_st)
+      p.q_boxes[1] = make_tmap_q(&p.map_q[1], r, r.B * tq, tq == 1 ? r.q_sb : r.q_st, 1, (int64_t)r.B * r.q_sb);
+  }
   int rc = make_tmap_kv(&p.map_k[0], r.k, p.D, p.tk, p.HKV, p.B, r.k_st, r.k_sh, r.k_sb, tile_keys);
   if (!rc) rc = make_tmap_kv(&p.map_v[0], r.v, p.DV, p.tk, p.HKV, p.B, r.v_st, r.v_sh, r.v_sb, tile_keys);
   if (p.tp > 0) {
@@ -955,7 +958,7 @@ int launch_attention_flash(const PlanOp& op, void* const* ptrs, const OpState*, 
       TileParams p{};
       const int tile_keys = pass == AF_PASS_WIDE ? 128 : AFK_N;
       if (pass == AF_PASS_WIDE && additive) return 5;  // (never planned)
-      int rc = tile_params(p, r, cls, (int)n1, (int)(n0 + n1), tile_keys);
+      int rc = tile_params(p, r, cls, (int)n1, (int)(n0 + n1), pass == AF_PASS_WIDE);
       p.publish = !together;
       p.drop_keys = (ctx.fault & FAULT_DROP_KEY_TILES) != 0;
       if (rc) return rc;
