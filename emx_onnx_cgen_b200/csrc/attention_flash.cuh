@@ -29,12 +29,18 @@ struct RowId {
 struct SmallDiv {
   uint32_t d, magic;
   __host__ static SmallDiv of(uint32_t d) { return {d, d > 1 ? (uint32_t)((1ull << 32) / d + 1) : 0u}; }
-  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, magic); }
+  __host__ __device__ __forceinline__ int div(int n) const {
+#ifdef __CUDA_ARCH__
+    return d == 1 ? n : (int)__umulhi((uint32_t)n, magic);
+#else
+    return d == 1 ? n : (int)(((unsigned long long)(uint32_t)n * magic) >> 32);
+#endif
+  }
 };
 
 // Row r of a work item's rows: (token, head of the group), tokens slowest, of
 // sequence b, or of every sequence one after the other.
-__device__ __forceinline__ RowId row_of(int r, const SmallDiv& group, const SmallDiv& TQ, int kvh, int b,
+__host__ __device__ __forceinline__ RowId row_of(int r, const SmallDiv& group, const SmallDiv& TQ, int kvh, int b,
                                         bool all_sequences) {
   const int bt = group.div(r), g = r - bt * (int)group.d;
   RowId id;
@@ -91,7 +97,7 @@ struct ItemClass {
 
 // Item `split` of `splits` takes floor(n split / splits) up to the next item's first of n tiles (32-bit: n may be
 // 2^25, splits some hundreds).
-__device__ __forceinline__ int split_start(int n, int split, int splits) {
+__host__ __device__ __forceinline__ int split_start(int n, int split, int splits) {
   const int whole = n / splits;
   return whole * split + (n - whole * splits) * split / splits;
 }
