@@ -10,7 +10,10 @@
 // evaluated online tile by tile: running reference m, sum l and output
 // accumulator are fp32 (TMEM for the latter); the weights are rounded to fp16
 // for the second matrix product (half an fp16 step each, 2^-11 relative: the
-// output type's own step) and the sum adds those same rounded weights.  A row
+// output type's own step; 2^-25 of the reference's weight below 2^-14 of it).
+// This pass's sum adds the rounded weights; the 256-row and the few-row pass
+// add them as they are, which keeps the conversions out of the sum's chain.
+// Either way numerator and sum are within half a step per weight of exact.  A row
 // that sees no key gives 0.  Additive entries are taken relative to a mask
 // reference of the row (attention_flash.cuh) before the score is added, so
 // scores keep their digits beside masks as large as the type's lowest value.

@@ -41,7 +41,7 @@ struct SmallDiv {
 // Row r of a work item's rows: (token, head of the group), tokens slowest, of
 // sequence b, or of every sequence one after the other.
 __host__ __device__ __forceinline__ RowId row_of(int r, const SmallDiv& group, const SmallDiv& TQ, int kvh, int b,
-                                        bool all_sequences) {
+                                                 bool all_sequences) {
   const int bt = group.div(r), g = r - bt * (int)group.d;
   RowId id;
   id.h = kvh * (int)group.d + g;

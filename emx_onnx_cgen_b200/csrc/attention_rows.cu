@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, 1) attention_rows_kernel(const 
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             s[u][n2][2 * h + e] = ex2_approx(s[u][n2][2 * h + e] + neg);
-            l[n2][e] += s[u][n2][2 * h + e];
+            l[n2][e] += s[u][n2][2 * h + e];  // (before the rounding)
           }
         }
 #pragma unroll

@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) attention_wide_kernel(const __g
                 // slots are what is short: [8, 16, 448 x 1500, 64] takes 50.6 us with none, 51.2 and 52.6 us with
                 // an eighth and a quarter.
                 const F2 w2 = NS == 2 && i % 8 == 7 ? ex2_poly(e) : F2(ex2_approx(e.lo()), ex2_approx(e.hi()));
-                sum[i & 1] = add2(sum[i & 1], w2);
+                sum[i & 1] = add2(sum[i & 1], w2);  // (before the rounding)
                 pw[i] = pack_f16x2(w2.lo(), w2.hi());
               }
               tmem_st16(s_col + 16u * q, pw);

@@ -158,3 +158,24 @@ def test_scores_of_keys_hidden_by_an_entry(q_seq, mask):
     want = decoder_attention(wl, x)
     x["K"][:, :, hidden] = np.array([np.inf, np.nan, -np.inf, np.nan, np.inf], np.float16)[:, None]
     check(run(wl, x), *want, str(kw))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q_seq=1, kv_seq=16384), dict(q_seq=9, kv_seq=16384, head_dim=128), dict(q_seq=40, kv_seq=16384),
+    dict(q_seq=300, kv_seq=16384), dict(q_seq=300, kv_seq=16384, head_dim=128),
+])
+@pytest.mark.parametrize("log2", [-14.5, -16.4, -18.6])
+def test_weights_below_fp16s_normal_range(kw, log2):
+    """One key of weight 1 and thousands far below 2^-14, which together matter: each is within half a step of fp16
+    (2^-25 there), whichever of the passes' sums it enters, rounded or not."""
+    require_gpu()
+    kw = dict(batch=1, q_heads=2, kv_heads=2, scale=1.0, **kw)
+    wl = W.decoder_attention(**kw)
+    x = wl.make_inputs(37)
+    x["Q"][:], x["K"][:] = 0, 0
+    x["Q"][..., 0] = 1
+    x["K"][..., 0] = log2 * np.log(2)
+    x["K"][:, :, 700, 0] = 0
+    x["V"][:] = 1 + 0.25 * x["V"]
+    x["V"][:, :, 700] = 0
+    check(run(wl, x), *decoder_attention(wl, x), str(kw))
