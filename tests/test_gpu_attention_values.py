@@ -179,3 +179,66 @@ def test_weights_below_fp16s_normal_range(kw, log2):
     x["V"][:] = 1 + 0.25 * x["V"]
     x["V"][:, :, 700] = 0
     check(run(wl, x), *decoder_attention(wl, x), str(kw))
+
+
+def _marked(t, d, n):
+    """Values [n, t, d] of which each column holds one key's mark, t, so that equal weights 1/t give 1 for a key that
+    counts once, 0 for one that is lost and 2 for one that counts twice; n columns sets share the keys."""
+    v = np.zeros((n, t, d), np.float16)
+    keys = np.arange(n * d) % t if n * d >= t else np.linspace(0, t - 1, n * d).round().astype(int)
+    if n * d < t:  # both sides of the tiles' edges rather than an even grid
+        edge = np.unique(np.concatenate([np.arange(0, t, 64), np.arange(63, t, 64), np.arange(15, t, 16)[:n * d], [0, t - 1]]))
+        keys[:min(len(edge), n * d)] = edge[:n * d]
+    v[np.arange(n * d) // d, keys, np.arange(n * d) % d] = t
+    return v
+
+
+@pytest.mark.parametrize("kw", [
+    dict(batch=1, q_heads=2, kv_heads=2, q_seq=1, kv_seq=5000, head_dim=128),
+    dict(batch=2, q_heads=32, kv_heads=16, q_seq=1, kv_seq=4096, head_dim=128),
+    dict(batch=3, q_heads=16, kv_heads=8, q_seq=3, kv_seq=4104, head_dim=64),
+    dict(batch=1, q_heads=48, kv_heads=24, q_seq=5, kv_seq=3000, head_dim=128),
+    dict(batch=1, q_heads=24, kv_heads=24, q_seq=40, kv_seq=3000, head_dim=128),            # 128-row pass
+    dict(batch=1, q_heads=16, kv_heads=16, q_seq=40, kv_seq=1000, head_dim=64, mask="f16"),
+    dict(batch=2, q_heads=24, kv_heads=12, q_seq=40, kv_seq=2000, head_dim=96, mask="f32"),
+    dict(batch=1, q_heads=32, kv_heads=32, q_seq=300, kv_seq=2000, head_dim=64),            # 256-row pass
+    dict(batch=2, q_heads=16, kv_heads=16, q_seq=150, kv_seq=3000, head_dim=128, mask="bool"),
+    dict(batch=2, q_heads=32, kv_heads=16, q_seq=1, kv_seq=3000, head_dim=128, mask="bool"),
+    dict(batch=3, q_heads=32, kv_heads=16, q_seq=1, kv_seq=24, past=9000, head_dim=128),    # a shared past in ranges
+    dict(batch=128, q_heads=16, kv_heads=16, q_seq=1, kv_seq=300, past=700, head_dim=64),
+    dict(batch=130, q_heads=64, kv_heads=16, q_seq=1, kv_seq=104, past=2000, head_dim=128, mask="bool"),
+    dict(batch=3, q_heads=16, kv_heads=16, q_seq=60, kv_seq=60, past=1940, head_dim=64),
+    dict(batch=2, q_heads=16, kv_heads=16, q_seq=2, kv_seq=40, past=1000, head_dim=64, shared_past=False),
+])
+def test_every_key_of_a_range_counts_once(kw):
+    require_gpu()
+    b, h, past, own, d = kw["batch"], kw["kv_heads"], kw.get("past", 0), kw["kv_seq"], kw["head_dim"]
+    t = past + own
+    assert t % 8 == 0 and t < 16384  # a mark is a whole fp16 number
+    if "mask" in kw:
+        kw = dict(kw, mask_shape=(b, 1, kw["q_seq"], t))
+    wl = W.decoder_attention(**kw)
+    x = wl.make_inputs(36)
+    x["Q"][:] = 0
+    if "mask" in x:
+        x["mask"][:] = x["mask"].dtype == bool
+    shared = past and kw.get("shared_past", True)
+    v = np.zeros((b, h, t, d), np.float16)
+    if shared:  # a sequence marks its own keys in half of the columns, all the past's in the others
+        v[:, :, :past, :d // 2] = _marked(past, d // 2, h) / np.float16(past) * np.float16(t)
+        v[:, :, past:, d // 2:] = (_marked(own, d - d // 2, b * h) / np.float16(own) * np.float16(t)).reshape(b, h, own, -1)
+        x["PV"][:] = v[:1, :, :past]
+        x["V"][:] = v[:, :, past:]
+    else:
+        v[:] = _marked(t, d, b * h).reshape(b, h, t, d)
+        if past:
+            x["PV"][:], x["V"][:] = v[:, :, :past], v[:, :, past:]
+        else:
+            x["V"][:] = v
+    got = run(wl, x).astype(np.float64)
+    want = (v != 0).sum(2, dtype=np.int64)  # [b, h, d]: 0 or 1
+    assert set(np.unique(want)) <= {0, 1} and want.any()
+    want = np.repeat(want, kw["q_heads"] // h, axis=1)[:, :, None]
+    # one mark times an exact weight over an exact sum (whole numbers below 2^24), and the roundings of the division,
+    # the merge's factors of 1 and the result
+    assert np.abs(got - want).max() <= 2.0 ** -10
