@@ -779,6 +779,9 @@ int prepare_attention_flash(const PlanOp& op, void* const*, OpState*, int, char*
     return fail(msg, n, 5, "Attention: head sizes %lld/%lld, needs multiples of 8 up to 128", (long long)d, (long long)dv);
   if (op.ip[AF_K_ST] > 0x7fffffff || op.ip[AF_V_ST] > 0x7fffffff)
     return fail(msg, n, 5, "Attention: key stride of more than 2^31 elements");
+  // (plans from before the references were kept have no room for them)
+  if (op.ip[AF_MASK_KIND] >= AF_MASK_F16 && op.ip[AF_SPLITS_K] + op.ip[AF_SPLITS_P] > 1 && op.ip[AF_PART_WIDTH] < dv + 3)
+    return fail(msg, n, 5, "Attention: split keys under an additive mask, planned for another version of this library; plan it again");
   cudaError_t re = prepare_attention_rows();
   if (re == cudaSuccess) re = prepare_attention_wide();
   if (re != cudaSuccess) return fail(msg, n, 4, "cudaFuncSetAttribute: %s", cudaGetErrorString(re));

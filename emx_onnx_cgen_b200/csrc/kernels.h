@@ -101,8 +101,8 @@ enum {
 enum { ATF_SCALE };
 
 // ---- K_ATTENTION_FLASH: t[0]=Q, t[1]=K, t[2]=V, t[3]=Y (fp16), t[4]=mask|-1, t[5]=past K|-1, t[6]=past V|-1,
-//      t[7]=valid key counts i64 [B]|-1, t[8]=partial results f32|-1 (slots x rows x (DV + 2, or 3 with an additive mask), slots = AF_SPLITS_K +
-//      AF_SPLITS_P, rows = B*TQ*HQ), t[9]=boolean mask as bits (16 bytes per mask row, then 8 per 64 keys of the past
+//      t[7]=valid key counts i64 [B]|-1, t[8]=partial results f32|-1 (slots x rows x AF_PART_WIDTH: DV + 2, with an additive mask
+//      DV + 3; slots = AF_SPLITS_K + AF_SPLITS_P, rows = B*TQ*HQ), t[9]=boolean mask as bits (16 bytes per mask row, then 8 per 64 keys of the past
 //      and of the current keys, each rounded up to 128), or additive mask in tiles of 64 keys (past first)|-1: for the tile passes.  Element (b, h, t, d) of Q, K, V, Y sits at b*SB + h*SH + t*ST + d; the past is contiguous
 //      [B or 1][HKV][TP][D].  Mask row of query (b, h, t): b*SB + h*SH + t*ST, each of AF_MASK_LEN keys, past first.
 enum {
@@ -111,7 +111,8 @@ enum {
   AF_PAST_SHARED /*one past for every sequence*/, AF_PASS_OWN /*pass that runs a sequence's rows on its own keys*/,
   AF_PASS_PAST /*pass of a shared past's items, NONE: the past's keys come first in a sequence's own items*/,
   AF_SPLITS_K, AF_SPLITS_P /*work items along the keys*/, AF_WARPS /*of an item of attention_rows.cu*/, AF_MASK_KIND,
-  AF_MASK_SB, AF_MASK_SH, AF_MASK_ST, AF_MASK_ROWS, AF_MASK_LEN
+  AF_MASK_SB, AF_MASK_SH, AF_MASK_ST, AF_MASK_ROWS, AF_MASK_LEN,
+  AF_PART_WIDTH
 };
 enum { AFF_SCALE };
 enum { AF_PASS_NONE = 0, AF_PASS_ROWS8 = 1, AF_PASS_ROWS16 = 2 /*attention_rows.cu*/, AF_PASS_TILES = 3 /*attention_flash.cu*/,

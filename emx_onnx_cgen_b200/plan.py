@@ -1628,8 +1628,8 @@ class B200PlanEmitter:
                    K.AF_SPLITS_P: sch.splits_past, K.AF_WARPS: sch.warps})
         if sch.slots > 1:
             # output, maximum and sum of a row, and with an additive mask its reference
-            t_part = self._b.arena_tensor(T_TEMP, "f32", (sch.slots, b * tq * hq, dv + 2 + (t_mask >= 0 and kind != K.AF_MASK_BOOL)),
-                                          name="attention:partials")
+            ip[K.AF_PART_WIDTH] = dv + 2 + int(t_mask >= 0 and kind != K.AF_MASK_BOOL)
+            t_part = self._b.arena_tensor(T_TEMP, "f32", (sch.slots, b * tq * hq, ip[K.AF_PART_WIDTH]), name="attention:partials")
         if t_mask >= 0 and not {K.AF_PASS_TILES, K.AF_PASS_WIDE}.isdisjoint((sch.own, sch.past)):
             if kind == K.AF_MASK_BOOL:
                 words = 2 * (-(-tp // (2 * FLASH_KEYS)) + -(-tk // (2 * FLASH_KEYS)))

@@ -62,3 +62,28 @@ def test_a_kernel_that_needs_a_boundary_names_it(make, mode, which, off):
     sess.sync()
     for n, t in zip(plan.output_names, outs):
         assert np.array_equal(t.cpu().numpy(), want[n])
+
+
+def test_a_plan_without_room_for_mask_references_is_refused_when_loaded():
+    """As written before partial results carried them: split keys under an additive mask."""
+    require_gpu()
+    import dataclasses
+    import struct
+
+    from emx_onnx_cgen_b200 import kernel_ids as K
+    for mask, ok in (("f16", False), ("f32", False), ("bool", True)):
+        wl = W.decoder_attention(batch=1, q_heads=2, kv_heads=2, q_seq=3, kv_seq=4000, mask=mask)
+        plan = plan_for(wl, attention_mode="flash")
+        op = plan.ops[-1]
+        assert op.ip[K.AF_SPLITS_K] > 1
+        blob = bytearray(plan.plan_bytes)
+        at = len(blob) - 440 + 8 + 12 * 4 + 8 * K.AF_PART_WIDTH  # the last op's integers
+        assert struct.unpack_from("<q", blob, at)[0] == op.ip[K.AF_PART_WIDTH]
+        struct.pack_into("<q", blob, at, 0)
+        old = dataclasses.replace(plan, plan_bytes=bytes(blob))
+        if ok:
+            Session(old).run(wl.make_inputs(1))
+            continue
+        with pytest.raises(EmxError, match="plan it again") as e:
+            Session(old)
+        assert e.value.status == EMX_ERR_UNSUPPORTED
