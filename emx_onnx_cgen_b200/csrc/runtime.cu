@@ -777,8 +777,13 @@ int emx_b200_sync(emx_plan_t* p) {
   int words[5] = {0, 0, 0, 0, 0};
   CUDA_TRY(cudaMemcpy(words, p->d_error, sizeof(words), cudaMemcpyDeviceToHost), "error word read");
   const int err = words[0], bad_index = words[4];
-  if (err) cudaMemset(p->d_error, 0, sizeof(int));
-  if (bad_index) cudaMemset(p->d_error + 4, 0, sizeof(int));
+  if (err || bad_index) {
+    // cleared before this returns (a memset may outlive its call): the next run must neither see a word of this one
+    // nor lose its own to the clearing
+    CUDA_TRY(cudaMemsetAsync(p->d_error, 0, sizeof(int), p->own_stream), "error word reset");
+    CUDA_TRY(cudaMemsetAsync(p->d_error + 4, 0, sizeof(int), p->own_stream), "error word reset");
+    CUDA_TRY(cudaStreamSynchronize(p->own_stream), "error word reset");
+  }
   if (err) return set_error(EMX_ERR_DEVICE_TIMEOUT, "device-side wait gave up (code %d)", err);
   if (bad_index)
     return set_error(EMX_ERR_INVALID_ARGUMENT, "an input of position ids or valid key counts holds a value out of range");

@@ -73,3 +73,28 @@ def test_positions_out_of_range_leave_the_attention_behind_them_alone():
     others = [0, 1, 2, 4]
     assert np.array_equal(got[others].view(np.uint16), want[others].view(np.uint16))
     assert np.isnan(got[3, 5:]).all() and np.isfinite(got[3, :5]).all()  # tokens behind it see its key
+
+
+def test_a_report_leaves_no_trace_in_the_next_run():
+    """Reports and good runs in turn, back to back on the plan's own stream and on another one: a report is neither
+    repeated nor lost, and no good run gives up on its account."""
+    require_gpu()
+    import torch
+    wl = W.decoder_attention(batch=4, q_heads=8, kv_heads=8, q_seq=200, kv_seq=900, count=True)
+    plan = plan_for(wl, attention_mode="flash")
+    x = wl.make_inputs(44)
+    sess = Session(plan)
+    want = sess.run(x)["Y"]
+    dev = {n: torch.from_numpy(v).cuda() for n, v in x.items()}
+    bad = torch.full((4,), 901, dtype=torch.int64, device="cuda")
+    y = torch.zeros(plan.output_shapes[0], dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    ptrs = {k: [(c if n == "count" else dev[n]).data_ptr() for n in plan.input_names] for k, c in (("bad", bad), ("good", dev["count"]))}
+    for i in range(40):
+        stream = (0, torch.cuda.Stream().cuda_stream)[i % 2]
+        sess.run_ptrs(ptrs["bad"], [y.data_ptr()], stream=stream)
+        with pytest.raises(EmxError, match="out of range"):
+            sess.sync()
+        sess.run_ptrs(ptrs["good"], [y.data_ptr()], stream=stream)
+        sess.sync()
+        assert np.array_equal(y.cpu().numpy().view(np.uint16), want.view(np.uint16))
