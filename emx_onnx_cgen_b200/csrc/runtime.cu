@@ -245,6 +245,9 @@ int prepare_ops(emx_plan* p) {
     int rc = p->entries[i]->prepare(p->ops[i], p->ptrs.data(), &p->states[i], p->device, msg, sizeof(msg));
     if (rc) return set_error(rc, "op %zu (%s): %s", i, p->entries[i]->name, msg);
   }
+  // The arena's zeroes, the weights and what the ops prepared were enqueued on the default stream, which the streams of
+  // runs need not wait for: without this wait a first run's staged inputs could be zeroed behind its back.
+  CUDA_TRY(cudaStreamSynchronize(cudaStreamLegacy), "load");
   return EMX_OK;
 }
 
@@ -822,6 +825,7 @@ int emx_b200_set_wait_budget(emx_plan_t* p, uint64_t ns) {
   const unsigned long long v = ns;
   CUDA_TRY(cudaMemcpy(reinterpret_cast<char*>(p->d_error) + 8, &v, sizeof(v), cudaMemcpyHostToDevice),
            "wait budget");
+  CUDA_TRY(cudaStreamSynchronize(cudaStreamLegacy), "wait budget");
   return EMX_OK;
 }
 
