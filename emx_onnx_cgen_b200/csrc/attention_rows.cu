@@ -9,8 +9,8 @@
 // a block cost a memory latency (1.2 us).  At D <= 64 and up to 8 rows a step
 // takes two blocks: the chain of a step (scores, maximum, exponentials,
 // transposes, output) is 1500 clocks long and two warps a scheduler do not cover
-// it (16 sequences x 16 heads, up to 1500 keys, D = 64: 16.5 us, 4.5 TB/s of
-// valid keys; 20.5 us with one block).  128 sequences x 8 heads of 4 rows, 150
+// it (16 sequences x 16 heads, up to 1500 keys, D = 64: 16.4 to 17.8 us over
+// several boards, 4.2 to 4.5 TB/s of valid keys; 4 us more with one block).  128 sequences x 8 heads of 4 rows, 150
 // keys on average, D = 128: 29 us alone, 3.5 TB/s, a third of the stalls at the
 // CTA's barriers.  The products are mma.sync.m16n8k16:
 // a tcgen05 form needs a 128-row tile, tensor maps, barriers and TMEM set up per
