@@ -89,7 +89,10 @@ def compile_model(model_path, dim_values=None, weights_bin=None, threshold=DEFAU
             model = constants_from_bin(model, Path(weights_bin).read_bytes(), threshold)
         except ValueError as e:
             raise CliError(f"{weights_bin}: {e}") from e
-    return (emitter or B200PlanEmitter()).emit_plan(model)
+    try:
+        return (emitter or B200PlanEmitter()).emit_plan(model)
+    except UnsupportedOpError as e:
+        raise CliError(f"{model_path}: {e}") from e
 
 
 def _load_npz(path) -> dict[str, np.ndarray]:

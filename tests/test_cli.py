@@ -217,3 +217,14 @@ def test_target_flag(tmp_path, capsys):
     assert (tmp_path / "out" / f"{wl.graph.name}.plan").exists()
     with pytest.raises(SystemExit):
         cli.main(["compile", str(model), "--target", "c"])
+
+
+def test_compile_reports_what_the_planner_refuses(tmp_path, capsys):
+    """An operator without a kernel for its form is one line on stderr, not a traceback."""
+    model = tmp_path / "a.onnx"
+    assert cli.main(["export", "decoder_attention", str(model), "--param", "mask=bool"]) == 0
+    capsys.readouterr()
+    assert cli.main(["compile", str(model), "-o", str(tmp_path / "out")]) == 2
+    err = capsys.readouterr().err
+    assert err.startswith("error: ") and "masks" in err and "exact mode" in err and err.count("\n") == 1
+    assert cli.main(["compile", str(model), "-o", str(tmp_path / "out"), "--attention-mode", "flash"]) == 0
