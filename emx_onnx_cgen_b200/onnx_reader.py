@@ -387,7 +387,12 @@ def infer_types(spec: GraphSpec) -> GraphSpec:
         elif op in ("RMSNormalization", "RotaryEmbedding"):
             res = [(x.dtype, x.shape)]
         elif op == "Expand":
-            res = [(x.dtype, _broadcast(x.shape, [int(v) for v in np.asarray(spec.initializers[ins[1]]).reshape(-1)]))]
+            if ins[1] not in spec.initializers:
+                raise OnnxFormatError(f"Expand: shape {ins[1]} must be an initializer")
+            try:
+                res = [(x.dtype, _broadcast(x.shape, [int(v) for v in np.asarray(spec.initializers[ins[1]]).reshape(-1)]))]
+            except ValueError as e:
+                raise OnnxFormatError(f"Expand: {tuple(x.shape)} to the shape in {ins[1]}: {e}") from e
         elif op == "Attention":
             v = t(ins[2])
             heads = int(a.get("kv_num_heads", 0)) if len(v.shape) == 3 else v.shape[1]

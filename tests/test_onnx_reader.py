@@ -105,3 +105,14 @@ def test_reference_fixture_lowers(name):
     model, lowered = refc.lower(g)
     assert len(lowered.ops) >= len(g.nodes) - 2  # the reference may fold reshapes
     assert tuple(lowered.output_shapes[0]) == (1, 10)
+
+
+@pytest.mark.parametrize("inits,match", [({}, "initializer"), ({"s": np.array([2, 4], np.int64)}, "Expand")])
+def test_expand_to_a_shape_that_cannot_be_had(inits, match):
+    """A shape computed at run time, or one the input does not broadcast to."""
+    from emx_onnx_cgen_b200.spec import GraphSpec, NodeSpec, TensorSpec
+    ins = [TensorSpec("X", "f16", (1, 3))] + ([] if inits else [TensorSpec("s", "i64", (2,))])
+    g = GraphSpec("e", ins, [TensorSpec("Y", "f16", (2, 3))],
+                  [NodeSpec("Expand", "e", ("X", "s"), ("Z",)), NodeSpec("Relu", "r", ("Z",), ("Y",))], inits)
+    with pytest.raises(OnnxFormatError, match=match):
+        infer_types(g)
