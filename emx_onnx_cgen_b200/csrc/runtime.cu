@@ -699,21 +699,23 @@ int emx_b200_run(emx_plan_t* p, const void* const* inputs, void* const* outputs,
   cudaStream_t stream = stream_ ? static_cast<cudaStream_t>(stream_) : p->own_stream;
   p->last_stream = stream;
   p->pending.clear();
+  // (a tensor without elements has no buffer to point to)
   for (size_t i = 0; i < p->inputs.size(); ++i)
-    if (!inputs[i]) return set_error(EMX_ERR_INVALID_ARGUMENT, "input %zu is NULL", i);
+    if (!inputs[i] && p->tensors[p->inputs[i]].nbytes)
+      return set_error(EMX_ERR_INVALID_ARGUMENT, "input %zu is NULL", i);
   for (size_t i = 0; i < p->outputs.size(); ++i)
-    if (!outputs[i]) return set_error(EMX_ERR_INVALID_ARGUMENT, "output %zu is NULL", i);
+    if (!outputs[i] && p->tensors[p->outputs[i]].nbytes)
+      return set_error(EMX_ERR_INVALID_ARGUMENT, "output %zu is NULL", i);
   p->in_kind.resize(p->inputs.size());
   p->out_kind.resize(p->outputs.size());
-  for (size_t i = 0; i < p->inputs.size(); ++i) p->in_kind[i] = mem_kind(inputs[i]);
-  for (size_t i = 0; i < p->outputs.size(); ++i) p->out_kind[i] = mem_kind(outputs[i]);
+  for (size_t i = 0; i < p->inputs.size(); ++i) p->in_kind[i] = inputs[i] ? mem_kind(inputs[i]) : MEM_DEVICE;
+  for (size_t i = 0; i < p->outputs.size(); ++i) p->out_kind[i] = outputs[i] ? mem_kind(outputs[i]) : MEM_DEVICE;
   if (can_overlap(p)) return run_overlapped(p, inputs, outputs, batch_begin, batch_count, stream);
   if (full > 0 && can_pipeline(p, batch_count))
     return run_pipelined(p, inputs, outputs, batch_begin, batch_count, stream);
   for (size_t i = 0; i < p->inputs.size(); ++i) {
     const PlanTensor& t = p->tensors[p->inputs[i]];
     const void* src = inputs[i];
-    if (!src) return set_error(EMX_ERR_INVALID_ARGUMENT, "input %zu is NULL", i);
     size_t off = 0, bytes = t.nbytes;
     if (full > 0 && t.batch_axis == 0) {
       off = (size_t)batch_begin * row_bytes(t);
@@ -731,7 +733,6 @@ int emx_b200_run(emx_plan_t* p, const void* const* inputs, void* const* outputs,
   for (size_t i = 0; i < p->outputs.size(); ++i) {
     const PlanTensor& t = p->tensors[p->outputs[i]];
     void* dst = outputs[i];
-    if (!dst) return set_error(EMX_ERR_INVALID_ARGUMENT, "output %zu is NULL", i);
     size_t off = 0, bytes = t.nbytes;
     if (full > 0 && t.batch_axis == 0) {
       off = (size_t)batch_begin * row_bytes(t);

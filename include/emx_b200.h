@@ -74,7 +74,8 @@ int emx_b200_plan_load_mem(const void *plan, size_t plan_len, const void *weight
 
 /* Run the plan.  inputs[i]/outputs[i] follow the graph's input/output order
  * (the parameter order of the generated `<model>(...)`, c_emitter.py:2297)
- * and may be host or device pointers (detected per pointer).  Host buffers
+ * and may be host or device pointers (detected per pointer; NULL for a tensor
+ * without elements).  Host buffers
  * are staged through the arena with cudaMemcpyAsync on `stream`; when every
  * host buffer is page-locked (cudaHostAlloc / cudaHostRegister), at least
  * 1 MiB crosses the bus, the plan is batchable on axis 0 and the run has two

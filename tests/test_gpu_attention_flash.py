@@ -548,3 +548,33 @@ def test_passes_side_by_side_read_what_came_before_both(kw, graphs):
             torch.cuda.synchronize()
             assert np.array_equal(y.cpu().numpy().view(np.uint16), w.view(np.uint16))
     sess.sync()
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_empty_past_on_the_device(shared):
+    """A first step's past of no tokens: its device tensors have no address."""
+    require_gpu()
+    import torch
+    kw = dict(batch=2, q_heads=4, kv_heads=2, q_seq=5, kv_seq=5, causal=True)
+    wl = W.decoder_attention(**kw, past=16, shared_past=shared)
+    g = wl.graph
+    for n in ("PK", "PV"):
+        i = next(k for k, t in enumerate(g.inputs) if t.name == n)
+        g.inputs[i] = TensorSpec(n, "f16", (1 if shared else 2, 2, 0, 64))
+        if shared:
+            g.initializers[n + "_shape"] = np.array([2, 2, 0, 64], np.int64)
+    g.values.clear()
+    plan = plan_for(wl, attention_mode="flash")
+    plain = W.decoder_attention(**kw)
+    x = plain.make_inputs(3)
+    dev = {n: torch.from_numpy(x[n]).cuda() for n in "QKV"}
+    dev.update({n: torch.empty(0, dtype=torch.float16, device="cuda") for n in ("PK", "PV")})
+    assert dev["PK"].data_ptr() == 0
+    y = torch.zeros(plan.output_shapes[0], dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    sess = Session(plan)
+    sess.run_ptrs([dev[n].data_ptr() for n in plan.input_names], [y.data_ptr()])
+    sess.sync()
+    check(y.cpu().numpy(), *decoder_attention(plain, x), str(kw))
+    with pytest.raises(EmxError, match="NULL"):
+        sess.run_ptrs([0 if n == "K" else dev[n].data_ptr() for n in plan.input_names], [y.data_ptr()])
