@@ -43,7 +43,7 @@
 // row and tile in registers, an exponential each), then, for short keys, the
 // set-up of a work item (TMEM, barriers, Q: some 5 us).  [57, 16, 45 x 2952, 96]
 // with an fp16 additive mask: 211 us, 221 TFLOP/s; [3, 12, 77 x 333, 80]: 16.4
-// us, three launches.
+// to 17.1 us, three launches.
 //
 // Boolean masks are first packed by mask_pack_kernel to one 64-bit word per
 // (mask row, 64 keys) plus each row's first and last visible key, so a row's

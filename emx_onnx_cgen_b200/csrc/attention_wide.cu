@@ -26,12 +26,12 @@
 // fp32 instructions.  Every wait is bounded (tc100.cuh).
 //
 // Measured: 4 x 32 heads of 128, 2048 rows, 2048-4096 of 4096 keys (8 key/value
-// heads): 418 to 443 us over several boards, 0.93 to 0.99 PFLOP/s, 67 to 71 % of
+// heads): 418 to 459 us over several boards, 0.90 to 0.99 PFLOP/s, 64 to 71 % of
 // what a library product sustains at the board's power limit.  Two row tiles' step takes 3000 clocks, of which the
 // products need 2050; a tile's own chain (products, TMEM load 120, maximum 350,
 // exponentials 1150) is 2100, and the other tile's softmax shares its issue
 // slots.  At D = 64 (8 x 16 heads, 448 x up to 1500) the step is as long: 49.3 to
-// 51.9 us.
+// 52.3 us.
 #include <cuda_fp16.h>
 
 #include "attention_flash.cuh"
