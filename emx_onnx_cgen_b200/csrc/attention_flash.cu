@@ -13,8 +13,8 @@
 // output type's own step; 2^-25 of the reference's weight below 2^-14 of it).
 // This pass's sum adds the rounded weights; the 256-row and the few-row pass
 // add them as they are, which keeps the conversions out of the sum's chain.
-// Either way numerator and sum are within half a step per weight of exact.  A row
-// that sees no key gives 0.  Additive entries are taken relative to a mask
+// Either way numerator and sum are within half a step per weight of exact.  A
+// row that sees no key gives 0.  Additive entries are taken relative to a mask
 // reference of the row (attention_flash.cuh) before the score is added, so
 // scores keep their digits beside masks as large as the type's lowest value.
 //
@@ -720,9 +720,9 @@ __global__ void __launch_bounds__(256) mask_pack_kernel(const uint8_t* __restric
 
 // ------------------------------------------------------------------ whole tiles of additive masks
 // y[tile][16-byte piece][row]: the past's tiles, then the current keys', -inf past the mask's length and each part's
-// keys.  A row's thread reads its row of a tile 16 bytes at a time: straight
-// from the mask, 32 rows' pieces are 32 sectors of 32 rows ([57, 16, 45 x 2952, 96] with a mask row per query took
-// 810 us so); from here they are 512 bytes in line.  A CTA copies 32 rows of a tile through shared memory.
+// keys.  A row's thread reads its row of a tile 16 bytes at a time: straight from the mask, 32 rows' pieces are 32
+// sectors of 32 rows ([57, 16, 45 x 2952, 96] with a mask row per query took 810 us so); from here they are 512 bytes in
+// line.  A CTA copies 32 rows of a tile through shared memory.
 template <typename T>
 __global__ void __launch_bounds__(256) mask_tiles_kernel(const T* __restrict__ mask, int len, int past, int keys, int words1,
                                                          int words, int64_t rows, uint4* __restrict__ y) {

@@ -10,11 +10,12 @@
 // takes two blocks: the chain of a step (scores, maximum, exponentials,
 // transposes, output) is 1500 clocks long and two warps a scheduler do not cover
 // it (16 sequences x 16 heads, up to 1500 keys, D = 64: 16.4 to 17.8 us over
-// several boards, 4.2 to 4.5 TB/s of valid keys; 4 us more with one block).  128 sequences x 8 heads of 4 rows, 150
-// keys on average, D = 128: 29 us alone, 3.5 TB/s, a third of the stalls at the
-// CTA's barriers.  The products are mma.sync.m16n8k16:
-// a tcgen05 form needs a 128-row tile, tensor maps, barriers and TMEM set up per
-// work item, and at these sizes a work item is over before that has paid off.
+// several boards, 4.2 to 4.5 TB/s of valid keys; 4 us more with one block).  128
+// sequences x 8 heads of 4 rows, 150 keys on average, D = 128: 29 us alone, 3.5
+// TB/s, a third of the stalls at the CTA's barriers.  The products are
+// mma.sync.m16n8k16: a tcgen05 form needs a 128-row tile, tensor maps, barriers
+// and TMEM set up per work item, and at these sizes a work item is over before
+// that has paid off.
 // Both products run transposed,
 //   S^T [16 keys x 8 rows] = K Q^T,   O^T [16 d x 8 rows] += V^T P^T,
 // so the row tiles are 8 wide and the big operands are the A side:
